@@ -369,6 +369,67 @@ B200_API int b200_rope_kv_cache_update_f32(const int64_t* d_position, const floa
                                            float* d_k_cache, float* d_v_cache, void* d_zero_ws, void* stream);
 B200_API int b200_widen_i32_to_i64(const int32_t* d_in, int64_t* d_out, int n, void* stream);
 
+/* ---- key/value cache in 4 bits ----------------------------------------------------
+ * No counterpart in the reference, whose caches are float32 (odml.update_kv_cache,
+ * tflite/experimental/genai/kvcache.cc:230-340): half the bytes of an int8 cache for a
+ * decode step that is bound by them. Keys and values each are two tensors, token-major
+ * like the other caches here:
+ *   nibbles uint8 [b, s_max, nkv, h / 2], channel 2 i in the low half of byte i (the order
+ *           of b200_pack_w4's elements), on a 16-byte boundary;
+ *   pairs   fp16 [b, s_max, nkv, h / block, 2]: scale and least value of each block of 32
+ *           or 64 channels; nibble u stands for scale * u + least. On a 4-byte boundary.
+ * h is a multiple of the block, at most 512. All calls: b = 0 or no tokens do nothing. */
+B200_API const char* b200_kv4_last_error(void);
+
+/* Quantizes t tokens per sequence and stores them: token i of sequence b goes to slot
+ * d_positions[b] + i; slots outside 0 .. s_max - 1 and tokens i >= d_counts[b] (optional:
+ * a padded batch) are left alone. d_k / d_v [b, t, nkv, h] f16 or f32 with heads and
+ * channels contiguous and strides (in elements) between sequences and tokens, so that
+ * they may be slices of a fused projection's output. Per block: least = fp16(min), scale =
+ * fp16((max - least) / 15) with difference and quotient rounded to float32, u = the integer
+ * nearest to (x - least) / scale (exactly decided, ties to even), clamped to 0 .. 15. A block
+ * that holds an infinity or NaN reads back as NaN. */
+B200_API int b200_kv4_append(const void* d_k, const void* d_v, int dtype, long long k_batch_stride, long long k_token_stride,
+                             long long v_batch_stride, long long v_token_stride, const int32_t* d_positions,
+                             const int32_t* d_counts, int b, int t, int nkv, int h, int block, int s_max, void* d_k_cache,
+                             void* d_v_cache, void* d_k_scale, void* d_v_scale, void* stream);
+
+/* The values of slots d_positions[b] (NULL: 0) .. + t - 1 as f16 or f32 rows [b, t, nkv, h]
+ * (on 16-byte boundaries): what a prompt chunk's attention (b200_sdpa_rows) reads. Slots
+ * outside the cache and rows i >= d_counts[b] (optional) are zeros. */
+B200_API int b200_kv4_read(const void* d_k_cache, const void* d_v_cache, const void* d_k_scale, const void* d_v_scale, int b,
+                           int s_max, int nkv, int h, int block, const int32_t* d_positions, const int32_t* d_counts, int t,
+                           int dtype, void* d_k, void* d_v, void* stream);
+
+/* odml.scaled_dot_product_attention (tflite/experimental/genai/sdpa.cc:361-662) over the cache:
+ * q / out [b, t, n, h] (f16 or f32); the t query tokens are the last t cached tokens, query i
+ * attends over all of the first d_lengths[b] (optional: s_max) slots but the last t - 1 - i.
+ * d_mask [b, 1, t, s_max] (optional) is added; a slot whose mask is -inf contributes nothing,
+ * whatever it holds. A row without a slot is zero. scale (0: 1 / sqrt(h)) and logit_cap (0:
+ * none) as in b200_sdpa_decode, never negative.
+ * d_scores [b, nkv, s_max] f32 (optional): += the softmax weights that each slot got from its KV
+ * head's n / nkv * t queries (what b200_kv4_evict ranks by); slots beyond the length are left
+ * alone. Any number of query heads per KV head. Workspace: on a 16-byte boundary, no initial
+ * contents. */
+B200_API size_t b200_kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int block, int s_max, int with_scores);
+B200_API int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache, const void* d_k_scale,
+                           const void* d_v_scale, const int32_t* d_lengths, const float* d_mask, float* d_scores, void* d_out,
+                           int b, int t, int n, int nkv, int h, int block, int s_max, int q_dtype, float scale,
+                           float logit_cap, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight: of each KV head of a sequence with more than `budget`
+ * cached tokens stay the first `sinks`, the last `recent` and, of the others, those with the largest
+ * d_scores [b, nkv, s_max] (ties: the lower slot; NaN ranks lowest), `budget` in all. The kept rows go,
+ * in their order, to slots 0 .. of the cache d_*_to [b, s_to, nkv, ...]: the same four tensors (in
+ * place), or others that do not overlap them. Shorter sequences keep everything. d_kept [b, nkv,
+ * budget] receives the kept slots, then -1; d_scores_out [b, nkv, s_to] their scores, then zeros;
+ * d_lengths_out [b] the new lengths (none of the three may overlap its input). Rows of the cache behind
+ * the kept ones are left as they were. */
+B200_API int b200_kv4_evict(void* d_k_cache, void* d_v_cache, void* d_k_scale, void* d_v_scale, int b, int s_max, int nkv,
+                            int h, int block, const float* d_scores, const int32_t* d_lengths, int budget, int sinks,
+                            int recent, void* d_k_to, void* d_v_to, void* d_k_scale_to, void* d_v_scale_to, int s_to,
+                            int32_t* d_kept, float* d_scores_out, int32_t* d_lengths_out, void* stream);
+
 /* ---- Gemma-shaped decoder, one decode step per call ---------------------------
  * A resident decoder for the decode benchmark: every projection is a dynamic-range
  * hybrid FULLY_CONNECTED (b200_fc_hybrid semantics: per-row asymmetric input

@@ -13,6 +13,7 @@ _i = ctypes.c_int
 _i32 = ctypes.c_int32
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
+_ll = ctypes.c_longlong
 
 # name -> (restype, argtypes); mirrors include/litert_b200.h one to one
 SIGNATURES = {
@@ -73,6 +74,14 @@ SIGNATURES = {
     "b200_rope_f32": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "b200_rope_kv_cache_update_f32": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "b200_widen_i32_to_i64": (_i, [_vp, _vp, _i, _vp]),
+    "b200_kv4_last_error": (ctypes.c_char_p, []),
+    "b200_kv4_append": (_i, [_vp, _vp, _i, _ll, _ll, _ll, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "b200_kv4_read": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "b200_kv4_sdpa_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "b200_kv4_sdpa": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _sz,
+                           _vp]),
+    "b200_kv4_evict": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp,
+                            _vp, _vp]),
     "b200_decoder_create": (_i, [_vp, _vp, ctypes.POINTER(_vp)]),
     "b200_decoder_destroy": (None, [_vp]),
     "b200_decoder_set_layer": (_i, [_vp, _i, _vp]),

@@ -56,7 +56,9 @@ class Workspace:
         return self.scratch
 
     def sdpa_for(self, b, n, nkv, h, s_max):
-        need = _lib.load().b200_sdpa_workspace_bytes(b, n, nkv, h, s_max)
+        return self.sdpa_bytes(_lib.load().b200_sdpa_workspace_bytes(b, n, nkv, h, s_max))
+
+    def sdpa_bytes(self, need):
         if self.sdpa is None or self.sdpa.numel() < need:
             self.sdpa = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self.sdpa
@@ -385,3 +387,154 @@ def lm_head_greedy(rows, weights, filter_scales, soft_cap=0.0, want_logits=False
                                     _ptr(weights.packed), weights.n, _ptr(weights.row_sums), _ptr(fs), float(soft_cap),
                                     _ptr(logits), _ptr(tokens), _ptr(wsb), need, _ptr(ws.zero), _stream()))
     return tokens, logits
+
+
+# ---- key/value cache in 4 bits (include/litert_b200.h) -----------------------------------------------------
+def _kcheck(rc):
+    if rc != 0:
+        raise B200Error(f"litert_b200 error {rc}: {_lib.load().b200_kv4_last_error().decode()}")
+
+
+def int4_kv_cache(b, s_max, nkv, h, block=64, device="cuda"):
+    """An empty cache for b sequences of up to s_max tokens: (k_cache, v_cache, k_scale, v_scale), nibbles uint8
+    [b, s_max, nkv, h / 2] (channel 2 i in the low half of byte i) and pairs (scale, least value) float16
+    [b, s_max, nkv, h / block, 2], block 32 or 64 channels."""
+    if block not in (32, 64) or h % block or not 0 < h <= 512:
+        raise B200Error("blocks of 32 or 64 channels that divide a head size up to 512")
+    nibbles = [torch.zeros((b, s_max, nkv, h // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+    pairs = [torch.zeros((b, s_max, nkv, h // block, 2), dtype=torch.float16, device=device) for _ in range(2)]
+    return (*nibbles, *pairs)
+
+
+def _int4_cache(k_cache, v_cache, k_scale, v_scale):
+    """Checks a cache's tensors; returns (b, s_max, nkv, h, block). They are written in place or read where they lie, so
+    nothing is converted."""
+    for t, dtype, dims, name in ((k_cache, torch.uint8, 4, "k_cache"), (v_cache, torch.uint8, 4, "v_cache"),
+                                 (k_scale, torch.float16, 5, "k_scale"), (v_scale, torch.float16, 5, "v_scale")):
+        if _need(t, dtype, name) is None or t.dim() != dims or not t.is_contiguous():
+            raise B200Error(f"{name} must be a contiguous tensor of {dims} dimensions")
+        if t.device != k_cache.device:
+            raise B200Error("the cache's tensors must be on one device")
+    b, s_max, nkv, half = k_cache.shape
+    groups = k_scale.shape[3]
+    if v_cache.shape != k_cache.shape or v_scale.shape != k_scale.shape or k_scale.shape[:3] != k_cache.shape[:3] \
+            or k_scale.shape[4] != 2 or groups == 0 or 2 * half % groups:
+        raise B200Error("the cache's tensors do not belong together")
+    return b, s_max, nkv, 2 * half, 2 * half // groups
+
+
+def _per_sequence(t, b, like, name):
+    """int32 [b] or None."""
+    t = _need(t, torch.int32, name)
+    if t is not None and (t.numel() != b or t.device != like.device):
+        raise B200Error(f"{name} must hold one entry per sequence, on the cache's device")
+    return t
+
+
+def kv_append_int4(k, v, positions, k_cache, v_cache, k_scale, v_scale, counts=None):
+    """Quantizes k and v [b, t, nkv, h] (float16 or float32; slices of a fused projection are read where they lie) and
+    stores token i of sequence b in slot positions[b] + i of the cache. Slots outside the cache and tokens
+    i >= counts[b] (a padded batch) are left alone."""
+    b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
+    if k.dtype not in (torch.float16, torch.float32):
+        raise B200Error("kv_append_int4 takes float16 or float32 rows")
+    rows = []
+    for x, name in ((k, "k"), (v, "v")):
+        if not x.is_cuda or x.device != k_cache.device or x.dtype != k.dtype:
+            raise B200Error(f"{name} must be on the cache's device and of k's type")
+        if x.dim() != 4 or x.shape[0] != b or x.shape[2:] != (nkv, h) or x.shape[1] != k.shape[1]:
+            raise B200Error(f"{name} must be [b, t, nkv, h] of the cache")
+        rows.append(x if x.stride(3) == 1 and (nkv == 1 or x.stride(2) == h) else x.contiguous())
+    positions = _per_sequence(positions, b, k_cache, "positions")
+    counts = _per_sequence(counts, b, k_cache, "counts")
+    if positions is None:
+        raise B200Error("positions are needed")
+    k, v = rows
+    with torch.cuda.device(k_cache.device):
+        _kcheck(_lib.load().b200_kv4_append(_ptr(k), _ptr(v), _DT[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                            _ptr(positions), _ptr(counts), b, k.shape[1], nkv, h, block, s_max, _ptr(k_cache),
+                                            _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _stream()))
+
+
+def kv_read_int4(k_cache, v_cache, k_scale, v_scale, tokens=None, positions=None, counts=None, dtype=torch.float16):
+    """The values of slots positions[b] (default 0) .. + tokens - 1 (default: the cache's length) as two tensors
+    [b, tokens, nkv, h]: what a prompt chunk's attention (sdpa_rows) reads. Slots outside the cache and rows
+    i >= counts[b] are zeros."""
+    b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
+    if dtype not in (torch.float16, torch.float32):
+        raise B200Error("kv_read_int4 gives float16 or float32 rows")
+    tokens = s_max if tokens is None else int(tokens)
+    if tokens < 0:
+        raise B200Error("tokens must not be negative")
+    positions = _per_sequence(positions, b, k_cache, "positions")
+    counts = _per_sequence(counts, b, k_cache, "counts")
+    k, v = (torch.empty((b, tokens, nkv, h), dtype=dtype, device=k_cache.device) for _ in range(2))
+    with torch.cuda.device(k_cache.device):
+        _kcheck(_lib.load().b200_kv4_read(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), b, s_max, nkv, h, block,
+                                          _ptr(positions), _ptr(counts), tokens, _DT[dtype], _ptr(k), _ptr(v), _stream()))
+    return k, v
+
+
+def sdpa_decode_int4(q, k_cache, v_cache, k_scale, v_scale, lengths=None, mask=None, scale=None, logit_cap=0.0, scores=None,
+                     ws=None):
+    """odml.scaled_dot_product_attention (tflite/experimental/genai/sdpa.cc:361-662) over a cache in 4 bits. q
+    [b, t, n, h] (float16 or float32): the t query tokens are the last t of the first lengths[b] cached ones, and query i
+    attends over all of these but the last t - 1 - i. mask float32 [b, 1, t, s_max] is added; -inf hides a slot whatever
+    it holds. scores float32 [b, nkv, s_max], where given, grows by the softmax weights that every slot got from the
+    queries of its KV head (kv_evict_int4 ranks by it)."""
+    b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
+    if q.dtype not in (torch.float16, torch.float32) or not q.is_cuda or q.device != k_cache.device:
+        raise B200Error("q must be float16 or float32, on the cache's device")
+    if q.dim() != 4 or q.shape[0] != b or q.shape[3] != h or q.shape[1] == 0 or q.shape[2] == 0 or q.shape[2] % nkv:
+        raise B200Error("q must be [b, t, n, h] of the cache, n a multiple of its KV heads")
+    q = q.contiguous()
+    t, n = q.shape[1], q.shape[2]
+    lengths = _per_sequence(lengths, b, k_cache, "lengths")
+    mask = _need(mask, torch.float32, "mask")
+    if mask is not None and (tuple(mask.shape) != (b, 1, t, s_max) or mask.device != q.device):
+        raise B200Error("mask must be [b, 1, t, s_max], on the cache's device")
+    if _need(scores, torch.float32, "scores") is not None and \
+            (tuple(scores.shape) != (b, nkv, s_max) or not scores.is_contiguous() or scores.device != q.device):
+        raise B200Error("scores must be contiguous [b, nkv, s_max], on the cache's device")
+    out = torch.empty_like(q)
+    lib = _lib.load()
+    need = lib.b200_kv4_sdpa_workspace_bytes(b, t, n, nkv, h, block, s_max, int(scores is not None))
+    with torch.cuda.device(q.device):
+        wsb = torch.empty(need, dtype=torch.uint8, device=q.device) if ws is None else ws.sdpa_bytes(need)
+        _kcheck(lib.b200_kv4_sdpa(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(lengths), _ptr(mask),
+                                  _ptr(scores), _ptr(out), b, t, n, nkv, h, block, s_max, _DT[q.dtype],
+                                  float(scale) if scale else 0.0, float(logit_cap), _ptr(wsb), wsb.numel(), _stream()))
+    return out
+
+
+def kv_evict_int4(k_cache, v_cache, k_scale, v_scale, scores, lengths, budget, sinks=0, recent=0, into=None):
+    """Cuts every sequence with more than `budget` cached tokens down to that many per KV head: the first `sinks` slots, the
+    last `recent`, and those of the largest scores [b, nkv, s_max] (ties: the lower slot). The kept rows move, in their
+    order, to the first slots of the cache itself, or of the cache `into` (the four tensors of another one with at least
+    `budget` slots). Returns (kept int32 [b, nkv, budget], -1 behind the last; scores [b, nkv, slots of the
+    destination], zeros behind; lengths int32 [b]): what the next steps go on with."""
+    b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
+    to = (k_cache, v_cache, k_scale, v_scale) if into is None else tuple(into)
+    if len(to) != 4:
+        raise B200Error("into must be the four tensors of a cache")
+    b_to, s_to, nkv_to, h_to, block_to = _int4_cache(*to)
+    if (b_to, nkv_to, h_to, block_to) != (b, nkv, h, block) or to[0].device != k_cache.device:
+        raise B200Error("into must be a cache of the same sequences, heads and blocks, on the same device")
+    scores = _need(scores, torch.float32, "scores")
+    if scores is None or tuple(scores.shape) != (b, nkv, s_max) or scores.device != k_cache.device:
+        raise B200Error("scores must be [b, nkv, s_max], on the cache's device")
+    lengths = _per_sequence(lengths, b, k_cache, "lengths")
+    if lengths is None:
+        raise B200Error("lengths are needed")
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if not (budget > 0 and sinks >= 0 and recent >= 0 and sinks + recent <= budget <= s_to):
+        raise B200Error(f"budget {budget} has to hold sinks {sinks} and recent {recent} and fit into {s_to} slots")
+    device = k_cache.device
+    kept = torch.empty((b, nkv, budget), dtype=torch.int32, device=device)
+    scores_out = torch.empty((b, nkv, s_to), dtype=torch.float32, device=device)
+    lengths_out = torch.empty(b, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        _kcheck(_lib.load().b200_kv4_evict(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), b, s_max, nkv, h, block,
+                                           _ptr(scores), _ptr(lengths), budget, sinks, recent, *(_ptr(x) for x in to), s_to,
+                                           _ptr(kept), _ptr(scores_out), _ptr(lengths_out), _stream()))
+    return kept, scores_out, lengths_out
