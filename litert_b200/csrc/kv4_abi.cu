@@ -138,7 +138,7 @@ int b200_kv4_evict(void* d_k_cache, void* d_v_cache, void* d_k_scale, void* d_v_
 
 size_t b200_kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int block, int s_max, int with_scores) {
   if (b <= 0 || t <= 0 || n <= 0 || nkv <= 0 || h <= 0 || s_max <= 0 || block <= 0) return 0;
-  return b200::kv4_sdpa_workspace_bytes(b, t, n, nkv, h, s_max, block, with_scores);
+  return b200::kv4_sdpa_workspace_bytes(b, t, n, nkv, h, s_max, with_scores);
 }
 
 int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache, const void* d_k_scale, const void* d_v_scale,
@@ -153,7 +153,7 @@ int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache,
   if (!(logit_cap >= 0.0f) || !(scale >= 0.0f)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: scale and logit cap are positive, or 0", name);
   if (b == 0) return B200_OK;
   if (!d_q || !d_out) return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
-  const size_t need = b200::kv4_sdpa_workspace_bytes(b, t, n, nkv, h, s_max, block, d_scores != nullptr);
+  const size_t need = b200::kv4_sdpa_workspace_bytes(b, t, n, nkv, h, s_max, d_scores != nullptr);
   if (!d_workspace || workspace_bytes < need || !aligned(d_workspace, 16))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes on a 16-byte boundary needed (b200_kv4_sdpa_workspace_bytes), got %zu", name,
                 need, workspace_bytes);

@@ -11,6 +11,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.h"
+#include "pieces.cuh"
 
 namespace b200 {
 
@@ -146,13 +147,752 @@ cudaError_t launch_rows(const Kv4Sdpa& p, cudaStream_t s) {
                         dim3(kRowsThreads), 0, s, p);
 }
 
-}  // namespace
+// ---- head sizes 64, 128 and 256: tensor cores -------------------------------------------------------------
+// Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; 16 slots are a
+// tile. A warp works on tiles of its own from the first copy to the last product, with its own running maximum, sum and
+// outputs: no barrier until the warps of a CTA merge at the end of a piece. (pieces.cuh: how the slots are cut.)
+template <int H, int BLOCK>
+struct Kv4Tile {
+  static constexpr int kG = H / BLOCK;                // blocks of a row
+  static constexpr int kNibbleBytes = kUnit * H / 2;  // of the keys (or values) of a tile
+  static constexpr int kPairBytes = kUnit * kG * 4;
+  static constexpr int kBytes = 2 * (kNibbleBytes + kPairBytes);
+  static constexpr int kWarps = H == 256 ? 8 : 16;
+  static constexpr int kStages = H == 64 ? 8 : 4;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kRec = H + 4;  // floats of a record per row: outputs, maximum, sum, padding
+  static constexpr int kRing = kWarps * kStages * kBytes;
+  static constexpr int kMerge = kWarps * 8 * kRec * 4;
+  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + 128;
+  static_assert(kBytes % 128 == 0 && kSmem <= 224 * 1024, "layout");
+};
 
-size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int block, int scores) {
-  const size_t rows = (size_t)b * t * n;
-  return (2 * rows + rows * s) * sizeof(float);
+struct Kv4Rows {
+  int group, rows, chunks;  // query heads per KV head; query rows per KV head; of eight rows each
+};
+__host__ __device__ inline Kv4Rows kv4_rows(int t, int n, int nkv) {
+  const int group = n / nkv, rows = t * group;
+  return {group, rows, (rows + 7) / 8};
 }
 
-cudaError_t launch_kv4_sdpa(const Kv4Sdpa& p, cudaStream_t s) { return launch_rows(p, s); }
+// Workspace of the piecewise kernels: records, then the logits [pair][slot (rounded up to a tile)][8 rows] where scores
+// are wanted.
+__host__ __device__ inline size_t kv4_records_floats(int ctas, long long pairs, int h) { return ((size_t)ctas + (size_t)pairs) * 8 * (h + 4); }
+
+__device__ __forceinline__ int kv4_length(const Kv4Sdpa& p, int b) {
+  return p.lengths ? max(0, min(p.lengths[b], p.cache.s)) : p.cache.s;
+}
+// Units of all sequences' pairs, and of the sequences below `b`. Whole warp.
+__device__ __forceinline__ void kv4_count_units(const Kv4Sdpa& p, int per, int b, int lane, int* total, int* below) {
+  int all = 0, low = 0;
+  for (int i = lane; i < p.cache.b; i += 32) {
+    const int u = units_of(kv4_length(p, i)) * per;
+    all += u;
+    if (i < b) low += u;
+  }
+  *total = (int)__reduce_add_sync(0xffffffffu, (unsigned)all);
+  *below = (int)__reduce_add_sync(0xffffffffu, (unsigned)low);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] = lds32(a);
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]) : "r"(a + 4 * i));
+  }
+}
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float2 pair_floats(uint32_t bits) { return __half22float2(*reinterpret_cast<const __half2*>(&bits)); }
+__device__ __forceinline__ uint32_t halves(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// a and b as fp16, and what that leaves as fp16: 22 bits of each.
+__device__ __forceinline__ void split_halves(float a, float b, uint32_t& high, uint32_t& low) {
+  high = halves(a, b);
+  const float2 r = pair_floats(high);
+  low = halves(a - r.x, b - r.y);
+}
+
+// Where in a tile's nibbles the 16-byte piece c of a row lies. Rows follow one another; within each 128 bytes the pieces
+// are exchanged by an XOR such that the fragment loads below touch 32 banks: of the keys, a load takes one or two
+// neighbouring pieces of rows 0 .. 7, of the values of rows 0, 2, 4, 6 (or 1, 3, 5, 7). Rows r and r + 8 are exchanged
+// alike, and c only enters through an XOR of bits 4 to 6.
+template <int H, bool VALUES>
+__device__ __forceinline__ uint32_t piece_at(int row, int c) {
+  constexpr int kRows = 256 / H;  // per 128 bytes
+  const int line = row / kRows, pos = (row % kRows) * (H / 32) + c;
+  int x;
+  if (VALUES) {
+    x = H == 256 ? row & 7 : H == 128 ? (line & 3) << 1 : (line & 1) << 1;
+  } else {
+    x = H == 256 ? ((row & 3) << 1) | ((row >> 2) & 1) : H == 128 ? ((line & 1) << 1) | ((line >> 1) & 1) : line & 1;
+  }
+  return (uint32_t)(line * 128 + ((pos ^ x) << 4));
+}
+
+// Nibbles become fp16 operands by a mask alone: in the low bits of a half, nibble u is the subnormal number u 2^-24, one
+// place up u 2^-20. So a word of eight nibbles is four pairs after one shift and four masks, exactly; the factor 16
+// between the two kinds goes into the other operand (keys: the queries of those channels are divided by 16) or into the
+// result (values: the kinds are the two halves of the product's rows), 2^-24 into the epilogue.
+constexpr uint32_t kLowNibbles = 0x000f000fu, kHighNibbles = 0x00f000f0u;
+
+template <int H, int BLOCK, bool QF32>
+__global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, const int min_units, float* logits_ws) {
+  using T = Kv4Tile<H, BLOCK>;
+  constexpr int G = T::kG, W = T::kWarps;
+  constexpr int kKeySlots = H / 32;                          // key words per thread and row
+  constexpr int kTiles = BLOCK == 64 ? 4 : 2;                // 16-channel tiles of the second product per block
+  extern __shared__ uint8_t kv4_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
+  __shared__ int s_pair[4];            // sequence, pair within it, first unit, units
+  __shared__ float s_m[W][8], s_l[W][8];
+  __shared__ float s_acc[W][8][G];     // what the least values contribute, per block
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int nkv = p.cache.nkv, s_max = p.cache.s;
+  const Kv4Rows rw = kv4_rows(p.t, p.n, nkv);
+  const int per = nkv * rw.chunks;     // pairs per sequence
+  pdl_wait();
+  // (only now: what a dependent kernel does ahead of its own wait may then read this kernel's inputs)
+  pdl_launch_dependents();
+  if (w == 0) {
+    int total, below;
+    kv4_count_units(p, per, 0, lane, &total, &below);
+    const Pieces cut(total, gridDim.x, min_units);
+    const int c = blockIdx.x;
+    const int u0 = c < cut.ctas ? cut.begin(c) : 0, u1 = c < cut.ctas ? cut.begin(c + 1) : 0;
+    int base = 0;
+    for (int b0 = 0; b0 < p.cache.b && u0 < u1; b0 += 32) {
+      const int units = b0 + lane < p.cache.b ? units_of(kv4_length(p, b0 + lane)) : 0;
+      int upto = units * per;  // inclusive prefix sum over the lanes
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      const int mine = base + upto - units * per;
+      const bool here = units > 0 && mine <= u0 && u0 < mine + units * per;
+      if (here) {
+        s_pair[0] = b0 + lane;
+        s_pair[1] = (u0 - mine) / units;
+        s_pair[2] = (u0 - mine) % units;
+      }
+      if (__any_sync(0xffffffffu, here)) break;
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) s_pair[3] = u1 - u0;
+  }
+  __syncthreads();
+  int left = s_pair[3];
+  if (left == 0) return;
+  int b = s_pair[0], in_b = s_pair[1], unit = s_pair[2];
+  int len = kv4_length(p, b);
+
+  // this warp's ring, and where a lane's copies go
+  const uint32_t ring = smem_u32(smem) + (uint32_t)(w * T::kStages * T::kBytes);
+  constexpr int kPieces = H / 32, kCopies = H / 64;  // 16-byte pieces of a row; copies per lane of a tile's keys
+  const int copy_row = lane / kPieces, copy_piece = lane % kPieces;
+  const size_t row_pitch = (size_t)nkv * (H / 2), pair_pitch = (size_t)nkv * G;  // bytes; pairs
+  // fragment places (see piece_at)
+  const uint32_t key_at = BLOCK == 64 ? piece_at<H, false>(g, t >> 1) + (uint32_t)(t & 1) * 8 : piece_at<H, false>(g, 0) + (uint32_t)t * 4;
+  const uint32_t val_piece = BLOCK == 64 ? (uint32_t)(g >> 2) : 0u, val_byte = BLOCK == 64 ? (uint32_t)(g & 3) * 4 : (uint32_t)(g >> 1) * 4;
+  const uint32_t val_at[2] = {piece_at<H, true>(2 * t, val_piece) + val_byte, piece_at<H, true>(2 * t + 1, val_piece) + val_byte};
+  const uint32_t val_select = (g & 1) ? 0x7632u : 0x5410u;  // blocks of 32: which half of the word this thread's channels are
+
+  while (left > 0) {
+    const int seg = min(left, units_of(len) - unit);
+    const int kvh = in_b / rw.chunks, chunk = in_b % rw.chunks;
+    const size_t pair = (size_t)b * per + in_b;
+    const int mine = seg > w ? (seg - w + W - 1) / W : 0;  // tiles of this warp
+    const size_t slot0 = (size_t)b * s_max;
+    const uint8_t* k_base = p.cache.k + (slot0 * nkv + kvh) * (H / 2);
+    const uint8_t* v_base = p.cache.v + (slot0 * nkv + kvh) * (H / 2);
+    const __half2* kp_base = p.cache.k_pairs + (slot0 * nkv + kvh) * G;
+    const __half2* vp_base = p.cache.v_pairs + (slot0 * nkv + kvh) * G;
+    // Requests this warp's tile k: rows behind the length arrive as zeros.
+    auto request = [&](int k) {
+      if (k < mine) {
+        const int first = (unit + w + k * W) * kUnit, there = len - first;
+        const uint32_t to = ring + (uint32_t)(k % T::kStages) * T::kBytes;
+        const uint8_t* ks = k_base + (size_t)first * row_pitch;
+        const uint8_t* vs = v_base + (size_t)first * row_pitch;
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+          const int row = copy_row + j * (1024 / H);
+          const bool ok = row < there;
+          const size_t from = (ok ? row * row_pitch : 0) + (size_t)copy_piece * 16;
+          cp_async16(to + piece_at<H, false>(row, copy_piece), ks + from, ok);
+          cp_async16(to + T::kNibbleBytes + piece_at<H, true>(row, copy_piece), vs + from, ok);
+        }
+        const __half2* kps = kp_base + (size_t)first * pair_pitch;
+        const __half2* vps = vp_base + (size_t)first * pair_pitch;
+#pragma unroll
+        for (int j = 0; j < (kUnit * G + 31) / 32; ++j) {
+          const int e = lane + 32 * j, row = e / G;
+          if (e < kUnit * G) {
+            const bool ok = row < there;
+            const size_t from = (ok ? row * pair_pitch : 0) + e % G;
+            cp_async4(to + 2 * T::kNibbleBytes + e * 4, kps + from, ok);
+            cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + e * 4, vps + from, ok);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < T::kStages - 1; ++k) request(k);
+
+    // Queries: thread (g, t) holds row g's elements at its words of a key, as the B operand. They are scaled by a power of
+    // two that brings the row's largest to 2^10 .. 2^11: dividing by 16 then loses nothing above 2^-36 of it, and a float32
+    // query is two fp16 numbers to 22 bits.
+    uint32_t q_high[kKeySlots][4], q_low[QF32 ? kKeySlots : 1][4];
+    float q_sum[G][2], factor[2];  // of the rows 2 t and 2 t + 1 (the products' columns)
+    int limit[2];
+    {
+      const int r = chunk * 8 + g;
+      const int i = r / rw.group;
+      const size_t at = (((size_t)b * p.t + i) * p.n + kvh * rw.group + r % rw.group) * H;
+      float raw[kKeySlots][8], top = 0.0f;
+#pragma unroll
+      for (int sl = 0; sl < kKeySlots; ++sl) {
+        const int word = BLOCK == 64 ? 8 * (sl / 2) + 2 * t + sl % 2 : 4 * sl + t;
+        if (r >= rw.rows) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) raw[sl][e] = 0.0f;
+        } else if constexpr (QF32) {
+          const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + 8 * word);
+          const float4 lo = __ldg(src), hi = __ldg(src + 1);
+          raw[sl][0] = lo.x, raw[sl][1] = lo.y, raw[sl][2] = lo.z, raw[sl][3] = lo.w;
+          raw[sl][4] = hi.x, raw[sl][5] = hi.y, raw[sl][6] = hi.z, raw[sl][7] = hi.w;
+        } else {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + at + 8 * word));
+          const float2 f0 = pair_floats(v.x), f1 = pair_floats(v.y), f2 = pair_floats(v.z), f3 = pair_floats(v.w);
+          raw[sl][0] = f0.x, raw[sl][1] = f0.y, raw[sl][2] = f1.x, raw[sl][3] = f1.y;
+          raw[sl][4] = f2.x, raw[sl][5] = f2.y, raw[sl][6] = f3.x, raw[sl][7] = f3.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(raw[sl][e]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int exponent = __float_as_int(top) >> 23;
+      const int up = exponent == 255 ? 127 : min(264 - exponent, 253);  // (an infinite query stays what it is)
+      const float scale_up = __int_as_float(up << 23), scale_down = __int_as_float((254 - up) << 23);
+      float sums[G];
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) sums[gr] = 0.0f;
+#pragma unroll
+      for (int sl = 0; sl < kKeySlots; ++sl) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          raw[sl][e] *= scale_up;
+          sums[BLOCK == 64 ? sl / 2 : sl] += raw[sl][e];
+        }
+        // channels 0, 4 | 2, 6 meet low nibbles, 1, 5 | 3, 7 high ones
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = e < 2 ? 2 * e : 2 * (e - 2) + 1;
+          const float f = e < 2 ? 1.0f : 0.0625f;
+          if constexpr (QF32) {
+            split_halves(raw[sl][c] * f, raw[sl][c + 4] * f, q_high[sl][e], q_low[sl][e]);
+          } else {
+            q_high[sl][e] = halves(raw[sl][c] * f, raw[sl][c + 4] * f);
+          }
+        }
+      }
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) {
+        sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], 1);
+        sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], 2);
+        sums[gr] *= 0x1p-24f;
+        q_sum[gr][0] = __shfl_sync(0xffffffffu, sums[gr], 8 * t);
+        q_sum[gr][1] = __shfl_sync(0xffffffffu, sums[gr], 8 * t + 4);
+      }
+      const float f = scale_down * p.scale;
+      // (in two steps: 2^24 times a small scale stays within fp32 either way)
+      factor[0] = __shfl_sync(0xffffffffu, f, 8 * t) * 0x1p24f;
+      factor[1] = __shfl_sync(0xffffffffu, f, 8 * t + 4) * 0x1p24f;
+    }
+    const float* mask[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = chunk * 8 + 2 * t + e, i = r / rw.group;
+      limit[e] = r < rw.rows ? kv4_limit(len, s_max, p.t, i) : 0;
+      mask[e] = p.mask && r < rw.rows ? p.mask + ((size_t)b * p.t + i) * s_max : nullptr;
+    }
+    // masks are requested a tile ahead of their use
+    auto masks = [&](int k, float (&m)[4]) {
+      const int first = (unit + w + k * W) * kUnit;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int slot = first + g + 8 * (e >> 1);
+        m[e] = mask[e & 1] && k < mine && slot < limit[e & 1] ? __ldg(mask[e & 1] + slot) : 0.0f;
+      }
+    };
+    float next_mask[4];
+    masks(0, next_mask);
+    const bool guard = p.mask != nullptr || p.t > 1;  // slots that some row does not see may hold anything
+    float* logits = logits_ws ? logits_ws + pair * (size_t)(units_of(s_max) * kUnit) * 8 : nullptr;
+
+    float o[G][kTiles][4], least_sum[G];
+#pragma unroll
+    for (int gr = 0; gr < G; ++gr) {
+      least_sum[gr] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) o[gr][i][0] = o[gr][i][1] = o[gr][i][2] = o[gr][i][3] = 0.0f;
+    }
+    float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, m_use[2] = {0.0f, 0.0f}, l_run[2] = {0.0f, 0.0f};
+    uint32_t exponent = 1;  // fp16 exponent field of the largest value scale so far: weights are in units of 2^(exponent - 29)
+
+#pragma unroll 1
+    for (int k = 0; k < mine; ++k) {
+      cp_async_wait<T::kStages - 2>();
+      __syncwarp();  // the tile is there, and everybody is done with the one whose place the next request takes
+      request(k + T::kStages - 1);
+      const uint32_t at = ring + (uint32_t)(k % T::kStages) * T::kBytes;
+      const uint32_t pairs_at = at + 2 * T::kNibbleBytes;
+      const int first = (unit + w + k * W) * kUnit;
+
+      // -- logits of slots g and g + 8, rows 2 t and 2 t + 1 --
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      {
+        uint32_t pa[G], pb[G];
+        lds_words(pairs_at + (uint32_t)(g * G * 4), pa);
+        lds_words(pairs_at + (uint32_t)((g + 8) * G * 4), pb);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+          constexpr int kN = BLOCK / 32;  // words of this block per thread and row
+          uint32_t wa[kN], wb[kN];
+          const uint32_t from = at + (key_at ^ (uint32_t)(gr * (BLOCK / 2)));
+          lds_words(from, wa);
+          lds_words(from + 4 * H, wb);
+          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            const int sl = gr * kN + j;
+            const uint32_t a8 = wa[j] >> 8, b8 = wb[j] >> 8;
+            const uint32_t l0 = wa[j] & kLowNibbles, l1 = wb[j] & kLowNibbles, l2 = a8 & kLowNibbles, l3 = b8 & kLowNibbles;
+            const uint32_t h0 = wa[j] & kHighNibbles, h1 = wb[j] & kHighNibbles, h2 = a8 & kHighNibbles, h3 = b8 & kHighNibbles;
+            mma_f16(acc, l0, l1, l2, l3, q_high[sl][0], q_high[sl][1]);
+            mma_f16(acc, h0, h1, h2, h3, q_high[sl][2], q_high[sl][3]);
+            if constexpr (QF32) {
+              mma_f16(acc, l0, l1, l2, l3, q_low[sl][0], q_low[sl][1]);
+              mma_f16(acc, h0, h1, h2, h3, q_low[sl][2], q_low[sl][3]);
+            }
+          }
+          const float2 fa = pair_floats(pa[gr]), fb = pair_floats(pb[gr]);
+          x[0] = fmaf(fa.x, acc[0], fmaf(fa.y, q_sum[gr][0], x[0]));
+          x[1] = fmaf(fa.x, acc[1], fmaf(fa.y, q_sum[gr][1], x[1]));
+          x[2] = fmaf(fb.x, acc[2], fmaf(fb.y, q_sum[gr][0], x[2]));
+          x[3] = fmaf(fb.x, acc[3], fmaf(fb.y, q_sum[gr][1], x[3]));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] *= factor[e & 1];
+      if (p.logit_cap > 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = p.logit_cap * tanhf(x[e] / p.logit_cap);
+      }
+      if (p.mask) {
+        float m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] = next_mask[e];
+        masks(k + 1, next_mask);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = m[e] == -CUDART_INF_F ? m[e] : x[e] + m[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = first + g + 8 * (e >> 1) < limit[e & 1] ? x[e] : -CUDART_INF_F;
+      if (logits) {
+        float* to = logits + (size_t)(first + g) * 8 + 2 * t;
+        *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
+        *reinterpret_cast<float2*>(to + 64) = make_float2(x[2], x[3]);
+      }
+
+      // -- the values' pairs of slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9, and the largest scale of the tile --
+      uint32_t vp[4][G];
+      uint32_t largest = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lds_words(pairs_at + T::kPairBytes + (uint32_t)((2 * t + (j & 1) + 8 * (j >> 1)) * G * 4), vp[j]);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) largest = __vmaxu2(largest, vp[j][gr] & 0x00007fffu);
+      }
+      const uint32_t now = max(exponent, min(__reduce_max_sync(0xffffffffu, largest) >> 10, 30u));
+      // -- running maximum and unit; both rarely change --
+      const bool grows = fmaxf(x[0], x[2]) > m_run[0] || fmaxf(x[1], x[3]) > m_run[1];
+      if (__any_sync(0xffffffffu, grows) || now != exponent) {
+        float alpha[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(x[e], x[e + 2]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          top = fmaxf(m_run[e], top);
+          const float use = top == -CUDART_INF_F ? 0.0f : top;
+          alpha[e] = m_run[e] == -CUDART_INF_F ? 0.0f : exp2f((m_run[e] - use) * kLog2e);
+          m_run[e] = top;
+          m_use[e] = use;
+          l_run[e] *= alpha[e];
+        }
+        const float shrink = __int_as_float((int)(127 + exponent - now) << 23);
+        exponent = now;
+        // (a least-value sum belongs to row g: its factor is with the threads of column g)
+        const float even = __shfl_sync(0xffffffffu, alpha[0], g >> 1), odd = __shfl_sync(0xffffffffu, alpha[1], g >> 1);
+        const float mine_alpha = ((g & 1) ? odd : even) * shrink;
+        alpha[0] *= shrink;
+        alpha[1] *= shrink;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+          least_sum[gr] *= mine_alpha;
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            o[gr][i][0] *= alpha[0];
+            o[gr][i][1] *= alpha[1];
+            o[gr][i][2] *= alpha[0];
+            o[gr][i][3] *= alpha[1];
+          }
+        }
+      }
+      float pr[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pr[e] = exp2f((x[e] - m_use[e & 1]) * kLog2e);
+      l_run[0] += pr[0] + pr[2];
+      l_run[1] += pr[1] + pr[3];
+      // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9, in units of the value scales
+      float pw[4];
+      const float to_units = __int_as_float((int)(156 - exponent) << 23);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t c0 = __float_as_uint(pr[2 * e]), c1 = __float_as_uint(pr[2 * e + 1]);
+        const uint32_t lo = transposed8x8(__byte_perm(c0, c1, 0x5410)), hi = transposed8x8(__byte_perm(c0, c1, 0x7632));
+        pw[2 * e] = __uint_as_float(__byte_perm(lo, hi, 0x5410)) * to_units;
+        pw[2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632)) * to_units;
+      }
+      if (guard) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int gr = 0; gr < G; ++gr) vp[j][gr] = pw[j] == 0.0f ? 0u : vp[j][gr];
+      }
+      // -- outputs: channels by slots times slots by rows; a weight is two fp16 numbers --
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) {
+        float ps[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = pair_floats(vp[j][gr]);
+          ps[j] = pw[j] * f.x;
+          least_sum[gr] = fmaf(pw[j], f.y, least_sum[gr]);
+        }
+        uint32_t high[2], low[2];
+        split_halves(ps[0], ps[1], high[0], low[0]);
+        split_halves(ps[2], ps[3], high[1], low[1]);
+        uint32_t words[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          words[j] = lds32(at + T::kNibbleBytes + (val_at[j & 1] ^ (uint32_t)(gr * (BLOCK / 2))) + (j >> 1) * 4 * H);
+#pragma unroll
+        for (int half = 0; half < kTiles / 2; ++half) {
+          const uint32_t select = BLOCK == 32 ? val_select : half ? 0x7632u : 0x5410u;
+          const uint32_t a = __byte_perm(words[0], words[1], select), c = __byte_perm(words[2], words[3], select);
+          const uint32_t a8 = a >> 8, c8 = c >> 8;
+          float (&o0)[4] = o[gr][2 * half], (&o1)[4] = o[gr][2 * half + 1];
+          mma_f16(o0, a & kLowNibbles, a & kHighNibbles, c & kLowNibbles, c & kHighNibbles, high[0], high[1]);
+          mma_f16(o1, a8 & kLowNibbles, a8 & kHighNibbles, c8 & kLowNibbles, c8 & kHighNibbles, high[0], high[1]);
+          mma_f16(o0, a & kLowNibbles, a & kHighNibbles, c & kLowNibbles, c & kHighNibbles, low[0], low[1]);
+          mma_f16(o1, a8 & kLowNibbles, a8 & kHighNibbles, c8 & kLowNibbles, c8 & kHighNibbles, low[0], low[1]);
+        }
+      }
+    }
+    cp_async_wait<0>();
+
+    // -- the warps' states become one record --
+    const int busy = min(W, seg);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], d);
+    if (g == 0) {
+      s_m[w][2 * t] = m_run[0], s_m[w][2 * t + 1] = m_run[1];
+      s_l[w][2 * t] = l_run[0], s_l[w][2 * t + 1] = l_run[1];
+    }
+    __syncthreads();  // (also: no ring is read any more)
+    if (w < busy) {
+      const float from_units = __int_as_float((int)(98 + exponent) << 23);  // 2^(exponent - 29)
+      float mine_f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -CUDART_INF_F;
+        for (int i = 0; i < busy; ++i) top = fmaxf(top, s_m[i][2 * t + e]);
+        mine_f[e] = m_run[e] == -CUDART_INF_F ? 0.0f : exp2f((m_run[e] - top) * kLog2e) * from_units;
+      }
+      const float even = __shfl_sync(0xffffffffu, mine_f[0], g >> 1), odd = __shfl_sync(0xffffffffu, mine_f[1], g >> 1);
+      const float f_row = (g & 1) ? odd : even;
+      float* part = reinterpret_cast<float*>(smem) + (size_t)w * 8 * T::kRec;
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) {
+        float sum = least_sum[gr];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (t == 0) s_acc[w][g][gr] = sum * f_row;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float low = mine_f[e] * 0x1p24f, high = mine_f[e] * 0x1p20f;
+          float* dst = part + (2 * t + e) * T::kRec + gr * BLOCK + g * (2 * kTiles);
+#pragma unroll
+          for (int i = 0; i < kTiles; i += 2)
+            *reinterpret_cast<float4*>(dst + 2 * i) =
+                make_float4(o[gr][i][e] * low, o[gr][i][2 + e] * high, o[gr][i + 1][e] * low, o[gr][i + 1][2 + e] * high);
+        }
+      }
+    }
+    __syncthreads();
+    float* rec = p.ws + ((size_t)blockIdx.x + pair) * 8 * T::kRec;
+    const int rows = min(8, rw.rows - chunk * 8);
+    for (int i = tid; i < rows * (H / 4); i += T::kThreads) {
+      const int row = i / (H / 4), d = i % (H / 4) * 4;
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int j = 0; j < busy; ++j) {
+        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + ((size_t)j * 8 + row) * T::kRec + d);
+        const float a = s_acc[j][row][d / BLOCK];
+        sum.x += v.x + a;
+        sum.y += v.y + a;
+        sum.z += v.z + a;
+        sum.w += v.w + a;
+      }
+      *reinterpret_cast<float4*>(rec + row * T::kRec + d) = sum;
+    }
+    if (tid < rows) {
+      float top = -CUDART_INF_F, sum = 0.0f;
+      for (int j = 0; j < busy; ++j) top = fmaxf(top, s_m[j][tid]);
+      for (int j = 0; j < busy; ++j) sum += s_m[j][tid] == -CUDART_INF_F ? s_l[j][tid] : exp2f((s_m[j][tid] - top) * kLog2e) * s_l[j][tid];
+      *reinterpret_cast<float2*>(rec + tid * T::kRec + H) = make_float2(top, sum);
+    }
+    left -= seg;
+    if (left > 0) {
+      __syncthreads();  // the next segment's copies go where the states were
+      unit = 0;
+      if (++in_b == per) {
+        in_b = 0;
+        do {
+          ++b;
+          len = kv4_length(p, b);
+        } while (len == 0);
+      }
+    }
+  }
+}
+
+// Merges the records of one query row (the first n t CTAs of a sequence), or adds the weights that 1024 slots of a KV head
+// got to the scores (the others).
+constexpr int kMergeThreads = 256;
+constexpr int kScoreSlots = 1024;
+template <int H, bool QF32>
+__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa p, const int split_ctas, const int min_units, const float* logits_ws) {
+  constexpr int kRec = H + 4, kQuads = H / 4, kGroups = kMergeThreads / kQuads, kBatch = 16;
+  constexpr size_t kStride = 8 * (size_t)kRec;
+  extern __shared__ float merge_w[];  // one weight per record
+  __shared__ float4 s_part[kMergeThreads];
+  __shared__ float s_stat[16];
+  pdl_launch_dependents();
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Kv4Rows rw = kv4_rows(p.t, p.n, p.cache.nkv);
+  const int per = p.cache.nkv * rw.chunks;
+  // what does not depend on the kernel before: it has waited for whatever wrote the lengths
+  int total, below;
+  kv4_count_units(p, per, b, lane, &total, &below);
+  const Pieces cut(total, split_ctas, min_units);
+  const int length = kv4_length(p, b), units = units_of(length);
+  auto records = [&](int in_b, int* count) {
+    *count = 0;
+    if (units == 0) return (const float*)nullptr;
+    const int u0 = below + in_b * units, c0 = cut.owner(u0), c1 = cut.owner(u0 + units - 1);
+    *count = c1 - c0 + 1;
+    return (const float*)p.ws + ((size_t)c0 + (size_t)b * per + in_b) * kStride;
+  };
+  if ((int)blockIdx.x < p.n * p.t) {
+    const int i = blockIdx.x / p.n, head = blockIdx.x % p.n, kvh = head / rw.group, r = i * rw.group + head % rw.group;
+    const int quad = threadIdx.x % kQuads, grp = threadIdx.x / kQuads;
+    int count;
+    const float* base = records(kvh * rw.chunks + r / 8, &count) + (r % 8) * kRec;
+    pdl_wait();
+    float4 first[kBatch];
+    request_quads(first, base + 4 * quad, kStride, count, grp, kGroups);
+    if (threadIdx.x < 32) {
+      const float l = record_weights(base + H, kStride, count, lane, merge_w, kLog2e);
+      if (lane == 0) s_stat[0] = l;
+    }
+    __syncthreads();
+    s_part[threadIdx.x] = merge_quad(base + 4 * quad, kStride, count, grp, kGroups, merge_w, first);
+    __syncthreads();
+    if (grp > 0) return;
+    float4 acc = s_part[quad];
+#pragma unroll 2
+    for (int j = 1; j < kGroups; ++j) {
+      const float4 v = s_part[j * kQuads + quad];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+    }
+    const float l = s_stat[0];
+    if (l == 0.0f) {
+      acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // no slot
+    } else {
+      acc = make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
+    }
+    const size_t at = (((size_t)b * p.t + i) * p.n + head) * H + 4 * quad;
+    if constexpr (QF32) {
+      float* o = static_cast<float*>(p.out) + at;
+      o[0] = acc.x, o[1] = acc.y, o[2] = acc.z, o[3] = acc.w;
+    } else {
+      __half* o = static_cast<__half*>(p.out) + at;
+      o[0] = __float2half_rn(acc.x), o[1] = __float2half_rn(acc.y), o[2] = __float2half_rn(acc.z), o[3] = __float2half_rn(acc.w);
+    }
+    return;
+  }
+  const int ranges = (p.cache.s + kScoreSlots - 1) / kScoreSlots;
+  const int at = blockIdx.x - p.n * p.t, kvh = at / ranges, slot0 = at % ranges * kScoreSlots;
+  pdl_wait();
+  if (slot0 >= length) return;
+  const size_t pitch = (size_t)(units_of(p.cache.s) * kUnit) * 8;
+  float sums[kScoreSlots / kMergeThreads];
+#pragma unroll
+  for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) sums[j] = 0.0f;
+  for (int c = 0; c < rw.chunks; ++c) {
+    const int in_b = kvh * rw.chunks + c, rows = min(8, rw.rows - 8 * c);
+    int count;
+    const float* ml = records(in_b, &count) + H;
+    __syncthreads();
+    if (warp < rows) {
+      float top = -CUDART_INF_F, l = 0.0f;
+      for (int j = lane; j < count; j += 32) top = fmaxf(top, __ldcg(ml + warp * kRec + j * kStride));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = top == -CUDART_INF_F ? 0.0f : top;
+      for (int j = lane; j < count; j += 32) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(ml + warp * kRec + j * kStride));
+        l += exp2f((v.x - top) * kLog2e) * v.y;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      if (lane == 0) {
+        s_stat[warp] = top;
+        s_stat[8 + warp] = l == 0.0f ? 0.0f : 1.0f / l;
+      }
+    } else if (lane == 0) {
+      s_stat[warp] = 0.0f;
+      s_stat[8 + warp] = 0.0f;
+    }
+    __syncthreads();
+    const float* logits = logits_ws + ((size_t)b * per + in_b) * pitch;
+#pragma unroll
+    for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) {
+      const int slot = slot0 + threadIdx.x + j * kMergeThreads;
+      if (slot < length) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(logits + (size_t)slot * 8)), y = __ldcg(reinterpret_cast<const float4*>(logits + (size_t)slot * 8) + 1);
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < rows) sums[j] = fmaf(exp2f((v[e] - s_stat[e]) * kLog2e), s_stat[8 + e], sums[j]);
+      }
+    }
+  }
+  float* scores = p.scores + ((size_t)b * p.cache.nkv + kvh) * p.cache.s;
+#pragma unroll
+  for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) {
+    const int slot = slot0 + threadIdx.x + j * kMergeThreads;
+    if (slot < length) scores[slot] += sums[j];
+  }
+}
+
+// Shortest piece worth a CTA of its own: a tile for every warp.
+constexpr int kv4_min_units(int h) { return h == 256 ? 8 : 16; }
+// CTAs of a launch: one per SM, fewer when even full caches give no piece for some.
+int kv4_ctas(long long pairs, int s, int h) {
+  const long long most = pairs * ((s + kUnit - 1) / kUnit), n = (most + kv4_min_units(h) - 1) / kv4_min_units(h);
+  const int sms = device_sm_count();
+  return n < sms ? (int)n : sms;
+}
+
+bool kv4_tensor_shape(int b, int t, int n, int nkv, int h, int s) {
+  const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
+  return (h == 64 || h == 128 || h == 256) && pairs * ((s + kUnit - 1) / kUnit) <= INT32_MAX &&
+         (long long)n * t + (long long)nkv * ((s + kScoreSlots - 1) / kScoreSlots) <= INT32_MAX;
+}
+
+template <int H, int BLOCK, bool QF32>
+cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
+  using T = Kv4Tile<H, BLOCK>;
+  const long long pairs = (long long)p.cache.b * p.cache.nkv * kv4_rows(p.t, p.n, p.cache.nkv).chunks;
+  const int ctas = kv4_ctas(pairs, p.cache.s, H), min_units = kv4_min_units(H);
+  float* logits = p.scores ? p.ws + kv4_records_floats(ctas, pairs, H) : nullptr;
+  static bool done[64] = {false};
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device < 0 || device >= 64) device = 0;
+  if (!done[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(kv4_sdpa_kernel<H, BLOCK, QF32>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
+    if (e != cudaSuccess) return e;
+    done[device] = true;
+  }
+  const cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, min_units, logits);
+  if (e != cudaSuccess) return e;
+  const int scores = p.scores ? p.cache.nkv * ((p.cache.s + kScoreSlots - 1) / kScoreSlots) : 0;
+  return launch_chained(kv4_merge_kernel<H, QF32>, dim3(p.n * p.t + scores, p.cache.b), dim3(kMergeThreads), sizeof(float) * (size_t)ctas, s, p,
+                        ctas, min_units, (const float*)logits);
+}
+template <int H, int BLOCK>
+cudaError_t launch_tensor_q(const Kv4Sdpa& p, cudaStream_t s) {
+  return p.f32 ? launch_tensor<H, BLOCK, true>(p, s) : launch_tensor<H, BLOCK, false>(p, s);
+}
+template <int H>
+cudaError_t launch_tensor_block(const Kv4Sdpa& p, cudaStream_t s) {
+  return p.cache.block == 64 ? launch_tensor_q<H, 64>(p, s) : launch_tensor_q<H, 32>(p, s);
+}
+
+}  // namespace
+
+size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int scores) {
+  const size_t rows = (size_t)b * t * n;
+  const size_t any = 2 * rows + rows * s;  // (also what queries off a 16-byte boundary need)
+  if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return any * sizeof(float);
+  const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
+  const size_t tensor = kv4_records_floats(kv4_ctas(pairs, s, h), pairs, h) +
+                        (scores ? (size_t)pairs * ((s + kUnit - 1) / kUnit * kUnit) * 8 : 0);
+  return (any > tensor ? any : tensor) * sizeof(float);
+}
+
+cudaError_t launch_kv4_sdpa(const Kv4Sdpa& p, cudaStream_t s) {
+  const Kv4Cache& c = p.cache;
+  if (!kv4_tensor_shape(c.b, p.t, p.n, c.nkv, c.h, c.s) || (reinterpret_cast<uintptr_t>(p.q) & 15) != 0) return launch_rows(p, s);
+  return c.h == 256 ? launch_tensor_block<256>(p, s) : c.h == 128 ? launch_tensor_block<128>(p, s) : launch_tensor_block<64>(p, s);
+}
 
 }  // namespace b200
