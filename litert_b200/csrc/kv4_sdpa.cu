@@ -148,23 +148,28 @@ cudaError_t launch_rows(const Kv4Sdpa& p, cudaStream_t s) {
 }
 
 // ---- head sizes 64, 128 and 256: tensor cores -------------------------------------------------------------
-// Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; 16 slots are a
-// tile. A warp works on tiles of its own from the first copy to the last product, with its own running maximum, sum and
-// outputs: no barrier until the warps of a CTA merge at the end of a piece. (pieces.cuh: how the slots are cut.)
+// Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; a tile is 32 slots,
+// two 16-row sides of it whose chains of products and exponentials run side by side. A warp works on tiles of its own
+// from the first copy to the last product, with its own running maximum, sum and outputs: no barrier until the warps of
+// a CTA merge at the end of a piece. (pieces.cuh: how the slots are cut.)
+constexpr int kSlots = 32;
+__host__ __device__ inline int tiles_of(int slots) { return (slots + kSlots - 1) / kSlots; }
+
 template <int H, int BLOCK>
 struct Kv4Tile {
-  static constexpr int kG = H / BLOCK;                // blocks of a row
-  static constexpr int kNibbleBytes = kUnit * H / 2;  // of the keys (or values) of a tile
-  static constexpr int kPairBytes = kUnit * kG * 4;
+  static constexpr int kG = H / BLOCK;                 // blocks of a row
+  static constexpr int kNibbleBytes = kSlots * H / 2;  // of the keys (or values) of a tile
+  static constexpr int kPairBytes = kSlots * kG * 4;
   static constexpr int kBytes = 2 * (kNibbleBytes + kPairBytes);
-  static constexpr int kWarps = H == 256 ? 8 : 16;
-  static constexpr int kStages = H == 64 ? 8 : 4;
+  static constexpr int kWarps = H == 256 ? 8 : H == 128 ? 12 : 16;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kRec = H + 4;  // floats of a record per row: outputs, maximum, sum, padding
-  static constexpr int kRing = kWarps * kStages * kBytes;
   static constexpr int kMerge = kWarps * 8 * kRec * 4;
+  static constexpr int kFit = 220 * 1024 / (kWarps * kBytes);
+  static constexpr int kStages = kFit > 6 ? 6 : kFit;
+  static constexpr int kRing = kWarps * kStages * kBytes;
   static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + 128;
-  static_assert(kBytes % 128 == 0 && kSmem <= 224 * 1024, "layout");
+  static_assert(kBytes % 128 == 0 && kStages >= 2 && kSmem <= 221 * 1024, "layout");
 };
 
 struct Kv4Rows {
@@ -182,11 +187,11 @@ __host__ __device__ inline size_t kv4_records_floats(int ctas, long long pairs, 
 __device__ __forceinline__ int kv4_length(const Kv4Sdpa& p, int b) {
   return p.lengths ? max(0, min(p.lengths[b], p.cache.s)) : p.cache.s;
 }
-// Units of all sequences' pairs, and of the sequences below `b`. Whole warp.
+// Tiles of all sequences' pairs, and of the sequences below `b`. Whole warp.
 __device__ __forceinline__ void kv4_count_units(const Kv4Sdpa& p, int per, int b, int lane, int* total, int* below) {
   int all = 0, low = 0;
   for (int i = lane; i < p.cache.b; i += 32) {
-    const int u = units_of(kv4_length(p, i)) * per;
+    const int u = tiles_of(kv4_length(p, i)) * per;
     all += u;
     if (i < b) low += u;
   }
@@ -256,11 +261,19 @@ __device__ __forceinline__ uint32_t piece_at(int row, int c) {
   return (uint32_t)(line * 128 + ((pos ^ x) << 4));
 }
 
-// Nibbles become fp16 operands by a mask alone: in the low bits of a half, nibble u is the subnormal number u 2^-24, one
-// place up u 2^-20. So a word of eight nibbles is four pairs after one shift and four masks, exactly; the factor 16
-// between the two kinds goes into the other operand (keys: the queries of those channels are divided by 16) or into the
-// result (values: the kinds are the two halves of the product's rows), 2^-24 into the epilogue.
+// Key nibbles become fp16 operands by a mask alone: in the low bits of a half, nibble u is the subnormal number u 2^-24,
+// one place up u 2^-20. So a word of eight nibbles is four pairs after one shift and four masks, exactly; the factor 16
+// between the two kinds goes into the queries of those channels, 2^-24 into the logits' factor.
+// Value nibbles are centred, u - 8, by way of the exponents that make a nibble's place the unit (1024) or an eighth of it
+// (64): sums of weights times values that are all positive lose to the tensor core's truncation (float32 outputs were
+// 3e-5 off; 8 x scale joins the least value instead).
 constexpr uint32_t kLowNibbles = 0x000f000fu, kHighNibbles = 0x00f000f0u;
+__device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t centred_low(uint32_t w) { return half2_sub((w & kLowNibbles) | 0x64006400u, 0x64086408u); }    // - 1032
+__device__ __forceinline__ uint32_t centred_high(uint32_t w) { return half2_sub((w & kHighNibbles) | 0x54005400u, 0x54805480u); }  // - 72
 
 template <int H, int BLOCK, bool QF32>
 __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, const int min_units, float* logits_ws) {
@@ -270,7 +283,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
   constexpr int kTiles = BLOCK == 64 ? 4 : 2;                // 16-channel tiles of the second product per block
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
-  __shared__ int s_pair[4];            // sequence, pair within it, first unit, units
+  __shared__ int s_pair[4];            // sequence, pair within it, first tile, tiles
   __shared__ float s_m[W][8], s_l[W][8];
   __shared__ float s_acc[W][8][G];     // what the least values contribute, per block
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -288,7 +301,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     const int u0 = c < cut.ctas ? cut.begin(c) : 0, u1 = c < cut.ctas ? cut.begin(c + 1) : 0;
     int base = 0;
     for (int b0 = 0; b0 < p.cache.b && u0 < u1; b0 += 32) {
-      const int units = b0 + lane < p.cache.b ? units_of(kv4_length(p, b0 + lane)) : 0;
+      const int units = b0 + lane < p.cache.b ? tiles_of(kv4_length(p, b0 + lane)) : 0;
       int upto = units * per;  // inclusive prefix sum over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -315,7 +328,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 
   // this warp's ring, and where a lane's copies go
   const uint32_t ring = smem_u32(smem) + (uint32_t)(w * T::kStages * T::kBytes);
-  constexpr int kPieces = H / 32, kCopies = H / 64;  // 16-byte pieces of a row; copies per lane of a tile's keys
+  constexpr int kPieces = H / 32, kCopies = H / 32;  // 16-byte pieces of a row; copies per lane of a tile's keys
   const int copy_row = lane / kPieces, copy_piece = lane % kPieces;
   const size_t row_pitch = (size_t)nkv * (H / 2), pair_pitch = (size_t)nkv * G;  // bytes; pairs
   // fragment places (see piece_at)
@@ -325,7 +338,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
   const uint32_t val_select = (g & 1) ? 0x7632u : 0x5410u;  // blocks of 32: which half of the word this thread's channels are
 
   while (left > 0) {
-    const int seg = min(left, units_of(len) - unit);
+    const int seg = min(left, tiles_of(len) - unit);
     const int kvh = in_b / rw.chunks, chunk = in_b % rw.chunks;
     const size_t pair = (size_t)b * per + in_b;
     const int mine = seg > w ? (seg - w + W - 1) / W : 0;  // tiles of this warp
@@ -337,7 +350,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     // Requests this warp's tile k: rows behind the length arrive as zeros.
     auto request = [&](int k) {
       if (k < mine) {
-        const int first = (unit + w + k * W) * kUnit, there = len - first;
+        const int first = (unit + w + k * W) * kSlots, there = len - first;
         const uint32_t to = ring + (uint32_t)(k % T::kStages) * T::kBytes;
         const uint8_t* ks = k_base + (size_t)first * row_pitch;
         const uint8_t* vs = v_base + (size_t)first * row_pitch;
@@ -352,14 +365,12 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
         const __half2* kps = kp_base + (size_t)first * pair_pitch;
         const __half2* vps = vp_base + (size_t)first * pair_pitch;
 #pragma unroll
-        for (int j = 0; j < (kUnit * G + 31) / 32; ++j) {
+        for (int j = 0; j < G; ++j) {
           const int e = lane + 32 * j, row = e / G;
-          if (e < kUnit * G) {
-            const bool ok = row < there;
-            const size_t from = (ok ? row * pair_pitch : 0) + e % G;
-            cp_async4(to + 2 * T::kNibbleBytes + e * 4, kps + from, ok);
-            cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + e * 4, vps + from, ok);
-          }
+          const bool ok = row < there;
+          const size_t from = (ok ? row * pair_pitch : 0) + e % G;
+          cp_async4(to + 2 * T::kNibbleBytes + e * 4, kps + from, ok);
+          cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + e * 4, vps + from, ok);
         }
       }
       cp_async_commit();
@@ -446,18 +457,20 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       mask[e] = p.mask && r < rw.rows ? p.mask + ((size_t)b * p.t + i) * s_max : nullptr;
     }
     // masks are requested a tile ahead of their use
-    auto masks = [&](int k, float (&m)[4]) {
-      const int first = (unit + w + k * W) * kUnit;
+    auto masks = [&](int k, float (&m)[2][4]) {
+      const int first = (unit + w + k * W) * kSlots;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int slot = first + g + 8 * (e >> 1);
-        m[e] = mask[e & 1] && k < mine && slot < limit[e & 1] ? __ldg(mask[e & 1] + slot) : 0.0f;
-      }
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int slot = first + 16 * side + g + 8 * (e >> 1);
+          m[side][e] = mask[e & 1] && k < mine && slot < limit[e & 1] ? __ldg(mask[e & 1] + slot) : 0.0f;
+        }
     };
-    float next_mask[4];
+    float next_mask[2][4];
     masks(0, next_mask);
     const bool guard = p.mask != nullptr || p.t > 1;  // slots that some row does not see may hold anything
-    float* logits = logits_ws ? logits_ws + pair * (size_t)(units_of(s_max) * kUnit) * 8 : nullptr;
+    float* logits = logits_ws ? logits_ws + pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
 
     float o[G][kTiles][4], least_sum[G];
 #pragma unroll
@@ -467,7 +480,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       for (int i = 0; i < kTiles; ++i) o[gr][i][0] = o[gr][i][1] = o[gr][i][2] = o[gr][i][3] = 0.0f;
     }
     float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, m_use[2] = {0.0f, 0.0f}, l_run[2] = {0.0f, 0.0f};
-    uint32_t exponent = 1;  // fp16 exponent field of the largest value scale so far: weights are in units of 2^(exponent - 29)
+    uint32_t exponent = 1;  // fp16 exponent field of the largest value scale so far: weights are in units of 2^(exponent - 23)
 
 #pragma unroll 1
     for (int k = 0; k < mine; ++k) {
@@ -476,19 +489,20 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       request(k + T::kStages - 1);
       const uint32_t at = ring + (uint32_t)(k % T::kStages) * T::kBytes;
       const uint32_t pairs_at = at + 2 * T::kNibbleBytes;
-      const int first = (unit + w + k * W) * kUnit;
+      const int first = (unit + w + k * W) * kSlots;
 
-      // -- logits of slots g and g + 8, rows 2 t and 2 t + 1 --
-      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      {
+      // -- logits of slots g, g + 8 (+ 16), rows 2 t and 2 t + 1 --
+      float x[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
         uint32_t pa[G], pb[G];
-        lds_words(pairs_at + (uint32_t)(g * G * 4), pa);
-        lds_words(pairs_at + (uint32_t)((g + 8) * G * 4), pb);
+        lds_words(pairs_at + (uint32_t)((16 * side + g) * G * 4), pa);
+        lds_words(pairs_at + (uint32_t)((16 * side + g + 8) * G * 4), pb);
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
           constexpr int kN = BLOCK / 32;  // words of this block per thread and row
           uint32_t wa[kN], wb[kN];
-          const uint32_t from = at + (key_at ^ (uint32_t)(gr * (BLOCK / 2)));
+          const uint32_t from = at + (key_at ^ (uint32_t)(gr * (BLOCK / 2))) + side * 8 * H;
           lds_words(from, wa);
           lds_words(from + 4 * H, wb);
           float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -506,51 +520,61 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
             }
           }
           const float2 fa = pair_floats(pa[gr]), fb = pair_floats(pb[gr]);
-          x[0] = fmaf(fa.x, acc[0], fmaf(fa.y, q_sum[gr][0], x[0]));
-          x[1] = fmaf(fa.x, acc[1], fmaf(fa.y, q_sum[gr][1], x[1]));
-          x[2] = fmaf(fb.x, acc[2], fmaf(fb.y, q_sum[gr][0], x[2]));
-          x[3] = fmaf(fb.x, acc[3], fmaf(fb.y, q_sum[gr][1], x[3]));
+          x[side][0] = fmaf(fa.x, acc[0], fmaf(fa.y, q_sum[gr][0], x[side][0]));
+          x[side][1] = fmaf(fa.x, acc[1], fmaf(fa.y, q_sum[gr][1], x[side][1]));
+          x[side][2] = fmaf(fb.x, acc[2], fmaf(fb.y, q_sum[gr][0], x[side][2]));
+          x[side][3] = fmaf(fb.x, acc[3], fmaf(fb.y, q_sum[gr][1], x[side][3]));
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= factor[e & 1];
+      for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] *= factor[e & 1];
       if (p.logit_cap > 0.0f) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = p.logit_cap * tanhf(x[e] / p.logit_cap);
+        for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = p.logit_cap * tanhf(x[e >> 2][e & 3] / p.logit_cap);
       }
       if (p.mask) {
-        float m[4];
+        float m[2][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m[e] = next_mask[e];
+        for (int e = 0; e < 8; ++e) m[e >> 2][e & 3] = next_mask[e >> 2][e & 3];
         masks(k + 1, next_mask);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = m[e] == -CUDART_INF_F ? m[e] : x[e] + m[e];
+        for (int e = 0; e < 8; ++e) {
+          const float a = m[e >> 2][e & 3];
+          x[e >> 2][e & 3] = a == -CUDART_INF_F ? a : x[e >> 2][e & 3] + a;
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = first + g + 8 * (e >> 1) < limit[e & 1] ? x[e] : -CUDART_INF_F;
+      for (int e = 0; e < 8; ++e) {
+        const int slot = first + 16 * (e >> 2) + g + 8 * ((e >> 1) & 1);
+        x[e >> 2][e & 3] = slot < limit[e & 1] ? x[e >> 2][e & 3] : -CUDART_INF_F;
+      }
       if (logits) {
-        float* to = logits + (size_t)(first + g) * 8 + 2 * t;
-        *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
-        *reinterpret_cast<float2*>(to + 64) = make_float2(x[2], x[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<float2*>(logits + (size_t)(first + g + 8 * e) * 8 + 2 * t) = make_float2(x[e >> 1][2 * (e & 1)], x[e >> 1][2 * (e & 1) + 1]);
       }
 
-      // -- the values' pairs of slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9, and the largest scale of the tile --
-      uint32_t vp[4][G];
-      uint32_t largest = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        lds_words(pairs_at + T::kPairBytes + (uint32_t)((2 * t + (j & 1) + 8 * (j >> 1)) * G * 4), vp[j]);
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) largest = __vmaxu2(largest, vp[j][gr] & 0x00007fffu);
-      }
-      const uint32_t now = max(exponent, min(__reduce_max_sync(0xffffffffu, largest) >> 10, 30u));
       // -- running maximum and unit; both rarely change --
-      const bool grows = fmaxf(x[0], x[2]) > m_run[0] || fmaxf(x[1], x[3]) > m_run[1];
+      // A weight may exceed 1 by e^kSlack: rescaling the outputs at every new maximum would happen in most tiles while a
+      // warp has seen few. The largest value scale of the tile: pairs compared as halves.
+      constexpr float kSlack = 4.0f;
+      __half2 largest = __float2half2_rn(0.0f);
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        const uint32_t pw_ = lds32(pairs_at + T::kPairBytes + (uint32_t)(lane + 32 * j) * 4);
+        largest = __hmax2(largest, *reinterpret_cast<const __half2*>(&pw_));
+      }
+      const uint32_t largest_bits = *reinterpret_cast<const uint32_t*>(&largest) & 0x7fffu;
+      const uint32_t now = max(exponent, min(__reduce_max_sync(0xffffffffu, largest_bits) >> 10, 30u));
+      float tops[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) tops[e] = fmaxf(fmaxf(x[0][e], x[0][2 + e]), fmaxf(x[1][e], x[1][2 + e]));
+      const bool grows = tops[0] > m_run[0] + kSlack || tops[1] > m_run[1] + kSlack;
       if (__any_sync(0xffffffffu, grows) || now != exponent) {
         float alpha[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(x[e], x[e + 2]);
+          float top = tops[e];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           top = fmaxf(m_run[e], top);
@@ -579,54 +603,66 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
           }
         }
       }
-      float pr[4];
+      // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (+ 16), in units of the value scales
+      float pw[2][4];
+      const float to_units = __int_as_float((int)(150 - exponent) << 23);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = exp2f((x[e] - m_use[e & 1]) * kLog2e);
-      l_run[0] += pr[0] + pr[2];
-      l_run[1] += pr[1] + pr[3];
-      // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9, in units of the value scales
-      float pw[4];
-      const float to_units = __int_as_float((int)(156 - exponent) << 23);
+      for (int side = 0; side < 2; ++side) {
+        float pr[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t c0 = __float_as_uint(pr[2 * e]), c1 = __float_as_uint(pr[2 * e + 1]);
-        const uint32_t lo = transposed8x8(__byte_perm(c0, c1, 0x5410)), hi = transposed8x8(__byte_perm(c0, c1, 0x7632));
-        pw[2 * e] = __uint_as_float(__byte_perm(lo, hi, 0x5410)) * to_units;
-        pw[2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632)) * to_units;
-      }
-      if (guard) {
+        for (int e = 0; e < 4; ++e) pr[e] = exp2f((x[side][e] - m_use[e & 1]) * kLog2e);
+        l_run[0] += pr[0] + pr[2];
+        l_run[1] += pr[1] + pr[3];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int gr = 0; gr < G; ++gr) vp[j][gr] = pw[j] == 0.0f ? 0u : vp[j][gr];
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t c0 = __float_as_uint(pr[2 * e]), c1 = __float_as_uint(pr[2 * e + 1]);
+          const uint32_t lo = transposed8x8(__byte_perm(c0, c1, 0x5410)), hi = transposed8x8(__byte_perm(c0, c1, 0x7632));
+          pw[side][2 * e] = __uint_as_float(__byte_perm(lo, hi, 0x5410)) * to_units;
+          pw[side][2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632)) * to_units;
+        }
       }
       // -- outputs: channels by slots times slots by rows; a weight is two fp16 numbers --
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        float ps[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = pair_floats(vp[j][gr]);
-          ps[j] = pw[j] * f.x;
-          least_sum[gr] = fmaf(pw[j], f.y, least_sum[gr]);
-        }
-        uint32_t high[2], low[2];
-        split_halves(ps[0], ps[1], high[0], low[0]);
-        split_halves(ps[2], ps[3], high[1], low[1]);
-        uint32_t words[4];
+      for (int side = 0; side < 2; ++side) {
+        uint32_t vp[4][G];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          words[j] = lds32(at + T::kNibbleBytes + (val_at[j & 1] ^ (uint32_t)(gr * (BLOCK / 2))) + (j >> 1) * 4 * H);
+          lds_words(pairs_at + T::kPairBytes + (uint32_t)((16 * side + 2 * t + (j & 1) + 8 * (j >> 1)) * G * 4), vp[j]);
+        if (guard) {
 #pragma unroll
-        for (int half = 0; half < kTiles / 2; ++half) {
-          const uint32_t select = BLOCK == 32 ? val_select : half ? 0x7632u : 0x5410u;
-          const uint32_t a = __byte_perm(words[0], words[1], select), c = __byte_perm(words[2], words[3], select);
-          const uint32_t a8 = a >> 8, c8 = c >> 8;
-          float (&o0)[4] = o[gr][2 * half], (&o1)[4] = o[gr][2 * half + 1];
-          mma_f16(o0, a & kLowNibbles, a & kHighNibbles, c & kLowNibbles, c & kHighNibbles, high[0], high[1]);
-          mma_f16(o1, a8 & kLowNibbles, a8 & kHighNibbles, c8 & kLowNibbles, c8 & kHighNibbles, high[0], high[1]);
-          mma_f16(o0, a & kLowNibbles, a & kHighNibbles, c & kLowNibbles, c & kHighNibbles, low[0], low[1]);
-          mma_f16(o1, a8 & kLowNibbles, a8 & kHighNibbles, c8 & kLowNibbles, c8 & kHighNibbles, low[0], low[1]);
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) vp[j][gr] = pw[side][j] == 0.0f ? 0u : vp[j][gr];
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+          float ps[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = pair_floats(vp[j][gr]);
+            ps[j] = pw[side][j] * f.x;
+            least_sum[gr] = fmaf(pw[side][j], fmaf(8.0f, f.x, f.y), least_sum[gr]);
+          }
+          uint32_t high[2], low[2];
+          split_halves(ps[0], ps[1], high[0], low[0]);
+          split_halves(ps[2], ps[3], high[1], low[1]);
+          uint32_t words[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            words[j] = lds32(at + T::kNibbleBytes + (val_at[j & 1] ^ (uint32_t)(gr * (BLOCK / 2))) + (2 * side + (j >> 1)) * 4 * H);
+#pragma unroll
+          for (int half = 0; half < kTiles / 2; ++half) {
+            const uint32_t select = BLOCK == 32 ? val_select : half ? 0x7632u : 0x5410u;
+            const uint32_t a = __byte_perm(words[0], words[1], select), c = __byte_perm(words[2], words[3], select);
+            const uint32_t a8 = a >> 8, c8 = c >> 8;
+            const uint32_t e0 = centred_low(a), e1 = centred_high(a), e2 = centred_low(c), e3 = centred_high(c);
+            const uint32_t f0 = centred_low(a8), f1 = centred_high(a8), f2 = centred_low(c8), f3 = centred_high(c8);
+            float (&o0)[4] = o[gr][2 * half], (&o1)[4] = o[gr][2 * half + 1];
+            mma_f16(o0, e0, e1, e2, e3, high[0], high[1]);
+            mma_f16(o1, f0, f1, f2, f3, high[0], high[1]);
+            mma_f16(o0, e0, e1, e2, e3, low[0], low[1]);
+            mma_f16(o1, f0, f1, f2, f3, low[0], low[1]);
+          }
         }
       }
     }
@@ -644,7 +680,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     }
     __syncthreads();  // (also: no ring is read any more)
     if (w < busy) {
-      const float from_units = __int_as_float((int)(98 + exponent) << 23);  // 2^(exponent - 29)
+      const float from_units = __int_as_float((int)(104 + exponent) << 23);  // 2^(exponent - 23)
       float mine_f[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -663,12 +699,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
         if (t == 0) s_acc[w][g][gr] = sum * f_row;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float low = mine_f[e] * 0x1p24f, high = mine_f[e] * 0x1p20f;
           float* dst = part + (2 * t + e) * T::kRec + gr * BLOCK + g * (2 * kTiles);
 #pragma unroll
           for (int i = 0; i < kTiles; i += 2)
             *reinterpret_cast<float4*>(dst + 2 * i) =
-                make_float4(o[gr][i][e] * low, o[gr][i][2 + e] * high, o[gr][i + 1][e] * low, o[gr][i + 1][2 + e] * high);
+                make_float4(o[gr][i][e] * mine_f[e], o[gr][i][2 + e] * mine_f[e], o[gr][i + 1][e] * mine_f[e], o[gr][i + 1][2 + e] * mine_f[e]);
         }
       }
     }
@@ -728,7 +763,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
   int total, below;
   kv4_count_units(p, per, b, lane, &total, &below);
   const Pieces cut(total, split_ctas, min_units);
-  const int length = kv4_length(p, b), units = units_of(length);
+  const int length = kv4_length(p, b), units = tiles_of(length);
   auto records = [&](int in_b, int* count) {
     *count = 0;
     if (units == 0) return (const float*)nullptr;
@@ -781,7 +816,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
   const int at = blockIdx.x - p.n * p.t, kvh = at / ranges, slot0 = at % ranges * kScoreSlots;
   pdl_wait();
   if (slot0 >= length) return;
-  const size_t pitch = (size_t)(units_of(p.cache.s) * kUnit) * 8;
+  const size_t pitch = (size_t)tiles_of(p.cache.s) * kSlots * 8;
   float sums[kScoreSlots / kMergeThreads];
 #pragma unroll
   for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) sums[j] = 0.0f;
@@ -833,17 +868,17 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
 }
 
 // Shortest piece worth a CTA of its own: a tile for every warp.
-constexpr int kv4_min_units(int h) { return h == 256 ? 8 : 16; }
+constexpr int kv4_min_units(int h) { return h == 256 ? 8 : h == 128 ? 12 : 16; }
 // CTAs of a launch: one per SM, fewer when even full caches give no piece for some.
 int kv4_ctas(long long pairs, int s, int h) {
-  const long long most = pairs * ((s + kUnit - 1) / kUnit), n = (most + kv4_min_units(h) - 1) / kv4_min_units(h);
+  const long long most = pairs * tiles_of(s), n = (most + kv4_min_units(h) - 1) / kv4_min_units(h);
   const int sms = device_sm_count();
   return n < sms ? (int)n : sms;
 }
 
 bool kv4_tensor_shape(int b, int t, int n, int nkv, int h, int s) {
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
-  return (h == 64 || h == 128 || h == 256) && pairs * ((s + kUnit - 1) / kUnit) <= INT32_MAX &&
+  return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX &&
          (long long)n * t + (long long)nkv * ((s + kScoreSlots - 1) / kScoreSlots) <= INT32_MAX;
 }
 
@@ -885,7 +920,7 @@ size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int 
   if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return any * sizeof(float);
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
   const size_t tensor = kv4_records_floats(kv4_ctas(pairs, s, h), pairs, h) +
-                        (scores ? (size_t)pairs * ((s + kUnit - 1) / kUnit * kUnit) * 8 : 0);
+                        (scores ? (size_t)pairs * tiles_of(s) * kSlots * 8 : 0);
   return (any > tensor ? any : tensor) * sizeof(float);
 }
 
