@@ -199,10 +199,16 @@ __device__ __forceinline__ void kv4_count_units(const Kv4Sdpa& p, int per, int b
   *below = (int)__reduce_add_sync(0xffffffffu, (unsigned)low);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -214,6 +220,28 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
+}
+// Four 8 x 8 matrices of 16-bit elements, lane l naming row l % 8 of matrix l / 8: thread (g, t) receives elements 2 t and
+// 2 t + 1 of row g; transposed, elements g of rows 2 t and 2 t + 1.
+__device__ __forceinline__ void load_matrices(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(a));
+}
+// D(16 x 8) += A(16 x 16) B(16 x 8). (Not volatile: products of different chains may be interleaved.)
+__device__ __forceinline__ void product(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 2^x; results below 2^-126 are zero.
+__device__ __forceinline__ float power2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 template <int N>
 __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
@@ -244,20 +272,14 @@ __device__ __forceinline__ void split_halves(float a, float b, uint32_t& high, u
   low = halves(a - r.x, b - r.y);
 }
 
-// Where in a tile's nibbles the 16-byte piece c of a row lies. Rows follow one another; within each 128 bytes the pieces
-// are exchanged by an XOR such that the fragment loads below touch 32 banks: of the keys, a load takes one or two
-// neighbouring pieces of rows 0 .. 7, of the values of rows 0, 2, 4, 6 (or 1, 3, 5, 7). Rows r and r + 8 are exchanged
-// alike, and c only enters through an XOR of bits 4 to 6.
-template <int H, bool VALUES>
+// Where in a tile's nibbles the 16-byte piece c (32 channels) of a row lies. Rows follow one another; within each 128 bytes
+// the pieces are exchanged by an XOR such that piece c of rows 8 i .. 8 i + 7 touches 32 banks. Rows r and r + 8 are
+// exchanged alike, and c only enters through an XOR of bits 4 to 6.
+template <int H>
 __device__ __forceinline__ uint32_t piece_at(int row, int c) {
   constexpr int kRows = 256 / H;  // per 128 bytes
   const int line = row / kRows, pos = (row % kRows) * (H / 32) + c;
-  int x;
-  if (VALUES) {
-    x = H == 256 ? row & 7 : H == 128 ? (line & 3) << 1 : (line & 1) << 1;
-  } else {
-    x = H == 256 ? ((row & 3) << 1) | ((row >> 2) & 1) : H == 128 ? ((line & 1) << 1) | ((line >> 1) & 1) : line & 1;
-  }
+  const int x = H == 256 ? row & 7 : H == 128 ? ((line & 1) << 1) | ((line >> 1) & 1) : line & 1;
   return (uint32_t)(line * 128 + ((pos ^ x) << 4));
 }
 
@@ -279,8 +301,8 @@ template <int H, int BLOCK, bool QF32>
 __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, const int min_units, float* logits_ws) {
   using T = Kv4Tile<H, BLOCK>;
   constexpr int G = T::kG, W = T::kWarps;
-  constexpr int kKeySlots = H / 32;                          // key words per thread and row
-  constexpr int kTiles = BLOCK == 64 ? 4 : 2;                // 16-channel tiles of the second product per block
+  constexpr int P = H / 32;           // 16-byte pieces of a row
+  constexpr int kPer = BLOCK / 32;    // of them in a block
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
   __shared__ int s_pair[4];            // sequence, pair within it, first tile, tiles
@@ -326,16 +348,14 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
   int b = s_pair[0], in_b = s_pair[1], unit = s_pair[2];
   int len = kv4_length(p, b);
 
-  // this warp's ring, and where a lane's copies go
+  // this warp's ring; where a lane's copies come from and go to (16-byte piece `lane % P` of rows lane / P + 32 / P j)
   const uint32_t ring = smem_u32(smem) + (uint32_t)(w * T::kStages * T::kBytes);
-  constexpr int kPieces = H / 32, kCopies = H / 32;  // 16-byte pieces of a row; copies per lane of a tile's keys
-  const int copy_row = lane / kPieces, copy_piece = lane % kPieces;
   const size_t row_pitch = (size_t)nkv * (H / 2), pair_pitch = (size_t)nkv * G;  // bytes; pairs
-  // fragment places (see piece_at)
-  const uint32_t key_at = BLOCK == 64 ? piece_at<H, false>(g, t >> 1) + (uint32_t)(t & 1) * 8 : piece_at<H, false>(g, 0) + (uint32_t)t * 4;
-  const uint32_t val_piece = BLOCK == 64 ? (uint32_t)(g >> 2) : 0u, val_byte = BLOCK == 64 ? (uint32_t)(g & 3) * 4 : (uint32_t)(g >> 1) * 4;
-  const uint32_t val_at[2] = {piece_at<H, true>(2 * t, val_piece) + val_byte, piece_at<H, true>(2 * t + 1, val_piece) + val_byte};
-  const uint32_t val_select = (g & 1) ? 0x7632u : 0x5410u;  // blocks of 32: which half of the word this thread's channels are
+  const int copy_row = lane / P, copy_piece = lane % P;
+  const size_t copy_from = copy_row * row_pitch + copy_piece * 16;
+  const size_t pair_from = (lane / G) * pair_pitch + lane % G;
+  // the row that this lane names for a load of matrices: of two pieces, rows 0 .. 15
+  const uint32_t matrix_at = piece_at<H>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
 
   while (left > 0) {
     const int seg = min(left, tiles_of(len) - unit);
@@ -347,51 +367,68 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     const uint8_t* v_base = p.cache.v + (slot0 * nkv + kvh) * (H / 2);
     const __half2* kp_base = p.cache.k_pairs + (slot0 * nkv + kvh) * G;
     const __half2* vp_base = p.cache.v_pairs + (slot0 * nkv + kvh) * G;
-    // Requests this warp's tile k: rows behind the length arrive as zeros.
-    auto request = [&](int k) {
-      if (k < mine) {
-        const int first = (unit + w + k * W) * kSlots, there = len - first;
-        const uint32_t to = ring + (uint32_t)(k % T::kStages) * T::kBytes;
-        const uint8_t* ks = k_base + (size_t)first * row_pitch;
-        const uint8_t* vs = v_base + (size_t)first * row_pitch;
+    // Requests this warp's next tile: rows behind the length arrive as zeros.
+    int asked = 0;
+    uint32_t to = ring;
+    const uint8_t* k_next = k_base + (size_t)(unit + w) * kSlots * row_pitch + copy_from;
+    const uint8_t* v_next = v_base + (size_t)(unit + w) * kSlots * row_pitch + copy_from;
+    const __half2* kp_next = kp_base + (size_t)(unit + w) * kSlots * pair_pitch + pair_from;
+    const __half2* vp_next = vp_base + (size_t)(unit + w) * kSlots * pair_pitch + pair_from;
+    auto request = [&]() {
+      if (asked < mine) {
+        const int there = len - (unit + w + asked * W) * kSlots;
+        if (there >= kSlots) {
 #pragma unroll
-        for (int j = 0; j < kCopies; ++j) {
-          const int row = copy_row + j * (1024 / H);
-          const bool ok = row < there;
-          const size_t from = (ok ? row * row_pitch : 0) + (size_t)copy_piece * 16;
-          cp_async16(to + piece_at<H, false>(row, copy_piece), ks + from, ok);
-          cp_async16(to + T::kNibbleBytes + piece_at<H, true>(row, copy_piece), vs + from, ok);
-        }
-        const __half2* kps = kp_base + (size_t)first * pair_pitch;
-        const __half2* vps = vp_base + (size_t)first * pair_pitch;
+          for (int j = 0; j < P; ++j) {
+            cp_async16(to + piece_at<H>(copy_row + j * (32 / P), copy_piece), k_next + j * (32 / P) * row_pitch);
+            cp_async16(to + T::kNibbleBytes + piece_at<H>(copy_row + j * (32 / P), copy_piece), v_next + j * (32 / P) * row_pitch);
+          }
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-          const int e = lane + 32 * j, row = e / G;
-          const bool ok = row < there;
-          const size_t from = (ok ? row * pair_pitch : 0) + e % G;
-          cp_async4(to + 2 * T::kNibbleBytes + e * 4, kps + from, ok);
-          cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + e * 4, vps + from, ok);
+          for (int j = 0; j < G; ++j) {
+            cp_async4(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, kp_next + j * (32 / G) * pair_pitch);
+            cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, vp_next + j * (32 / G) * pair_pitch);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            const int row = copy_row + j * (32 / P);
+            const bool ok = row < there;
+            cp_async16_or_zero(to + piece_at<H>(row, copy_piece), ok ? k_next + j * (32 / P) * row_pitch : k_base, ok);
+            cp_async16_or_zero(to + T::kNibbleBytes + piece_at<H>(row, copy_piece), ok ? v_next + j * (32 / P) * row_pitch : v_base, ok);
+          }
+#pragma unroll
+          for (int j = 0; j < G; ++j) {
+            const bool ok = (lane + 32 * j) / G < there;
+            cp_async4_or_zero(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, ok ? kp_next + j * (32 / G) * pair_pitch : kp_base, ok);
+            cp_async4_or_zero(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, ok ? vp_next + j * (32 / G) * pair_pitch : vp_base, ok);
+          }
         }
+        k_next += W * kSlots * row_pitch;
+        v_next += W * kSlots * row_pitch;
+        kp_next += W * kSlots * pair_pitch;
+        vp_next += W * kSlots * pair_pitch;
+        to = to + T::kBytes == ring + T::kStages * T::kBytes ? ring : to + T::kBytes;
+        ++asked;
       }
       cp_async_commit();
     };
 #pragma unroll
-    for (int k = 0; k < T::kStages - 1; ++k) request(k);
+    for (int k = 0; k < T::kStages - 1; ++k) request();
 
     // Queries: thread (g, t) holds row g's elements at its words of a key, as the B operand. They are scaled by a power of
     // two that brings the row's largest to 2^10 .. 2^11: dividing by 16 then loses nothing above 2^-36 of it, and a float32
     // query is two fp16 numbers to 22 bits.
-    uint32_t q_high[kKeySlots][4], q_low[QF32 ? kKeySlots : 1][4];
+    uint32_t q_high[P][4], q_low[QF32 ? P : 1][4];
     float q_sum[G][2], factor[2];  // of the rows 2 t and 2 t + 1 (the products' columns)
     int limit[2];
     {
       const int r = chunk * 8 + g;
       const int i = r / rw.group;
       const size_t at = (((size_t)b * p.t + i) * p.n + kvh * rw.group + r % rw.group) * H;
-      float raw[kKeySlots][8], top = 0.0f;
+      float raw[P][8], top = 0.0f;
 #pragma unroll
-      for (int sl = 0; sl < kKeySlots; ++sl) {
-        const int word = BLOCK == 64 ? 8 * (sl / 2) + 2 * t + sl % 2 : 4 * sl + t;
+      for (int sl = 0; sl < P; ++sl) {
+        const int word = 4 * sl + t;
         if (r >= rw.rows) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) raw[sl][e] = 0.0f;
@@ -418,11 +455,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) sums[gr] = 0.0f;
 #pragma unroll
-      for (int sl = 0; sl < kKeySlots; ++sl) {
+      for (int sl = 0; sl < P; ++sl) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           raw[sl][e] *= scale_up;
-          sums[BLOCK == 64 ? sl / 2 : sl] += raw[sl][e];
+          sums[sl / kPer] += raw[sl][e];
         }
         // channels 0, 4 | 2, 6 meet low nibbles, 1, 5 | 3, 7 high ones
 #pragma unroll
@@ -453,9 +490,10 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = chunk * 8 + 2 * t + e, i = r / rw.group;
-      limit[e] = r < rw.rows ? kv4_limit(len, s_max, p.t, i) : 0;
+      limit[e] = r < rw.rows ? kv4_limit(len, s_max, p.t, i) : len;  // (columns without a row are computed and dropped)
       mask[e] = p.mask && r < rw.rows ? p.mask + ((size_t)b * p.t + i) * s_max : nullptr;
     }
+    const int least_limit = kv4_limit(len, s_max, p.t, chunk * 8 / rw.group);  // of any row
     // masks are requested a tile ahead of their use
     auto masks = [&](int k, float (&m)[2][4]) {
       const int first = (unit + w + k * W) * kSlots;
@@ -472,59 +510,72 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     const bool guard = p.mask != nullptr || p.t > 1;  // slots that some row does not see may hold anything
     float* logits = logits_ws ? logits_ws + pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
 
-    float o[G][kTiles][4], least_sum[G];
+    // outputs: of piece i and its channels 4 g + {0, 1} and 4 g + {2, 3}, rows 2 t and 2 t + 1
+    float o[P][2][4], least_sum[G];
 #pragma unroll
-    for (int gr = 0; gr < G; ++gr) {
-      least_sum[gr] = 0.0f;
+    for (int gr = 0; gr < G; ++gr) least_sum[gr] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) o[gr][i][0] = o[gr][i][1] = o[gr][i][2] = o[gr][i][3] = 0.0f;
-    }
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][0][e] = o[i][1][e] = 0.0f;
     float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, m_use[2] = {0.0f, 0.0f}, l_run[2] = {0.0f, 0.0f};
     uint32_t exponent = 1;  // fp16 exponent field of the largest value scale so far: weights are in units of 2^(exponent - 23)
 
+    uint32_t at = ring;
 #pragma unroll 1
-    for (int k = 0; k < mine; ++k) {
+    for (int k = 0; k < mine; ++k, at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes) {
       cp_async_wait<T::kStages - 2>();
       __syncwarp();  // the tile is there, and everybody is done with the one whose place the next request takes
-      request(k + T::kStages - 1);
-      const uint32_t at = ring + (uint32_t)(k % T::kStages) * T::kBytes;
+      request();
       const uint32_t pairs_at = at + 2 * T::kNibbleBytes;
       const int first = (unit + w + k * W) * kSlots;
 
       // -- logits of slots g, g + 8 (+ 16), rows 2 t and 2 t + 1 --
       float x[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+      // Four pieces and both sides at a time, one product of each chain after the other: a warp waits for a chain's last
+      // product before its next.
+      constexpr int kAtOnce = P < 4 ? P : 4, kChains = kAtOnce / kPer;
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        uint32_t pa[G], pb[G];
-        lds_words(pairs_at + (uint32_t)((16 * side + g) * G * 4), pa);
-        lds_words(pairs_at + (uint32_t)((16 * side + g + 8) * G * 4), pb);
+      for (int i0 = 0; i0 < P; i0 += kAtOnce) {
+        uint32_t words[2][kAtOnce / 2][4];
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          constexpr int kN = BLOCK / 32;  // words of this block per thread and row
-          uint32_t wa[kN], wb[kN];
-          const uint32_t from = at + (key_at ^ (uint32_t)(gr * (BLOCK / 2))) + side * 8 * H;
-          lds_words(from, wa);
-          lds_words(from + 4 * H, wb);
-          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < kAtOnce; i += 2)
 #pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            const int sl = gr * kN + j;
-            const uint32_t a8 = wa[j] >> 8, b8 = wb[j] >> 8;
-            const uint32_t l0 = wa[j] & kLowNibbles, l1 = wb[j] & kLowNibbles, l2 = a8 & kLowNibbles, l3 = b8 & kLowNibbles;
-            const uint32_t h0 = wa[j] & kHighNibbles, h1 = wb[j] & kHighNibbles, h2 = a8 & kHighNibbles, h3 = b8 & kHighNibbles;
-            mma_f16(acc, l0, l1, l2, l3, q_high[sl][0], q_high[sl][1]);
-            mma_f16(acc, h0, h1, h2, h3, q_high[sl][2], q_high[sl][3]);
-            if constexpr (QF32) {
-              mma_f16(acc, l0, l1, l2, l3, q_low[sl][0], q_low[sl][1]);
-              mma_f16(acc, h0, h1, h2, h3, q_low[sl][2], q_low[sl][3]);
-            }
-          }
-          const float2 fa = pair_floats(pa[gr]), fb = pair_floats(pb[gr]);
-          x[side][0] = fmaf(fa.x, acc[0], fmaf(fa.y, q_sum[gr][0], x[side][0]));
-          x[side][1] = fmaf(fa.x, acc[1], fmaf(fa.y, q_sum[gr][1], x[side][1]));
-          x[side][2] = fmaf(fb.x, acc[2], fmaf(fb.y, q_sum[gr][0], x[side][2]));
-          x[side][3] = fmaf(fb.x, acc[3], fmaf(fb.y, q_sum[gr][1], x[side][3]));
+          for (int side = 0; side < 2; ++side)
+            load_matrices(at + (matrix_at ^ (uint32_t)((i0 + i) * 16)) + side * 8 * H, words[side][i / 2]);
+        float acc[2][kChains][4];
+#pragma unroll
+        for (int side = 0; side < 2; ++side)
+#pragma unroll
+          for (int c = 0; c < kChains; ++c) acc[side][c][0] = acc[side][c][1] = acc[side][c][2] = acc[side][c][3] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+#pragma unroll
+          for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+            for (int c = 0; c < kChains; ++c)
+#pragma unroll
+              for (int side = 0; side < 2; ++side) {
+                const int i = c * kPer + j;
+                const uint32_t wa = words[side][i / 2][2 * (i & 1)], wb = words[side][i / 2][2 * (i & 1) + 1];
+                const uint32_t keep = odd ? kHighNibbles : kLowNibbles;
+                const uint32_t a0 = wa & keep, a1 = wb & keep, a2 = (wa >> 8) & keep, a3 = (wb >> 8) & keep;
+                product(acc[side][c], a0, a1, a2, a3, q_high[i0 + i][2 * odd], q_high[i0 + i][2 * odd + 1]);
+                if constexpr (QF32) product(acc[side][c], a0, a1, a2, a3, q_low[i0 + i][2 * odd], q_low[i0 + i][2 * odd + 1]);
+              }
         }
+#pragma unroll
+        for (int c = 0; c < kChains; ++c)
+#pragma unroll
+          for (int side = 0; side < 2; ++side) {
+            const int gr = i0 / kPer + c;
+            const float2 fa = pair_floats(lds32(pairs_at + (uint32_t)(((16 * side + g) * G + gr) * 4)));
+            const float2 fb = pair_floats(lds32(pairs_at + (uint32_t)(((16 * side + g + 8) * G + gr) * 4)));
+            x[side][0] = fmaf(fa.x, acc[side][c][0], fmaf(fa.y, q_sum[gr][0], x[side][0]));
+            x[side][1] = fmaf(fa.x, acc[side][c][1], fmaf(fa.y, q_sum[gr][1], x[side][1]));
+            x[side][2] = fmaf(fb.x, acc[side][c][2], fmaf(fb.y, q_sum[gr][0], x[side][2]));
+            x[side][3] = fmaf(fb.x, acc[side][c][3], fmaf(fb.y, q_sum[gr][1], x[side][3]));
+          }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] *= factor[e & 1];
@@ -543,10 +594,12 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
           x[e >> 2][e & 3] = a == -CUDART_INF_F ? a : x[e >> 2][e & 3] + a;
         }
       }
+      if (first + kSlots > least_limit) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int slot = first + 16 * (e >> 2) + g + 8 * ((e >> 1) & 1);
-        x[e >> 2][e & 3] = slot < limit[e & 1] ? x[e >> 2][e & 3] : -CUDART_INF_F;
+        for (int e = 0; e < 8; ++e) {
+          const int slot = first + 16 * (e >> 2) + g + 8 * ((e >> 1) & 1);
+          x[e >> 2][e & 3] = slot < limit[e & 1] ? x[e >> 2][e & 3] : -CUDART_INF_F;
+        }
       }
       if (logits) {
 #pragma unroll
@@ -579,7 +632,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           top = fmaxf(m_run[e], top);
           const float use = top == -CUDART_INF_F ? 0.0f : top;
-          alpha[e] = m_run[e] == -CUDART_INF_F ? 0.0f : exp2f((m_run[e] - use) * kLog2e);
+          alpha[e] = m_run[e] == -CUDART_INF_F ? 0.0f : power2((m_run[e] - use) * kLog2e);
           m_run[e] = top;
           m_use[e] = use;
           l_run[e] *= alpha[e];
@@ -592,16 +645,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
         alpha[0] *= shrink;
         alpha[1] *= shrink;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          least_sum[gr] *= mine_alpha;
+        for (int gr = 0; gr < G; ++gr) least_sum[gr] *= mine_alpha;
 #pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            o[gr][i][0] *= alpha[0];
-            o[gr][i][1] *= alpha[1];
-            o[gr][i][2] *= alpha[0];
-            o[gr][i][3] *= alpha[1];
-          }
-        }
+        for (int i = 0; i < 2 * P; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i >> 1][i & 1][e] *= alpha[e & 1];
       }
       // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (+ 16), in units of the value scales
       float pw[2][4];
@@ -610,7 +658,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       for (int side = 0; side < 2; ++side) {
         float pr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = exp2f((x[side][e] - m_use[e & 1]) * kLog2e);
+        for (int e = 0; e < 4; ++e) pr[e] = power2((x[side][e] - m_use[e & 1]) * kLog2e);
         l_run[0] += pr[0] + pr[2];
         l_run[1] += pr[1] + pr[3];
 #pragma unroll
@@ -634,6 +682,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) vp[j][gr] = pw[side][j] == 0.0f ? 0u : vp[j][gr];
         }
+        uint32_t high[G][2], low[G][2];
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
           float ps[4];
@@ -643,25 +692,27 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
             ps[j] = pw[side][j] * f.x;
             least_sum[gr] = fmaf(pw[side][j], fmaf(8.0f, f.x, f.y), least_sum[gr]);
           }
-          uint32_t high[2], low[2];
-          split_halves(ps[0], ps[1], high[0], low[0]);
-          split_halves(ps[2], ps[3], high[1], low[1]);
-          uint32_t words[4];
+          split_halves(ps[0], ps[1], high[gr][0], low[gr][0]);
+          split_halves(ps[2], ps[3], high[gr][1], low[gr][1]);
+        }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            words[j] = lds32(at + T::kNibbleBytes + (val_at[j & 1] ^ (uint32_t)(gr * (BLOCK / 2))) + (2 * side + (j >> 1)) * 4 * H);
+        for (int i = 0; i < P; i += 2) {
+          uint32_t words[4], e[4][4];
+          load_matrices_transposed(at + T::kNibbleBytes + (matrix_at ^ (uint32_t)(i * 16)) + side * 8 * H, words);
 #pragma unroll
-          for (int half = 0; half < kTiles / 2; ++half) {
-            const uint32_t select = BLOCK == 32 ? val_select : half ? 0x7632u : 0x5410u;
-            const uint32_t a = __byte_perm(words[0], words[1], select), c = __byte_perm(words[2], words[3], select);
-            const uint32_t a8 = a >> 8, c8 = c >> 8;
-            const uint32_t e0 = centred_low(a), e1 = centred_high(a), e2 = centred_low(c), e3 = centred_high(c);
-            const uint32_t f0 = centred_low(a8), f1 = centred_high(a8), f2 = centred_low(c8), f3 = centred_high(c8);
-            float (&o0)[4] = o[gr][2 * half], (&o1)[4] = o[gr][2 * half + 1];
-            mma_f16(o0, e0, e1, e2, e3, high[0], high[1]);
-            mma_f16(o1, f0, f1, f2, f3, high[0], high[1]);
-            mma_f16(o0, e0, e1, e2, e3, low[0], low[1]);
-            mma_f16(o1, f0, f1, f2, f3, low[0], low[1]);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a = j & 1 ? words[j & 2] >> 8 : words[j & 2], c = j & 1 ? words[(j & 2) + 1] >> 8 : words[(j & 2) + 1];
+            e[j][0] = centred_low(a), e[j][1] = centred_high(a), e[j][2] = centred_low(c), e[j][3] = centred_high(c);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int gr = (i + (j >> 1)) / kPer;
+            product(o[i + (j >> 1)][j & 1], e[j][0], e[j][1], e[j][2], e[j][3], high[gr][0], high[gr][1]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int gr = (i + (j >> 1)) / kPer;
+            product(o[i + (j >> 1)][j & 1], e[j][0], e[j][1], e[j][2], e[j][3], low[gr][0], low[gr][1]);
           }
         }
       }
@@ -686,7 +737,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       for (int e = 0; e < 2; ++e) {
         float top = -CUDART_INF_F;
         for (int i = 0; i < busy; ++i) top = fmaxf(top, s_m[i][2 * t + e]);
-        mine_f[e] = m_run[e] == -CUDART_INF_F ? 0.0f : exp2f((m_run[e] - top) * kLog2e) * from_units;
+        mine_f[e] = m_run[e] == -CUDART_INF_F ? 0.0f : power2((m_run[e] - top) * kLog2e) * from_units;
       }
       const float even = __shfl_sync(0xffffffffu, mine_f[0], g >> 1), odd = __shfl_sync(0xffffffffu, mine_f[1], g >> 1);
       const float f_row = (g & 1) ? odd : even;
@@ -697,15 +748,13 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         if (t == 0) s_acc[w][g][gr] = sum * f_row;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float* dst = part + (2 * t + e) * T::kRec + gr * BLOCK + g * (2 * kTiles);
-#pragma unroll
-          for (int i = 0; i < kTiles; i += 2)
-            *reinterpret_cast<float4*>(dst + 2 * i) =
-                make_float4(o[gr][i][e] * mine_f[e], o[gr][i][2 + e] * mine_f[e], o[gr][i + 1][e] * mine_f[e], o[gr][i + 1][2 + e] * mine_f[e]);
-        }
       }
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float4*>(part + (2 * t + e) * T::kRec + i * 32 + g * 4) =
+              make_float4(o[i][0][e] * mine_f[e], o[i][0][2 + e] * mine_f[e], o[i][1][e] * mine_f[e], o[i][1][2 + e] * mine_f[e]);
     }
     __syncthreads();
     float* rec = p.ws + ((size_t)blockIdx.x + pair) * 8 * T::kRec;
@@ -726,7 +775,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     if (tid < rows) {
       float top = -CUDART_INF_F, sum = 0.0f;
       for (int j = 0; j < busy; ++j) top = fmaxf(top, s_m[j][tid]);
-      for (int j = 0; j < busy; ++j) sum += s_m[j][tid] == -CUDART_INF_F ? s_l[j][tid] : exp2f((s_m[j][tid] - top) * kLog2e) * s_l[j][tid];
+      for (int j = 0; j < busy; ++j) sum += s_m[j][tid] == -CUDART_INF_F ? s_l[j][tid] : power2((s_m[j][tid] - top) * kLog2e) * s_l[j][tid];
       *reinterpret_cast<float2*>(rec + tid * T::kRec + H) = make_float2(top, sum);
     }
     left -= seg;
