@@ -149,11 +149,17 @@ cudaError_t launch_rows(const Kv4Sdpa& p, cudaStream_t s) {
 
 // ---- head sizes 64, 128 and 256: tensor cores -------------------------------------------------------------
 // Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; a tile is 32 slots,
-// two 16-row sides of it whose chains of products and exponentials run side by side. A warp works on tiles of its own
-// from the first copy to the last product, with its own running maximum, sum and outputs: no barrier until the warps of
-// a CTA merge at the end of a piece. (pieces.cuh: how the slots are cut.)
+// two 16-row sides of it whose chains of products and exponentials run side by side. The tiles of all (sequence, KV head,
+// eight rows) pairs form one row, cut into equal pieces, one per warp, whatever the lengths are (pieces.cuh). A warp walks
+// through its piece without meeting another one. At its end the warps of a CTA add their states of a common pair to one
+// partial record (un-normalised outputs, maximum, sum); a warp that goes on to another pair writes a record of the first on
+// its own. A second kernel merges a pair's records.
+// 16 ragged sequences of up to 8192 tokens, 8 heads x 256, replayed: 20.3 us with a record per warp (the second kernel reads
+// 9.8 MB then), 19.4 with a piece per CTA (6 of them in the CTAs that had parts of two sequences one after the other).
 constexpr int kSlots = 32;
 __host__ __device__ inline int tiles_of(int slots) { return (slots + kSlots - 1) / kSlots; }
+
+__host__ __device__ constexpr int kv4_warps(int h) { return h == 256 ? 8 : h == 128 ? 12 : 16; }
 
 template <int H, int BLOCK>
 struct Kv4Tile {
@@ -161,14 +167,14 @@ struct Kv4Tile {
   static constexpr int kNibbleBytes = kSlots * H / 2;  // of the keys (or values) of a tile
   static constexpr int kPairBytes = kSlots * kG * 4;
   static constexpr int kBytes = 2 * (kNibbleBytes + kPairBytes);
-  static constexpr int kWarps = H == 256 ? 8 : H == 128 ? 12 : 16;
+  static constexpr int kWarps = kv4_warps(H);
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kRec = H + 4;  // floats of a record per row: outputs, maximum, sum, padding
-  static constexpr int kMerge = kWarps * 8 * kRec * 4;
   static constexpr int kFit = 220 * 1024 / (kWarps * kBytes);
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kRing = kWarps * kStages * kBytes;
-  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + 128;
+  static constexpr int kSmem = kRing + 128;
+  static_assert(8 * kRec * 4 <= kStages * kBytes, "a warp's state fits into its ring");
   static_assert(kBytes % 128 == 0 && kStages >= 2 && kSmem <= 221 * 1024, "layout");
 };
 
@@ -180,15 +186,15 @@ __host__ __device__ inline Kv4Rows kv4_rows(int t, int n, int nkv) {
   return {group, rows, (rows + 7) / 8};
 }
 
-// Workspace of the piecewise kernels: records, then the logits [pair][slot (rounded up to a tile)][8 rows] where scores
+// Workspace of the piecewise kernels: records (a piece and a pair name one), then the logits [pair][slot (rounded up to a tile)][8 rows] where scores
 // are wanted.
-__host__ __device__ inline size_t kv4_records_floats(int ctas, long long pairs, int h) { return ((size_t)ctas + (size_t)pairs) * 8 * (h + 4); }
+__host__ __device__ inline size_t kv4_records_floats(int pieces, long long pairs, int h) { return ((size_t)pieces + (size_t)pairs) * 8 * (h + 4); }
 
 __device__ __forceinline__ int kv4_length(const Kv4Sdpa& p, int b) {
   return p.lengths ? max(0, min(p.lengths[b], p.cache.s)) : p.cache.s;
 }
 // Tiles of all sequences' pairs, and of the sequences below `b`. Whole warp.
-__device__ __forceinline__ void kv4_count_units(const Kv4Sdpa& p, int per, int b, int lane, int* total, int* below) {
+__device__ __forceinline__ void kv4_count_tiles(const Kv4Sdpa& p, int per, int b, int lane, int* total, int* below) {
   int all = 0, low = 0;
   for (int i = lane; i < p.cache.b; i += 32) {
     const int u = tiles_of(kv4_length(p, i)) * per;
@@ -297,56 +303,65 @@ __device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t centred_low(uint32_t w) { return half2_sub((w & kLowNibbles) | 0x64006400u, 0x64086408u); }    // - 1032
 __device__ __forceinline__ uint32_t centred_high(uint32_t w) { return half2_sub((w & kHighNibbles) | 0x54005400u, 0x54805480u); }  // - 72
 
+// How many warps of a CTA get a piece: few tiles are spread over the CTAs first.
+__device__ __forceinline__ int kv4_busy_warps(int total, int ctas, int warps) { return max(1, min(warps, (total + ctas - 1) / ctas)); }
+
 template <int H, int BLOCK, bool QF32>
-__global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, const int min_units, float* logits_ws) {
+__global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, float* logits_ws) {
   using T = Kv4Tile<H, BLOCK>;
-  constexpr int G = T::kG, W = T::kWarps;
+  constexpr int G = T::kG;
   constexpr int P = H / 32;           // 16-byte pieces of a row
   constexpr int kPer = BLOCK / 32;    // of them in a block
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
-  __shared__ int s_pair[4];            // sequence, pair within it, first tile, tiles
-  __shared__ float s_m[W][8], s_l[W][8];
-  __shared__ float s_acc[W][8][G];     // what the least values contribute, per block
-  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  __shared__ float s_m[T::kWarps][8], s_l[T::kWarps][8];  // maxima and sums of the warps' last pairs
+  __shared__ long long s_pair[T::kWarps];                 // and which these are
+  __shared__ int s_rows[T::kWarps];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int nkv = p.cache.nkv, s_max = p.cache.s;
   const Kv4Rows rw = kv4_rows(p.t, p.n, nkv);
-  const int per = nkv * rw.chunks;     // pairs per sequence
+  const int per = nkv * rw.chunks;  // pairs per sequence
   pdl_wait();
   // (only now: what a dependent kernel does ahead of its own wait may then read this kernel's inputs)
   pdl_launch_dependents();
-  if (w == 0) {
-    int total, below;
-    kv4_count_units(p, per, 0, lane, &total, &below);
-    const Pieces cut(total, gridDim.x, min_units);
-    const int c = blockIdx.x;
-    const int u0 = c < cut.ctas ? cut.begin(c) : 0, u1 = c < cut.ctas ? cut.begin(c + 1) : 0;
-    int base = 0;
-    for (int b0 = 0; b0 < p.cache.b && u0 < u1; b0 += 32) {
-      const int units = b0 + lane < p.cache.b ? tiles_of(kv4_length(p, b0 + lane)) : 0;
-      int upto = units * per;  // inclusive prefix sum over the lanes
+  // this warp's piece, and the pair in which it starts
+  int len = lane < p.cache.b ? kv4_length(p, lane) : 0;
+  int total = tiles_of(len) * per, below;
+  if (p.cache.b <= 32) {
+    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+  } else {
+    kv4_count_tiles(p, per, 0, lane, &total, &below);
+  }
+  const int busy = kv4_busy_warps(total, gridDim.x, T::kWarps);
+  const Pieces cut(total, gridDim.x * busy, 1);
+  const int piece = blockIdx.x * busy + w;
+  int left = 0, b = 0, in_b = 0, unit = 0;
+  if (w < busy && piece < cut.ctas && total > 0) {
+    const int u0 = cut.begin(piece);
+    left = cut.begin(piece + 1) - u0;
+    for (int b0 = 0, base = 0;; b0 += 32) {
+      if (b0 > 0) len = b0 + lane < p.cache.b ? kv4_length(p, b0 + lane) : 0;
+      const int mine = tiles_of(len) * per;
+      int upto = mine;  // inclusive prefix sum over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
       }
-      const int mine = base + upto - units * per;
-      const bool here = units > 0 && mine <= u0 && u0 < mine + units * per;
-      if (here) {
-        s_pair[0] = b0 + lane;
-        s_pair[1] = (u0 - mine) / units;
-        s_pair[2] = (u0 - mine) % units;
+      const uint32_t here = __ballot_sync(0xffffffffu, base + upto > u0);
+      if (here) {  // (there is one: u0 < total)
+        const int src = __ffs(here) - 1;
+        const int from = __shfl_sync(0xffffffffu, base + upto - mine, src);
+        len = __shfl_sync(0xffffffffu, len, src);
+        b = b0 + src;
+        in_b = (u0 - from) / tiles_of(len);
+        unit = (u0 - from) % tiles_of(len);
+        break;
       }
-      if (__any_sync(0xffffffffu, here)) break;
       base += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) s_pair[3] = u1 - u0;
   }
-  __syncthreads();
-  int left = s_pair[3];
-  if (left == 0) return;
-  int b = s_pair[0], in_b = s_pair[1], unit = s_pair[2];
-  int len = kv4_length(p, b);
+  if (lane == 0) s_pair[w] = -1;  // no state yet
 
   // this warp's ring; where a lane's copies come from and go to (16-byte piece `lane % P` of rows lane / P + 32 / P j)
   const uint32_t ring = smem_u32(smem) + (uint32_t)(w * T::kStages * T::kBytes);
@@ -361,7 +376,6 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     const int seg = min(left, tiles_of(len) - unit);
     const int kvh = in_b / rw.chunks, chunk = in_b % rw.chunks;
     const size_t pair = (size_t)b * per + in_b;
-    const int mine = seg > w ? (seg - w + W - 1) / W : 0;  // tiles of this warp
     const size_t slot0 = (size_t)b * s_max;
     const uint8_t* k_base = p.cache.k + (slot0 * nkv + kvh) * (H / 2);
     const uint8_t* v_base = p.cache.v + (slot0 * nkv + kvh) * (H / 2);
@@ -370,13 +384,13 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     // Requests this warp's next tile: rows behind the length arrive as zeros.
     int asked = 0;
     uint32_t to = ring;
-    const uint8_t* k_next = k_base + (size_t)(unit + w) * kSlots * row_pitch + copy_from;
-    const uint8_t* v_next = v_base + (size_t)(unit + w) * kSlots * row_pitch + copy_from;
-    const __half2* kp_next = kp_base + (size_t)(unit + w) * kSlots * pair_pitch + pair_from;
-    const __half2* vp_next = vp_base + (size_t)(unit + w) * kSlots * pair_pitch + pair_from;
+    const uint8_t* k_next = k_base + (size_t)unit * kSlots * row_pitch + copy_from;
+    const uint8_t* v_next = v_base + (size_t)unit * kSlots * row_pitch + copy_from;
+    const __half2* kp_next = kp_base + (size_t)unit * kSlots * pair_pitch + pair_from;
+    const __half2* vp_next = vp_base + (size_t)unit * kSlots * pair_pitch + pair_from;
     auto request = [&]() {
-      if (asked < mine) {
-        const int there = len - (unit + w + asked * W) * kSlots;
+      if (asked < seg) {
+        const int there = len - (unit + asked) * kSlots;
         if (there >= kSlots) {
 #pragma unroll
           for (int j = 0; j < P; ++j) {
@@ -403,16 +417,16 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
             cp_async4_or_zero(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, ok ? vp_next + j * (32 / G) * pair_pitch : vp_base, ok);
           }
         }
-        k_next += W * kSlots * row_pitch;
-        v_next += W * kSlots * row_pitch;
-        kp_next += W * kSlots * pair_pitch;
-        vp_next += W * kSlots * pair_pitch;
+        k_next += kSlots * row_pitch;
+        v_next += kSlots * row_pitch;
+        kp_next += kSlots * pair_pitch;
+        vp_next += kSlots * pair_pitch;
         to = to + T::kBytes == ring + T::kStages * T::kBytes ? ring : to + T::kBytes;
         ++asked;
       }
       cp_async_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < T::kStages - 1; ++k) request();
 
     // Queries: thread (g, t) holds row g's elements at its words of a key, as the B operand. They are scaled by a power of
@@ -496,13 +510,13 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     const int least_limit = kv4_limit(len, s_max, p.t, chunk * 8 / rw.group);  // of any row
     // masks are requested a tile ahead of their use
     auto masks = [&](int k, float (&m)[2][4]) {
-      const int first = (unit + w + k * W) * kSlots;
+      const int first = (unit + k) * kSlots;
 #pragma unroll
       for (int side = 0; side < 2; ++side)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int slot = first + 16 * side + g + 8 * (e >> 1);
-          m[side][e] = mask[e & 1] && k < mine && slot < limit[e & 1] ? __ldg(mask[e & 1] + slot) : 0.0f;
+          m[side][e] = mask[e & 1] && k < seg && slot < limit[e & 1] ? __ldg(mask[e & 1] + slot) : 0.0f;
         }
     };
     float next_mask[2][4];
@@ -523,12 +537,12 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 
     uint32_t at = ring;
 #pragma unroll 1
-    for (int k = 0; k < mine; ++k, at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes) {
+    for (int k = 0; k < seg; ++k, at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes) {
       cp_async_wait<T::kStages - 2>();
       __syncwarp();  // the tile is there, and everybody is done with the one whose place the next request takes
       request();
       const uint32_t pairs_at = at + 2 * T::kNibbleBytes;
-      const int first = (unit + w + k * W) * kSlots;
+      const int first = (unit + k) * kSlots;
 
       // -- logits of slots g, g + 8 (+ 16), rows 2 t and 2 t + 1 --
       float x[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -719,68 +733,46 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     }
     cp_async_wait<0>();
 
-    // -- the warps' states become one record --
-    const int busy = min(W, seg);
+    // -- this pair's state: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
+    left -= seg;
+    const float from_units = __int_as_float((int)(104 + exponent) << 23);  // 2^(exponent - 23)
+    const int rows = min(8, rw.rows - chunk * 8);
+    // the last one to the warp's own part of the shared memory, another one straight to its record
+    float* rec = left > 0 ? p.ws + ((size_t)piece + pair) * 8 * T::kRec : reinterpret_cast<float*>(smem + w * T::kStages * T::kBytes);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], d);
-    if (g == 0) {
-      s_m[w][2 * t] = m_run[0], s_m[w][2 * t + 1] = m_run[1];
-      s_l[w][2 * t] = l_run[0], s_l[w][2 * t + 1] = l_run[1];
-    }
-    __syncthreads();  // (also: no ring is read any more)
-    if (w < busy) {
-      const float from_units = __int_as_float((int)(104 + exponent) << 23);  // 2^(exponent - 23)
-      float mine_f[2];
+    __syncwarp();  // (the ring is not read any more)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float top = -CUDART_INF_F;
-        for (int i = 0; i < busy; ++i) top = fmaxf(top, s_m[i][2 * t + e]);
-        mine_f[e] = m_run[e] == -CUDART_INF_F ? 0.0f : power2((m_run[e] - top) * kLog2e) * from_units;
-      }
-      const float even = __shfl_sync(0xffffffffu, mine_f[0], g >> 1), odd = __shfl_sync(0xffffffffu, mine_f[1], g >> 1);
-      const float f_row = (g & 1) ? odd : even;
-      float* part = reinterpret_cast<float*>(smem) + (size_t)w * 8 * T::kRec;
+    for (int gr = 0; gr < G; ++gr) {
+      float sum = least_sum[gr];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const float least[2] = {__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4)};
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        float sum = least_sum[gr];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (t == 0) s_acc[w][g][gr] = sum * f_row;
-      }
-#pragma unroll
-      for (int i = 0; i < P; ++i)
+      for (int i = gr * kPer; i < (gr + 1) * kPer; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float4*>(part + (2 * t + e) * T::kRec + i * 32 + g * 4) =
-              make_float4(o[i][0][e] * mine_f[e], o[i][0][2 + e] * mine_f[e], o[i][1][e] * mine_f[e], o[i][1][2 + e] * mine_f[e]);
+          if (2 * t + e < rows)
+            *reinterpret_cast<float4*>(rec + (2 * t + e) * T::kRec + i * 32 + g * 4) =
+                make_float4((o[i][0][e] + least[e]) * from_units, (o[i][0][2 + e] + least[e]) * from_units, (o[i][1][e] + least[e]) * from_units,
+                            (o[i][1][2 + e] + least[e]) * from_units);
     }
-    __syncthreads();
-    float* rec = p.ws + ((size_t)blockIdx.x + pair) * 8 * T::kRec;
-    const int rows = min(8, rw.rows - chunk * 8);
-    for (int i = tid; i < rows * (H / 4); i += T::kThreads) {
-      const int row = i / (H / 4), d = i % (H / 4) * 4;
-      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int j = 0; j < busy; ++j) {
-        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + ((size_t)j * 8 + row) * T::kRec + d);
-        const float a = s_acc[j][row][d / BLOCK];
-        sum.x += v.x + a;
-        sum.y += v.y + a;
-        sum.z += v.z + a;
-        sum.w += v.w + a;
+    if (g < 2 && 2 * t + g < rows) {
+      const float m = g ? m_run[1] : m_run[0], l = g ? l_run[1] : l_run[0];
+      if (left > 0) {
+        *reinterpret_cast<float2*>(rec + (2 * t + g) * T::kRec + H) = make_float2(m, l);
+      } else {
+        s_m[w][2 * t + g] = m;
+        s_l[w][2 * t + g] = l;
       }
-      *reinterpret_cast<float4*>(rec + row * T::kRec + d) = sum;
     }
-    if (tid < rows) {
-      float top = -CUDART_INF_F, sum = 0.0f;
-      for (int j = 0; j < busy; ++j) top = fmaxf(top, s_m[j][tid]);
-      for (int j = 0; j < busy; ++j) sum += s_m[j][tid] == -CUDART_INF_F ? s_l[j][tid] : power2((s_m[j][tid] - top) * kLog2e) * s_l[j][tid];
-      *reinterpret_cast<float2*>(rec + tid * T::kRec + H) = make_float2(top, sum);
+    if (lane == 0 && left == 0) {
+      s_pair[w] = (long long)pair;
+      s_rows[w] = rows;
     }
-    left -= seg;
     if (left > 0) {
-      __syncthreads();  // the next segment's copies go where the states were
       unit = 0;
       if (++in_b == per) {
         in_b = 0;
@@ -791,67 +783,168 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       }
     }
   }
+
+  // -- neighbouring warps that ended in the same pair: one record, under the first one's piece --
+  __syncthreads();
+  for (int first = 0; first < T::kWarps;) {
+    const long long pair = s_pair[first];
+    if (pair < 0) break;  // (pieces are in order: behind a warp without one there is none)
+    int end = first + 1;
+    while (end < T::kWarps && s_pair[end] == pair) ++end;
+    float* rec = p.ws + ((size_t)(blockIdx.x * busy + first) + (size_t)pair) * 8 * T::kRec;
+    for (int i = threadIdx.x; i < s_rows[first] * (H / 4); i += T::kThreads) {
+      const int row = i / (H / 4), d = i % (H / 4) * 4;
+      float top = -CUDART_INF_F, sum = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < T::kWarps; ++j)
+        if (j >= first && j < end) top = fmaxf(top, s_m[j][row]);
+      const float use = top == -CUDART_INF_F ? 0.0f : top;
+#pragma unroll
+      for (int j = 0; j < T::kWarps; ++j) {
+        if (j >= first && j < end) {
+          const float f = power2((s_m[j][row] - use) * kLog2e);
+          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + j * T::kStages * T::kBytes) + row * T::kRec + d);
+          acc.x = fmaf(f, v.x, acc.x);
+          acc.y = fmaf(f, v.y, acc.y);
+          acc.z = fmaf(f, v.z, acc.z);
+          acc.w = fmaf(f, v.w, acc.w);
+          sum = fmaf(f, s_l[j][row], sum);
+        }
+      }
+      *reinterpret_cast<float4*>(rec + row * T::kRec + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(rec + row * T::kRec + H) = make_float2(top, sum);
+    }
+    first = end;
+  }
 }
 
-// Merges the records of one query row (the first n t CTAs of a sequence), or adds the weights that 1024 slots of a KV head
-// got to the scores (the others).
+// Merges the records of one query row, H >> part_log2 channels per CTA (the first n t << part_log2 CTAs of a sequence), or
+// adds the weights that 1024 slots of a KV head got to the scores (the others). What it costs are L2 round trips, so the
+// records are requested before their weights are known.
 constexpr int kMergeThreads = 256;
 constexpr int kScoreSlots = 1024;
+
+__device__ __forceinline__ float merge_reduce(float v, bool max, float* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float y = __shfl_xor_sync(0xffffffffu, v, o);
+    v = max ? fmaxf(v, y) : v + y;
+  }
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int i = 1; i < kMergeThreads / 32; ++i) v = max ? fmaxf(v, red[i]) : v + red[i];
+  return v;
+}
+
 template <int H, bool QF32>
-__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa p, const int split_ctas, const int min_units, const float* logits_ws) {
-  constexpr int kRec = H + 4, kQuads = H / 4, kGroups = kMergeThreads / kQuads, kBatch = 16;
+__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa p, const int ctas, const int part_log2, const float* logits_ws) {
+  constexpr int kRec = H + 4, kBatch = 8;
   constexpr size_t kStride = 8 * (size_t)kRec;
-  extern __shared__ float merge_w[];  // one weight per record
+  extern __shared__ float merge_w[];  // per record a weight, then per record a sum
   __shared__ float4 s_part[kMergeThreads];
   __shared__ float s_stat[16];
   pdl_launch_dependents();
-  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Kv4Rows rw = kv4_rows(p.t, p.n, p.cache.nkv);
   const int per = p.cache.nkv * rw.chunks;
   // what does not depend on the kernel before: it has waited for whatever wrote the lengths
   int total, below;
-  kv4_count_units(p, per, b, lane, &total, &below);
-  const Pieces cut(total, split_ctas, min_units);
-  const int length = kv4_length(p, b), units = tiles_of(length);
-  auto records = [&](int in_b, int* count) {
-    *count = 0;
-    if (units == 0) return (const float*)nullptr;
-    const int u0 = below + in_b * units, c0 = cut.owner(u0), c1 = cut.owner(u0 + units - 1);
-    *count = c1 - c0 + 1;
-    return (const float*)p.ws + ((size_t)c0 + (size_t)b * per + in_b) * kStride;
+  kv4_count_tiles(p, per, b, lane, &total, &below);
+  const int busy = kv4_busy_warps(total, ctas, kv4_warps(H));
+  const Pieces cut(total, ctas * busy, 1);
+  const int length = kv4_length(p, b), tiles = tiles_of(length);
+  // Records of a pair: of every CTA that ended in it the one under the first such piece, and that of the last piece where
+  // this goes on to another pair.
+  struct Records {
+    const float* base;  // of piece 0
+    int first, cta, leaders, last, count;
+    __device__ __forceinline__ const float* at(int j, int busy) const {
+      const int piece = j >= leaders ? last : j == 0 ? first : (cta + j) * busy;
+      return base + piece * kStride;
+    }
   };
-  if ((int)blockIdx.x < p.n * p.t) {
-    const int i = blockIdx.x / p.n, head = blockIdx.x % p.n, kvh = head / rw.group, r = i * rw.group + head % rw.group;
-    const int quad = threadIdx.x % kQuads, grp = threadIdx.x / kQuads;
-    int count;
-    const float* base = records(kvh * rw.chunks + r / 8, &count) + (r % 8) * kRec;
+  auto records = [&](int in_b) {
+    Records r{p.ws + ((size_t)b * per + in_b) * kStride, 0, 0, 0, 0, 0};
+    if (tiles == 0) return r;
+    const int u0 = below + in_b * tiles, u1 = u0 + tiles;
+    r.first = cut.owner(u0);
+    r.last = cut.owner(u1 - 1);
+    r.cta = r.first / busy;
+    const bool goes_on = cut.begin(r.last + 1) > u1;  // then it has a record of its own and leads nothing
+    const int last_leader = goes_on ? r.last - 1 : r.last;
+    r.leaders = last_leader < r.first ? 0 : last_leader / busy - r.cta + 1;
+    r.count = r.leaders + (goes_on ? 1 : 0);
+    return r;
+  };
+  if ((int)blockIdx.x < (p.n * p.t) << part_log2) {
+    const int row = blockIdx.x >> part_log2, part = blockIdx.x & ((1 << part_log2) - 1);
+    const int i = row / p.n, head = row % p.n, kvh = head / rw.group, r = i * rw.group + head % rw.group;
+    const int quads = (H / 4) >> part_log2, groups = kMergeThreads / quads;
+    const int quad = tid % quads, grp = tid / quads, channel = 4 * (part * quads + quad);
+    const Records rec = records(kvh * rw.chunks + r / 8);
+    const int count = rec.count, in_rec = (r % 8) * kRec;
     pdl_wait();
     float4 first[kBatch];
-    request_quads(first, base + 4 * quad, kStride, count, grp, kGroups);
-    if (threadIdx.x < 32) {
-      const float l = record_weights(base + H, kStride, count, lane, merge_w, kLog2e);
-      if (lane == 0) s_stat[0] = l;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int c = grp + j * groups;
+      first[j] = c < count ? __ldcg(reinterpret_cast<const float4*>(rec.at(c, busy) + in_rec + channel)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    __syncthreads();
-    s_part[threadIdx.x] = merge_quad(base + 4 * quad, kStride, count, grp, kGroups, merge_w, first);
+    float* sums = merge_w + ctas + 1;
+    float top = -CUDART_INF_F, l = 0.0f;
+    for (int c = tid; c < count; c += kMergeThreads) {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(rec.at(c, busy) + in_rec + H));
+      merge_w[c] = v.x;
+      sums[c] = v.y;
+      top = fmaxf(top, v.x);
+    }
+    top = merge_reduce(top, true, s_stat);
+    top = top == -CUDART_INF_F ? 0.0f : top;
+    for (int c = tid; c < count; c += kMergeThreads) {
+      const float f = exp2f((merge_w[c] - top) * kLog2e);
+      merge_w[c] = f;
+      l += f * sums[c];
+    }
+    l = merge_reduce(l, false, s_stat + 8);  // (its barrier also publishes the weights)
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c0 = grp; c0 < count; c0 += kBatch * groups) {
+      if (c0 > grp) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (c0 + j * groups < count) first[j] = __ldcg(reinterpret_cast<const float4*>(rec.at(c0 + j * groups, busy) + in_rec + channel));
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (c0 + j * groups < count) {
+          const float f = merge_w[c0 + j * groups];
+          acc.x = fmaf(f, first[j].x, acc.x);
+          acc.y = fmaf(f, first[j].y, acc.y);
+          acc.z = fmaf(f, first[j].z, acc.z);
+          acc.w = fmaf(f, first[j].w, acc.w);
+        }
+      }
+    }
+    s_part[tid] = acc;
     __syncthreads();
     if (grp > 0) return;
-    float4 acc = s_part[quad];
-#pragma unroll 2
-    for (int j = 1; j < kGroups; ++j) {
-      const float4 v = s_part[j * kQuads + quad];
+#pragma unroll 4
+    for (int j = 1; j < groups; ++j) {
+      const float4 v = s_part[j * quads + quad];
       acc.x += v.x;
       acc.y += v.y;
       acc.z += v.z;
       acc.w += v.w;
     }
-    const float l = s_stat[0];
     if (l == 0.0f) {
       acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // no slot
     } else {
       acc = make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
     }
-    const size_t at = (((size_t)b * p.t + i) * p.n + head) * H + 4 * quad;
+    const size_t at = (((size_t)b * p.t + i) * p.n + head) * H + channel;
     if constexpr (QF32) {
       float* o = static_cast<float*>(p.out) + at;
       o[0] = acc.x, o[1] = acc.y, o[2] = acc.z, o[3] = acc.w;
@@ -862,7 +955,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
     return;
   }
   const int ranges = (p.cache.s + kScoreSlots - 1) / kScoreSlots;
-  const int at = blockIdx.x - p.n * p.t, kvh = at / ranges, slot0 = at % ranges * kScoreSlots;
+  const int at = blockIdx.x - ((p.n * p.t) << part_log2), kvh = at / ranges, slot0 = at % ranges * kScoreSlots;
   pdl_wait();
   if (slot0 >= length) return;
   const size_t pitch = (size_t)tiles_of(p.cache.s) * kSlots * 8;
@@ -871,17 +964,17 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
   for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) sums[j] = 0.0f;
   for (int c = 0; c < rw.chunks; ++c) {
     const int in_b = kvh * rw.chunks + c, rows = min(8, rw.rows - 8 * c);
-    int count;
-    const float* ml = records(in_b, &count) + H;
+    const Records rec = records(in_b);
+    const int in_rec = warp * kRec + H;
     __syncthreads();
     if (warp < rows) {
       float top = -CUDART_INF_F, l = 0.0f;
-      for (int j = lane; j < count; j += 32) top = fmaxf(top, __ldcg(ml + warp * kRec + j * kStride));
+      for (int j = lane; j < rec.count; j += 32) top = fmaxf(top, __ldcg(rec.at(j, busy) + in_rec));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       top = top == -CUDART_INF_F ? 0.0f : top;
-      for (int j = lane; j < count; j += 32) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(ml + warp * kRec + j * kStride));
+      for (int j = lane; j < rec.count; j += 32) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(rec.at(j, busy) + in_rec));
         l += exp2f((v.x - top) * kLog2e) * v.y;
       }
 #pragma unroll
@@ -916,27 +1009,25 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
   }
 }
 
-// Shortest piece worth a CTA of its own: a tile for every warp.
-constexpr int kv4_min_units(int h) { return h == 256 ? 8 : h == 128 ? 12 : 16; }
-// CTAs of a launch: one per SM, fewer when even full caches give no piece for some.
-int kv4_ctas(long long pairs, int s, int h) {
-  const long long most = pairs * tiles_of(s), n = (most + kv4_min_units(h) - 1) / kv4_min_units(h);
+// CTAs of a launch: one per SM, fewer when even full caches leave some without a tile.
+int kv4_ctas(long long pairs, int s) {
+  const long long most = pairs * tiles_of(s);
   const int sms = device_sm_count();
-  return n < sms ? (int)n : sms;
+  return most < sms ? (int)most : sms;
 }
 
 bool kv4_tensor_shape(int b, int t, int n, int nkv, int h, int s) {
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
   return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX &&
-         (long long)n * t + (long long)nkv * ((s + kScoreSlots - 1) / kScoreSlots) <= INT32_MAX;
+         4ll * n * t + (long long)nkv * ((s + kScoreSlots - 1) / kScoreSlots) <= INT32_MAX;
 }
 
 template <int H, int BLOCK, bool QF32>
 cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
   using T = Kv4Tile<H, BLOCK>;
   const long long pairs = (long long)p.cache.b * p.cache.nkv * kv4_rows(p.t, p.n, p.cache.nkv).chunks;
-  const int ctas = kv4_ctas(pairs, p.cache.s, H), min_units = kv4_min_units(H);
-  float* logits = p.scores ? p.ws + kv4_records_floats(ctas, pairs, H) : nullptr;
+  const int ctas = kv4_ctas(pairs, p.cache.s), pieces = ctas * T::kWarps;
+  float* logits = p.scores ? p.ws + kv4_records_floats(pieces, pairs, H) : nullptr;
   static bool done[64] = {false};
   int device = 0;
   cudaGetDevice(&device);
@@ -946,11 +1037,14 @@ cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     done[device] = true;
   }
-  const cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, min_units, logits);
+  const cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, logits);
   if (e != cudaSuccess) return e;
   const int scores = p.scores ? p.cache.nkv * ((p.cache.s + kScoreSlots - 1) / kScoreSlots) : 0;
-  return launch_chained(kv4_merge_kernel<H, QF32>, dim3(p.n * p.t + scores, p.cache.b), dim3(kMergeThreads), sizeof(float) * (size_t)ctas, s, p,
-                        ctas, min_units, (const float*)logits);
+  // few rows are cut by channels too: their records are many
+  int part_log2 = 0;
+  while (part_log2 < 2 && ((long long)p.cache.b * p.n * p.t << part_log2) < device_sm_count()) ++part_log2;
+  return launch_chained(kv4_merge_kernel<H, QF32>, dim3(((p.n * p.t) << part_log2) + scores, p.cache.b), dim3(kMergeThreads),
+                        2 * sizeof(float) * (size_t)(ctas + 1), s, p, ctas, part_log2, (const float*)logits);
 }
 template <int H, int BLOCK>
 cudaError_t launch_tensor_q(const Kv4Sdpa& p, cudaStream_t s) {
@@ -968,7 +1062,7 @@ size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int 
   const size_t any = 2 * rows + rows * s;  // (also what queries off a 16-byte boundary need)
   if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return any * sizeof(float);
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
-  const size_t tensor = kv4_records_floats(kv4_ctas(pairs, s, h), pairs, h) +
+  const size_t tensor = kv4_records_floats(kv4_ctas(pairs, s) * kv4_warps(h), pairs, h) +
                         (scores ? (size_t)pairs * tiles_of(s) * kSlots * 8 : 0);
   return (any > tensor ? any : tensor) * sizeof(float);
 }
