@@ -11,7 +11,6 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.h"
-#include "pieces.cuh"
 
 namespace b200 {
 
@@ -149,13 +148,13 @@ cudaError_t launch_rows(const Kv4Sdpa& p, cudaStream_t s) {
 
 // ---- head sizes 64, 128 and 256: tensor cores -------------------------------------------------------------
 // Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; a tile is 32 slots,
-// two 16-row sides of it whose chains of products and exponentials run side by side. The tiles of all (sequence, KV head,
-// eight rows) pairs form one row, cut into equal pieces, one per warp, whatever the lengths are (pieces.cuh). A warp walks
-// through its piece without meeting another one. At its end the warps of a CTA add their states of a common pair to one
-// partial record (un-normalised outputs, maximum, sum); a warp that goes on to another pair writes a record of the first on
-// its own. A second kernel merges a pair's records.
-// 16 ragged sequences of up to 8192 tokens, 8 heads x 256, replayed: 20.3 us with a record per warp (the second kernel reads
-// 9.8 MB then), 19.4 with a piece per CTA (6 of them in the CTAs that had parts of two sequences one after the other).
+// two 16-row sides of it whose chains of products and exponentials run side by side. Every (sequence, KV head, eight rows)
+// pair is cut into pieces of a common greatest length, one per warp. A warp walks through its piece without meeting another
+// one; at the end the warps of a CTA add their states of a common pair to one partial record (un-normalised outputs, maximum,
+// sum), and a second kernel merges a pair's records.
+// Measured with 16 ragged sequences of up to 8192 tokens, 8 heads x 256, replayed: pieces that run on from one pair to the
+// next (all of one length) 17.5 us, 4 of them in the warps that had parts of two pairs; such pieces per CTA 19.4; a record
+// for every warp 20.3 (the second kernel reads 9.8 MB then).
 constexpr int kSlots = 32;
 __host__ __device__ inline int tiles_of(int slots) { return (slots + kSlots - 1) / kSlots; }
 
@@ -186,23 +185,64 @@ __host__ __device__ inline Kv4Rows kv4_rows(int t, int n, int nkv) {
   return {group, rows, (rows + 7) / 8};
 }
 
-// Workspace of the piecewise kernels: records (a piece and a pair name one), then the logits [pair][slot (rounded up to a tile)][8 rows] where scores
-// are wanted.
-__host__ __device__ inline size_t kv4_records_floats(int pieces, long long pairs, int h) { return ((size_t)pieces + (size_t)pairs) * 8 * (h + 4); }
+// Workspace of the tensor-core kernels: a record per piece (of which the first of a pair in each CTA is written), then the
+// logits [pair][slot (rounded up to a tile)][8 rows] where scores are wanted.
+__host__ __device__ inline size_t kv4_records_floats(long long pieces, int h) { return (size_t)pieces * 8 * (h + 4); }
 
 __device__ __forceinline__ int kv4_length(const Kv4Sdpa& p, int b) {
   return p.lengths ? max(0, min(p.lengths[b], p.cache.s)) : p.cache.s;
 }
-// Tiles of all sequences' pairs, and of the sequences below `b`. Whole warp.
-__device__ __forceinline__ void kv4_count_tiles(const Kv4Sdpa& p, int per, int b, int lane, int* total, int* below) {
-  int all = 0, low = 0;
-  for (int i = lane; i < p.cache.b; i += 32) {
-    const int u = tiles_of(kv4_length(p, i)) * per;
-    all += u;
-    if (i < b) low += u;
+
+// a / b for a below 2^22, given 1 / b. (The divisions stand in chains of dependent instructions at the kernels' start.)
+__device__ __forceinline__ int divide(int a, int b, float inverse) {
+  int q = (int)((float)a * inverse);
+  const int r = a - q * b;
+  q += (r >= b ? 1 : 0) - (r < 0 ? 1 : 0);
+  return q;
+}
+
+// How the pairs are cut: into pieces of up to about `size` tiles, each pair's of equal lengths (to a tile), the smallest size
+// that needs no more pieces than there are warps. Every CTA gets an equal number of the pieces (to one). What is rounded
+// here is so in both kernels.
+struct Kv4Cut {
+  int size, each, longer;  // the first `longer` CTAs have one piece more than `each`
+  float inverse;           // 1 / size
+  int len;                 // attended slots of sequence `lane`
+  __device__ __forceinline__ int pieces_of(int slots) const {
+    const int tiles = tiles_of(slots);
+    return tiles == 0 ? 0 : max(1, min(tiles, (int)((float)(tiles + size - 1) * inverse)));
   }
-  *total = (int)__reduce_add_sync(0xffffffffu, (unsigned)all);
-  *below = (int)__reduce_add_sync(0xffffffffu, (unsigned)low);
+  __device__ __forceinline__ int begin(int cta) const { return cta * each + min(cta, longer); }
+  __device__ __forceinline__ int owner(int piece) const {
+    const int front = longer * (each + 1);
+    return piece < front ? divide(piece, each + 1, __frcp_rn((float)(each + 1))) : longer + divide(piece - front, each, __frcp_rn((float)each));
+  }
+};
+// Pieces of the sequences below `upto`, all pairs. Whole warp.
+__device__ __forceinline__ int count_pieces(const Kv4Sdpa& p, int per, const Kv4Cut& c, int lane, int upto) {
+  int n = lane < upto ? c.pieces_of(c.len) * per : 0;
+  for (int i = lane + 32; i < upto; i += 32) n += c.pieces_of(kv4_length(p, i)) * per;
+  return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+}
+__device__ __forceinline__ Kv4Cut kv4_cut(const Kv4Sdpa& p, int per, int ctas, int warps, int lane) {
+  const int room = ctas * warps;
+  const float inverse_room = __frcp_rn((float)room), inverse_ctas = __frcp_rn((float)ctas);
+  Kv4Cut c;
+  c.len = lane < p.cache.b ? kv4_length(p, lane) : 0;
+  int total = tiles_of(c.len) * per;
+  for (int i = lane + 32; i < p.cache.b; i += 32) total += tiles_of(kv4_length(p, i)) * per;
+  total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+  c.size = max(1, (int)ceilf((float)total * inverse_room));
+  int n;
+  while (true) {  // (ends: there is room for twice the pairs, and a large enough size makes a piece of each)
+    c.inverse = __frcp_rn((float)c.size);
+    n = count_pieces(p, per, c, lane, p.cache.b);
+    if (n <= room) break;
+    c.size += 1 + c.size / 16;
+  }
+  c.each = divide(n, ctas, inverse_ctas);
+  c.longer = n - c.each * ctas;
+  return c;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -242,6 +282,17 @@ __device__ __forceinline__ void product(float (&d)[4], uint32_t a0, uint32_t a1,
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void first_product(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// p + j * step in one instruction.
+__device__ __forceinline__ const void* advance(const void* p, int j, uint32_t step) {
+  uint64_t r;
+  asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(j), "r"(step), "l"(p));
+  return reinterpret_cast<const void*>(r);
 }
 // 2^x; results below 2^-126 are zero.
 __device__ __forceinline__ float power2(float x) {
@@ -303,9 +354,6 @@ __device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t centred_low(uint32_t w) { return half2_sub((w & kLowNibbles) | 0x64006400u, 0x64086408u); }    // - 1032
 __device__ __forceinline__ uint32_t centred_high(uint32_t w) { return half2_sub((w & kHighNibbles) | 0x54005400u, 0x54805480u); }  // - 72
 
-// How many warps of a CTA get a piece: few tiles are spread over the CTAs first.
-__device__ __forceinline__ int kv4_busy_warps(int total, int ctas, int warps) { return max(1, min(warps, (total + ctas - 1) / ctas)); }
-
 template <int H, int BLOCK, bool QF32>
 __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, float* logits_ws) {
   using T = Kv4Tile<H, BLOCK>;
@@ -314,48 +362,50 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
   constexpr int kPer = BLOCK / 32;    // of them in a block
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
-  __shared__ float s_m[T::kWarps][8], s_l[T::kWarps][8];  // maxima and sums of the warps' last pairs
-  __shared__ long long s_pair[T::kWarps];                 // and which these are
+  __shared__ float s_m[T::kWarps][8], s_l[T::kWarps][8];  // maxima and sums of the warps' states
+  __shared__ int s_pair[T::kWarps];                       // and whose these are
   __shared__ int s_rows[T::kWarps];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int nkv = p.cache.nkv, s_max = p.cache.s;
   const Kv4Rows rw = kv4_rows(p.t, p.n, nkv);
   const int per = nkv * rw.chunks;  // pairs per sequence
+  // this warp's ring; where a lane's copies come from and go to (16-byte piece `lane % P` of rows lane / P + 32 / P j)
+  const uint32_t ring = smem_u32(smem) + (uint32_t)(w * T::kStages * T::kBytes);
+  const uint32_t row_pitch = (uint32_t)nkv * (H / 2), pair_pitch = (uint32_t)nkv * G * 4;  // bytes
+  const int copy_row = lane / P, copy_piece = lane % P;
+  const uint32_t copy_from = (uint32_t)copy_row * row_pitch + copy_piece * 16, pair_from = (uint32_t)(lane / G) * pair_pitch + lane % G * 4;
+  const uint32_t row_step = row_pitch * (32 / P), pair_step = pair_pitch * (32 / G);
+  // the row that this lane names for a load of matrices: of two pieces, rows 0 .. 15
+  const uint32_t matrix_at = piece_at<H>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
+  const float inverse_chunks = __frcp_rn((float)rw.chunks), inverse_group = __frcp_rn((float)rw.group);
   pdl_wait();
   // (only now: what a dependent kernel does ahead of its own wait may then read this kernel's inputs)
   pdl_launch_dependents();
-  // this warp's piece, and the pair in which it starts
-  int len = lane < p.cache.b ? kv4_length(p, lane) : 0;
-  int total = tiles_of(len) * per, below;
-  if (p.cache.b <= 32) {
-    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
-  } else {
-    kv4_count_tiles(p, per, 0, lane, &total, &below);
-  }
-  const int busy = kv4_busy_warps(total, gridDim.x, T::kWarps);
-  const Pieces cut(total, gridDim.x * busy, 1);
-  const int piece = blockIdx.x * busy + w;
-  int left = 0, b = 0, in_b = 0, unit = 0;
-  if (w < busy && piece < cut.ctas && total > 0) {
-    const int u0 = cut.begin(piece);
-    left = cut.begin(piece + 1) - u0;
-    for (int b0 = 0, base = 0;; b0 += 32) {
+  // this warp's piece
+  const Kv4Cut cut = kv4_cut(p, per, gridDim.x, T::kWarps, lane);
+  const int first_piece = cut.begin(blockIdx.x), piece = first_piece + w;
+  int seg = 0, b = 0, in_b = 0, unit = 0, len = cut.len;  // seg tiles from `unit` on of pair in_b of sequence b
+  if (w < cut.each + ((int)blockIdx.x < cut.longer ? 1 : 0)) {
+    for (int b0 = 0, base = 0; b0 < p.cache.b; b0 += 32) {
       if (b0 > 0) len = b0 + lane < p.cache.b ? kv4_length(p, b0 + lane) : 0;
-      const int mine = tiles_of(len) * per;
-      int upto = mine;  // inclusive prefix sum over the lanes
+      int n = cut.pieces_of(len), upto = n * per;  // inclusive prefix sum over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
       }
-      const uint32_t here = __ballot_sync(0xffffffffu, base + upto > u0);
-      if (here) {  // (there is one: u0 < total)
+      const uint32_t here = __ballot_sync(0xffffffffu, base + upto > piece);
+      if (here) {
         const int src = __ffs(here) - 1;
-        const int from = __shfl_sync(0xffffffffu, base + upto - mine, src);
+        const int rest = piece - __shfl_sync(0xffffffffu, base + upto - n * per, src);
         len = __shfl_sync(0xffffffffu, len, src);
+        n = __shfl_sync(0xffffffffu, n, src);
         b = b0 + src;
-        in_b = (u0 - from) / tiles_of(len);
-        unit = (u0 - from) % tiles_of(len);
+        const float inverse = __frcp_rn((float)n);
+        in_b = divide(rest, n, inverse);
+        const int part = rest - in_b * n, tiles = tiles_of(len), each = divide(tiles, n, inverse), longer = tiles - each * n;
+        unit = part * each + min(part, longer);
+        seg = each + (part < longer ? 1 : 0);
         break;
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
@@ -363,64 +413,73 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
   }
   if (lane == 0) s_pair[w] = -1;  // no state yet
 
-  // this warp's ring; where a lane's copies come from and go to (16-byte piece `lane % P` of rows lane / P + 32 / P j)
-  const uint32_t ring = smem_u32(smem) + (uint32_t)(w * T::kStages * T::kBytes);
-  const size_t row_pitch = (size_t)nkv * (H / 2), pair_pitch = (size_t)nkv * G;  // bytes; pairs
-  const int copy_row = lane / P, copy_piece = lane % P;
-  const size_t copy_from = copy_row * row_pitch + copy_piece * 16;
-  const size_t pair_from = (lane / G) * pair_pitch + lane % G;
-  // the row that this lane names for a load of matrices: of two pieces, rows 0 .. 15
-  const uint32_t matrix_at = piece_at<H>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
-
-  while (left > 0) {
-    const int seg = min(left, tiles_of(len) - unit);
-    const int kvh = in_b / rw.chunks, chunk = in_b % rw.chunks;
-    const size_t pair = (size_t)b * per + in_b;
-    const size_t slot0 = (size_t)b * s_max;
-    const uint8_t* k_base = p.cache.k + (slot0 * nkv + kvh) * (H / 2);
-    const uint8_t* v_base = p.cache.v + (slot0 * nkv + kvh) * (H / 2);
-    const __half2* kp_base = p.cache.k_pairs + (slot0 * nkv + kvh) * G;
-    const __half2* vp_base = p.cache.v_pairs + (slot0 * nkv + kvh) * G;
+  if (seg > 0) {
+    const int kvh = divide(in_b, rw.chunks, inverse_chunks), chunk = in_b - kvh * rw.chunks;
+    const int pair = b * per + in_b;
+    // the queries are asked for first, the tiles arrive meanwhile
+    const int q_row = chunk * 8 + g;
+    uint4 q_bits[QF32 ? 2 * P : P];
+    {
+      const int i = divide(q_row, rw.group, inverse_group);
+      const size_t at = (((size_t)b * p.t + i) * p.n + kvh * rw.group + (q_row - i * rw.group)) * H + 8 * t;
+#pragma unroll
+      for (int sl = 0; sl < P; ++sl) {
+        if constexpr (QF32) {
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.q) + at + 32 * sl);
+          q_bits[2 * sl] = q_row < rw.rows ? __ldg(src) : make_uint4(0, 0, 0, 0);
+          q_bits[2 * sl + 1] = q_row < rw.rows ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+        } else {
+          q_bits[sl] = q_row < rw.rows ? __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + at + 32 * sl)) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
     // Requests this warp's next tile: rows behind the length arrive as zeros.
+    const size_t row0 = ((size_t)b * s_max + (size_t)unit * kSlots) * nkv + kvh;
+    const uint8_t* k_next = p.cache.k + row0 * (H / 2);
+    const uint8_t* v_next = p.cache.v + row0 * (H / 2);
+    const __half2* kp_next = p.cache.k_pairs + row0 * G;
+    const __half2* vp_next = p.cache.v_pairs + row0 * G;
     int asked = 0;
     uint32_t to = ring;
-    const uint8_t* k_next = k_base + (size_t)unit * kSlots * row_pitch + copy_from;
-    const uint8_t* v_next = v_base + (size_t)unit * kSlots * row_pitch + copy_from;
-    const __half2* kp_next = kp_base + (size_t)unit * kSlots * pair_pitch + pair_from;
-    const __half2* vp_next = vp_base + (size_t)unit * kSlots * pair_pitch + pair_from;
     auto request = [&]() {
       if (asked < seg) {
         const int there = len - (unit + asked) * kSlots;
         if (there >= kSlots) {
+          const void* ks = k_next + copy_from;
+          const void* vs = v_next + copy_from;
+          const void* kps = reinterpret_cast<const uint8_t*>(kp_next) + pair_from;
+          const void* vps = reinterpret_cast<const uint8_t*>(vp_next) + pair_from;
 #pragma unroll
           for (int j = 0; j < P; ++j) {
-            cp_async16(to + piece_at<H>(copy_row + j * (32 / P), copy_piece), k_next + j * (32 / P) * row_pitch);
-            cp_async16(to + T::kNibbleBytes + piece_at<H>(copy_row + j * (32 / P), copy_piece), v_next + j * (32 / P) * row_pitch);
+            cp_async16(to + piece_at<H>(copy_row + j * (32 / P), copy_piece), advance(ks, j, row_step));
+            cp_async16(to + T::kNibbleBytes + piece_at<H>(copy_row + j * (32 / P), copy_piece), advance(vs, j, row_step));
           }
 #pragma unroll
           for (int j = 0; j < G; ++j) {
-            cp_async4(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, kp_next + j * (32 / G) * pair_pitch);
-            cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, vp_next + j * (32 / G) * pair_pitch);
+            cp_async4(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, advance(kps, j, pair_step));
+            cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, advance(vps, j, pair_step));
           }
-        } else {
-#pragma unroll
+        } else {  // (one tile of a pair at most)
+#pragma unroll 1
           for (int j = 0; j < P; ++j) {
             const int row = copy_row + j * (32 / P);
             const bool ok = row < there;
-            cp_async16_or_zero(to + piece_at<H>(row, copy_piece), ok ? k_next + j * (32 / P) * row_pitch : k_base, ok);
-            cp_async16_or_zero(to + T::kNibbleBytes + piece_at<H>(row, copy_piece), ok ? v_next + j * (32 / P) * row_pitch : v_base, ok);
+            const uint32_t from = ok ? copy_from + j * row_step : 0u;
+            cp_async16_or_zero(to + piece_at<H>(row, copy_piece), k_next + from, ok);
+            cp_async16_or_zero(to + T::kNibbleBytes + piece_at<H>(row, copy_piece), v_next + from, ok);
           }
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < G; ++j) {
             const bool ok = (lane + 32 * j) / G < there;
-            cp_async4_or_zero(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, ok ? kp_next + j * (32 / G) * pair_pitch : kp_base, ok);
-            cp_async4_or_zero(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, ok ? vp_next + j * (32 / G) * pair_pitch : vp_base, ok);
+            const uint32_t from = ok ? pair_from + j * pair_step : 0u;
+            cp_async4_or_zero(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, reinterpret_cast<const uint8_t*>(kp_next) + from, ok);
+            cp_async4_or_zero(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, reinterpret_cast<const uint8_t*>(vp_next) + from, ok);
           }
         }
-        k_next += kSlots * row_pitch;
-        v_next += kSlots * row_pitch;
-        kp_next += kSlots * pair_pitch;
-        vp_next += kSlots * pair_pitch;
+        k_next += (size_t)kSlots * row_pitch;
+        v_next += (size_t)kSlots * row_pitch;
+        kp_next += (size_t)kSlots * nkv * G;
+        vp_next += (size_t)kSlots * nkv * G;
         to = to + T::kBytes == ring + T::kStages * T::kBytes ? ring : to + T::kBytes;
         ++asked;
       }
@@ -436,23 +495,15 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     float q_sum[G][2], factor[2];  // of the rows 2 t and 2 t + 1 (the products' columns)
     int limit[2];
     {
-      const int r = chunk * 8 + g;
-      const int i = r / rw.group;
-      const size_t at = (((size_t)b * p.t + i) * p.n + kvh * rw.group + r % rw.group) * H;
       float raw[P][8], top = 0.0f;
 #pragma unroll
       for (int sl = 0; sl < P; ++sl) {
-        const int word = 4 * sl + t;
-        if (r >= rw.rows) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) raw[sl][e] = 0.0f;
-        } else if constexpr (QF32) {
-          const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at + 8 * word);
-          const float4 lo = __ldg(src), hi = __ldg(src + 1);
-          raw[sl][0] = lo.x, raw[sl][1] = lo.y, raw[sl][2] = lo.z, raw[sl][3] = lo.w;
-          raw[sl][4] = hi.x, raw[sl][5] = hi.y, raw[sl][6] = hi.z, raw[sl][7] = hi.w;
+        if constexpr (QF32) {
+          const uint4 lo = q_bits[2 * sl], hi = q_bits[2 * sl + 1];
+          raw[sl][0] = __uint_as_float(lo.x), raw[sl][1] = __uint_as_float(lo.y), raw[sl][2] = __uint_as_float(lo.z), raw[sl][3] = __uint_as_float(lo.w);
+          raw[sl][4] = __uint_as_float(hi.x), raw[sl][5] = __uint_as_float(hi.y), raw[sl][6] = __uint_as_float(hi.z), raw[sl][7] = __uint_as_float(hi.w);
         } else {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + at + 8 * word));
+          const uint4 v = q_bits[sl];
           const float2 f0 = pair_floats(v.x), f1 = pair_floats(v.y), f2 = pair_floats(v.z), f3 = pair_floats(v.w);
           raw[sl][0] = f0.x, raw[sl][1] = f0.y, raw[sl][2] = f1.x, raw[sl][3] = f1.y;
           raw[sl][4] = f2.x, raw[sl][5] = f2.y, raw[sl][6] = f3.x, raw[sl][7] = f3.y;
@@ -503,11 +554,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     const float* mask[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = chunk * 8 + 2 * t + e, i = r / rw.group;
+      const int r = chunk * 8 + 2 * t + e, i = divide(r, rw.group, inverse_group);
       limit[e] = r < rw.rows ? kv4_limit(len, s_max, p.t, i) : len;  // (columns without a row are computed and dropped)
       mask[e] = p.mask && r < rw.rows ? p.mask + ((size_t)b * p.t + i) * s_max : nullptr;
     }
-    const int least_limit = kv4_limit(len, s_max, p.t, chunk * 8 / rw.group);  // of any row
+    const int least_limit = kv4_limit(len, s_max, p.t, divide(chunk * 8, rw.group, inverse_group));  // of any row
     // masks are requested a tile ahead of their use
     auto masks = [&](int k, float (&m)[2][4]) {
       const int first = (unit + k) * kSlots;
@@ -522,7 +573,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     float next_mask[2][4];
     masks(0, next_mask);
     const bool guard = p.mask != nullptr || p.t > 1;  // slots that some row does not see may hold anything
-    float* logits = logits_ws ? logits_ws + pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
+    float* logits = logits_ws ? logits_ws + (size_t)pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
 
     // outputs: of piece i and its channels 4 g + {0, 1} and 4 g + {2, 3}, rows 2 t and 2 t + 1
     float o[P][2][4], least_sum[G];
@@ -559,10 +610,6 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
             load_matrices(at + (matrix_at ^ (uint32_t)((i0 + i) * 16)) + side * 8 * H, words[side][i / 2]);
         float acc[2][kChains][4];
 #pragma unroll
-        for (int side = 0; side < 2; ++side)
-#pragma unroll
-          for (int c = 0; c < kChains; ++c) acc[side][c][0] = acc[side][c][1] = acc[side][c][2] = acc[side][c][3] = 0.0f;
-#pragma unroll
         for (int j = 0; j < kPer; ++j) {
 #pragma unroll
           for (int odd = 0; odd < 2; ++odd)
@@ -574,7 +621,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
                 const uint32_t wa = words[side][i / 2][2 * (i & 1)], wb = words[side][i / 2][2 * (i & 1) + 1];
                 const uint32_t keep = odd ? kHighNibbles : kLowNibbles;
                 const uint32_t a0 = wa & keep, a1 = wb & keep, a2 = (wa >> 8) & keep, a3 = (wb >> 8) & keep;
-                product(acc[side][c], a0, a1, a2, a3, q_high[i0 + i][2 * odd], q_high[i0 + i][2 * odd + 1]);
+                if (j == 0 && odd == 0) {
+                  first_product(acc[side][c], a0, a1, a2, a3, q_high[i0 + i][0], q_high[i0 + i][1]);
+                } else {
+                  product(acc[side][c], a0, a1, a2, a3, q_high[i0 + i][2 * odd], q_high[i0 + i][2 * odd + 1]);
+                }
                 if constexpr (QF32) product(acc[side][c], a0, a1, a2, a3, q_low[i0 + i][2 * odd], q_low[i0 + i][2 * odd + 1]);
               }
         }
@@ -649,7 +700,6 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
           alpha[e] = m_run[e] == -CUDART_INF_F ? 0.0f : power2((m_run[e] - use) * kLog2e);
           m_run[e] = top;
           m_use[e] = use;
-          l_run[e] *= alpha[e];
         }
         const float shrink = __int_as_float((int)(127 + exponent - now) << 23);
         exponent = now;
@@ -658,6 +708,8 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
         const float mine_alpha = ((g & 1) ? odd : even) * shrink;
         alpha[0] *= shrink;
         alpha[1] *= shrink;
+        l_run[0] *= alpha[0];
+        l_run[1] *= alpha[1];
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) least_sum[gr] *= mine_alpha;
 #pragma unroll
@@ -667,20 +719,20 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       }
       // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (+ 16), in units of the value scales
       float pw[2][4];
-      const float to_units = __int_as_float((int)(150 - exponent) << 23);
+      const float to_units = 23.0f - (float)exponent;
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
         float pr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = power2((x[side][e] - m_use[e & 1]) * kLog2e);
+        for (int e = 0; e < 4; ++e) pr[e] = power2(fmaf(x[side][e] - m_use[e & 1], kLog2e, to_units));
         l_run[0] += pr[0] + pr[2];
         l_run[1] += pr[1] + pr[3];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t c0 = __float_as_uint(pr[2 * e]), c1 = __float_as_uint(pr[2 * e + 1]);
           const uint32_t lo = transposed8x8(__byte_perm(c0, c1, 0x5410)), hi = transposed8x8(__byte_perm(c0, c1, 0x7632));
-          pw[side][2 * e] = __uint_as_float(__byte_perm(lo, hi, 0x5410)) * to_units;
-          pw[side][2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632)) * to_units;
+          pw[side][2 * e] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+          pw[side][2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
         }
       }
       // -- outputs: channels by slots times slots by rows; a weight is two fp16 numbers --
@@ -734,11 +786,9 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     cp_async_wait<0>();
 
     // -- this pair's state: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
-    left -= seg;
     const float from_units = __int_as_float((int)(104 + exponent) << 23);  // 2^(exponent - 23)
     const int rows = min(8, rw.rows - chunk * 8);
-    // the last one to the warp's own part of the shared memory, another one straight to its record
-    float* rec = left > 0 ? p.ws + ((size_t)piece + pair) * 8 * T::kRec : reinterpret_cast<float*>(smem + w * T::kStages * T::kBytes);
+    float* state = reinterpret_cast<float*>(smem + w * T::kStages * T::kBytes);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -755,43 +805,28 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           if (2 * t + e < rows)
-            *reinterpret_cast<float4*>(rec + (2 * t + e) * T::kRec + i * 32 + g * 4) =
+            *reinterpret_cast<float4*>(state + (2 * t + e) * T::kRec + i * 32 + g * 4) =
                 make_float4((o[i][0][e] + least[e]) * from_units, (o[i][0][2 + e] + least[e]) * from_units, (o[i][1][e] + least[e]) * from_units,
                             (o[i][1][2 + e] + least[e]) * from_units);
     }
-    if (g < 2 && 2 * t + g < rows) {
-      const float m = g ? m_run[1] : m_run[0], l = g ? l_run[1] : l_run[0];
-      if (left > 0) {
-        *reinterpret_cast<float2*>(rec + (2 * t + g) * T::kRec + H) = make_float2(m, l);
-      } else {
-        s_m[w][2 * t + g] = m;
-        s_l[w][2 * t + g] = l;
-      }
+    if (g < 2) {
+      s_m[w][2 * t + g] = g ? m_run[1] : m_run[0];
+      s_l[w][2 * t + g] = (g ? l_run[1] : l_run[0]) * from_units;
     }
-    if (lane == 0 && left == 0) {
-      s_pair[w] = (long long)pair;
+    if (lane == 0) {
+      s_pair[w] = pair;
       s_rows[w] = rows;
-    }
-    if (left > 0) {
-      unit = 0;
-      if (++in_b == per) {
-        in_b = 0;
-        do {
-          ++b;
-          len = kv4_length(p, b);
-        } while (len == 0);
-      }
     }
   }
 
-  // -- neighbouring warps that ended in the same pair: one record, under the first one's piece --
+  // -- neighbouring warps of one pair: one record, under the first one's piece --
   __syncthreads();
   for (int first = 0; first < T::kWarps;) {
-    const long long pair = s_pair[first];
+    const int pair = s_pair[first];
     if (pair < 0) break;  // (pieces are in order: behind a warp without one there is none)
     int end = first + 1;
     while (end < T::kWarps && s_pair[end] == pair) ++end;
-    float* rec = p.ws + ((size_t)(blockIdx.x * busy + first) + (size_t)pair) * 8 * T::kRec;
+    float* rec = p.ws + (size_t)(first_piece + first) * 8 * T::kRec;
     for (int i = threadIdx.x; i < s_rows[first] * (H / 4); i += T::kThreads) {
       const int row = i / (H / 4), d = i % (H / 4) * 4;
       float top = -CUDART_INF_F, sum = 0.0f;
@@ -852,34 +887,20 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
   const Kv4Rows rw = kv4_rows(p.t, p.n, p.cache.nkv);
   const int per = p.cache.nkv * rw.chunks;
   // what does not depend on the kernel before: it has waited for whatever wrote the lengths
-  int total, below;
-  kv4_count_tiles(p, per, b, lane, &total, &below);
-  const int busy = kv4_busy_warps(total, ctas, kv4_warps(H));
-  const Pieces cut(total, ctas * busy, 1);
-  const int length = kv4_length(p, b), tiles = tiles_of(length);
-  // Records of a pair: of every CTA that ended in it the one under the first such piece, and that of the last piece where
-  // this goes on to another pair.
+  const Kv4Cut cut = kv4_cut(p, per, ctas, kv4_warps(H), lane);
+  const int length = kv4_length(p, b), pieces = cut.pieces_of(length), below = count_pieces(p, per, cut, lane, b);
+  // Records of a pair: under its first piece, and under the first piece of every further CTA.
   struct Records {
     const float* base;  // of piece 0
-    int first, cta, leaders, last, count;
-    __device__ __forceinline__ const float* at(int j, int busy) const {
-      const int piece = j >= leaders ? last : j == 0 ? first : (cta + j) * busy;
-      return base + piece * kStride;
-    }
+    int first, cta, count;
   };
   auto records = [&](int in_b) {
-    Records r{p.ws + ((size_t)b * per + in_b) * kStride, 0, 0, 0, 0, 0};
-    if (tiles == 0) return r;
-    const int u0 = below + in_b * tiles, u1 = u0 + tiles;
-    r.first = cut.owner(u0);
-    r.last = cut.owner(u1 - 1);
-    r.cta = r.first / busy;
-    const bool goes_on = cut.begin(r.last + 1) > u1;  // then it has a record of its own and leads nothing
-    const int last_leader = goes_on ? r.last - 1 : r.last;
-    r.leaders = last_leader < r.first ? 0 : last_leader / busy - r.cta + 1;
-    r.count = r.leaders + (goes_on ? 1 : 0);
-    return r;
+    const int first = below + in_b * pieces;
+    if (pieces == 0) return Records{p.ws, 0, 0, 0};
+    const int cta = cut.owner(first);
+    return Records{p.ws, first, cta, cut.owner(first + pieces - 1) - cta + 1};
   };
+  auto record_at = [&](const Records& r, int j) { return r.base + (j == 0 ? r.first : cut.begin(r.cta + j)) * kStride; };
   if ((int)blockIdx.x < (p.n * p.t) << part_log2) {
     const int row = blockIdx.x >> part_log2, part = blockIdx.x & ((1 << part_log2) - 1);
     const int i = row / p.n, head = row % p.n, kvh = head / rw.group, r = i * rw.group + head % rw.group;
@@ -892,12 +913,12 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int c = grp + j * groups;
-      first[j] = c < count ? __ldcg(reinterpret_cast<const float4*>(rec.at(c, busy) + in_rec + channel)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      first[j] = c < count ? __ldcg(reinterpret_cast<const float4*>(record_at(rec, c) + in_rec + channel)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    float* sums = merge_w + ctas + 1;
+    float* sums = merge_w + ctas;
     float top = -CUDART_INF_F, l = 0.0f;
     for (int c = tid; c < count; c += kMergeThreads) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(rec.at(c, busy) + in_rec + H));
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(record_at(rec, c) + in_rec + H));
       merge_w[c] = v.x;
       sums[c] = v.y;
       top = fmaxf(top, v.x);
@@ -915,7 +936,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
       if (c0 > grp) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
-          if (c0 + j * groups < count) first[j] = __ldcg(reinterpret_cast<const float4*>(rec.at(c0 + j * groups, busy) + in_rec + channel));
+          if (c0 + j * groups < count) first[j] = __ldcg(reinterpret_cast<const float4*>(record_at(rec, c0 + j * groups) + in_rec + channel));
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
@@ -969,12 +990,12 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
     __syncthreads();
     if (warp < rows) {
       float top = -CUDART_INF_F, l = 0.0f;
-      for (int j = lane; j < rec.count; j += 32) top = fmaxf(top, __ldcg(rec.at(j, busy) + in_rec));
+      for (int j = lane; j < rec.count; j += 32) top = fmaxf(top, __ldcg(record_at(rec, j) + in_rec));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       top = top == -CUDART_INF_F ? 0.0f : top;
       for (int j = lane; j < rec.count; j += 32) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(rec.at(j, busy) + in_rec));
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(record_at(rec, j) + in_rec));
         l += exp2f((v.x - top) * kLog2e) * v.y;
       }
 #pragma unroll
@@ -1009,16 +1030,17 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
   }
 }
 
-// CTAs of a launch: one per SM, fewer when even full caches leave some without a tile.
-int kv4_ctas(long long pairs, int s) {
-  const long long most = pairs * tiles_of(s);
-  const int sms = device_sm_count();
-  return most < sms ? (int)most : sms;
+// CTAs of a launch: one per SM, fewer when even full caches leave some without a tile, more where the pairs are so many that
+// their pieces would not find warps.
+int kv4_ctas(long long pairs, int s, int h) {
+  const long long most = pairs * tiles_of(s), room = (2 * pairs + kv4_warps(h) - 1) / kv4_warps(h);
+  const long long n = room > device_sm_count() ? room : device_sm_count();
+  return (int)(most < n ? most : n);
 }
 
 bool kv4_tensor_shape(int b, int t, int n, int nkv, int h, int s) {
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
-  return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX &&
+  return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX / 2 && pairs <= (1 << 19) && tiles_of(s) < (1 << 22) &&
          4ll * n * t + (long long)nkv * ((s + kScoreSlots - 1) / kScoreSlots) <= INT32_MAX;
 }
 
@@ -1026,8 +1048,8 @@ template <int H, int BLOCK, bool QF32>
 cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
   using T = Kv4Tile<H, BLOCK>;
   const long long pairs = (long long)p.cache.b * p.cache.nkv * kv4_rows(p.t, p.n, p.cache.nkv).chunks;
-  const int ctas = kv4_ctas(pairs, p.cache.s), pieces = ctas * T::kWarps;
-  float* logits = p.scores ? p.ws + kv4_records_floats(pieces, pairs, H) : nullptr;
+  const int ctas = kv4_ctas(pairs, p.cache.s, H);
+  float* logits = p.scores ? p.ws + kv4_records_floats((long long)ctas * T::kWarps, H) : nullptr;
   static bool done[64] = {false};
   int device = 0;
   cudaGetDevice(&device);
@@ -1044,7 +1066,7 @@ cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
   int part_log2 = 0;
   while (part_log2 < 2 && ((long long)p.cache.b * p.n * p.t << part_log2) < device_sm_count()) ++part_log2;
   return launch_chained(kv4_merge_kernel<H, QF32>, dim3(((p.n * p.t) << part_log2) + scores, p.cache.b), dim3(kMergeThreads),
-                        2 * sizeof(float) * (size_t)(ctas + 1), s, p, ctas, part_log2, (const float*)logits);
+                        2 * sizeof(float) * (size_t)ctas, s, p, ctas, part_log2, (const float*)logits);
 }
 template <int H, int BLOCK>
 cudaError_t launch_tensor_q(const Kv4Sdpa& p, cudaStream_t s) {
@@ -1062,7 +1084,7 @@ size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int 
   const size_t any = 2 * rows + rows * s;  // (also what queries off a 16-byte boundary need)
   if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return any * sizeof(float);
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
-  const size_t tensor = kv4_records_floats(kv4_ctas(pairs, s) * kv4_warps(h), pairs, h) +
+  const size_t tensor = kv4_records_floats((long long)kv4_ctas(pairs, s, h) * kv4_warps(h), h) +
                         (scores ? (size_t)pairs * tiles_of(s) * kSlots * 8 : 0);
   return (any > tensor ? any : tensor) * sizeof(float);
 }

@@ -17,7 +17,6 @@
 
 #include "common.cuh"
 #include "kernels.h"
-#include "pieces.cuh"
 #include "quant.cuh"
 
 namespace b200 {
@@ -25,6 +24,8 @@ namespace b200 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnit = 16;  // tokens per unit: the rows of one MMA tile and of one copy box
+
 enum : int { kKvF16 = 0, kKvI8 = 1, kKvF32 = 2 };
 
 template <int KV, int H, bool QF32>
@@ -76,6 +77,23 @@ constexpr size_t split_smem_bytes() {
 __device__ __forceinline__ int row_length(const SdpaParams& p, int b) {
   return p.lengths ? max(0, min(p.lengths[b], p.s_max)) : p.s_max;
 }
+__device__ __forceinline__ int units_of(int len) { return (len + kUnit - 1) / kUnit; }
+
+// How `total` units are cut: `ctas` pieces, the first `rest` of them one unit longer than the others. No piece is
+// shorter than min_units, so that short caches are not scattered over more records than they are worth.
+struct Pieces {
+  int ctas, size, rest;
+  __device__ __forceinline__ Pieces(int total, int grid, int min_units) {
+    ctas = max(1, min(grid, (total + min_units - 1) / min_units));
+    size = total / ctas;
+    rest = total - size * ctas;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c * size + min(c, rest); }
+  __device__ __forceinline__ int owner(int u) const {
+    const int longer = rest * (size + 1);
+    return u < longer ? u / (size + 1) : rest + (u - longer) / size;
+  }
+};
 
 // Units of all rows, and of the rows below `b`. Whole warp. (32 bits hold them: see sdpa_split_supported.)
 __device__ __forceinline__ void count_units(const SdpaParams& p, int b, int lane, int* total, int* below) {
@@ -654,6 +672,71 @@ __device__ __forceinline__ PairRecords pair_records(const SdpaParams& p, int b, 
   r.first = p.ws + ((size_t)c0 + (size_t)b * p.nkv + kvh) * 8 * (H + 4);
   r.count = c1 - c0 + 1;
   return r;
+}
+
+// Weights exp2(m_record - m) of a head's records, from their (maximum, sum) pairs at `ml`; returns the softmax
+// denominator, or kLostRecord where a record is one. Whole warp; the first 64 pairs in one round trip.
+__device__ __forceinline__ float record_weights(const float* ml, size_t stride, int count, int lane, float* weights) {
+  const float2 none = make_float2(-CUDART_INF_F, 0.0f);
+  const float2 a = lane < count ? __ldcg(reinterpret_cast<const float2*>(ml + lane * stride)) : none;
+  const float2 b = lane + 32 < count ? __ldcg(reinterpret_cast<const float2*>(ml + (lane + 32) * stride)) : none;
+  float mm = fmaxf(a.x, b.x);
+  for (int c = lane + 64; c < count; c += 32) mm = fmaxf(mm, __ldcg(ml + c * stride));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  const float muse = mm == -CUDART_INF_F ? 0.0f : mm;
+  const float fa = exp2f(a.x - muse), fb = exp2f(b.x - muse);
+  float l = fa * a.y + fb * b.y;
+  bool lost = a.y == kLostRecord || b.y == kLostRecord;
+  if (lane < count) weights[lane] = fa;
+  if (lane + 32 < count) weights[lane + 32] = fb;
+  for (int c = lane + 64; c < count; c += 32) {
+    const float2 v = __ldcg(reinterpret_cast<const float2*>(ml + c * stride));
+    const float f = exp2f(v.x - muse);
+    weights[c] = f;
+    l += f * v.y;
+    lost = lost || v.y == kLostRecord;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  return __any_sync(0xffffffffu, lost) ? kLostRecord : l;
+}
+
+// Sum of a head's records, weighted, for the four outputs d4 .. d4 + 3: records grp, grp + groups, ...
+// (`first`: the first kBatch of them, requested earlier).
+template <int kBatch>
+__device__ __forceinline__ float4 merge_quad(const float* base, size_t stride, int count, int grp, int groups, const float* weights,
+                                             const float4 (&first)[kBatch]) {
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float w, const float4& v) {
+    acc.x += w * v.x;
+    acc.y += w * v.y;
+    acc.z += w * v.z;
+    acc.w += w * v.w;
+  };
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) {
+    const int c = grp + j * groups;
+    if (c < count) add(weights[c], first[j]);
+  }
+  for (int c0 = grp + kBatch * groups; c0 < count; c0 += 4 * groups) {
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j * groups < count) v[j] = __ldcg(reinterpret_cast<const float4*>(base + (size_t)(c0 + j * groups) * stride));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j * groups < count) add(weights[c0 + j * groups], v[j]);
+  }
+  return acc;
+}
+template <int kBatch>
+__device__ __forceinline__ void request_quads(float4 (&v)[kBatch], const float* base, size_t stride, int count, int grp, int groups) {
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j) {
+    const int c = grp + j * groups;
+    v[j] = c < count ? __ldcg(reinterpret_cast<const float4*>(base + (size_t)c * stride)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
 }
 
 // Merges the records of one (row, query head): grid (n, b), 256 threads. What it costs are L2 round trips (0.7 us
