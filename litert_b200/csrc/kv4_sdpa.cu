@@ -147,33 +147,35 @@ cudaError_t launch_rows(const Kv4Sdpa& p, cudaStream_t s) {
 }
 
 // ---- head sizes 64, 128 and 256: tensor cores -------------------------------------------------------------
-// Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; a tile is 32 slots,
-// two 16-row sides of it whose chains of products and exponentials run side by side. Every (sequence, KV head, eight rows)
-// pair is cut into pieces of a common greatest length, one per warp. A warp walks through its piece without meeting another
-// one; at the end the warps of a CTA add their states of a common pair to one partial record (un-normalised outputs, maximum,
-// sum), and a second kernel merges a pair's records.
-// Measured with 16 ragged sequences of up to 8192 tokens, 8 heads x 256, replayed: pieces that run on from one pair to the
-// next (all of one length) 17.5 us, 4 of them in the warps that had parts of two pairs; such pieces per CTA 19.4; a record
-// for every warp 20.3 (the second kernel reads 9.8 MB then).
-constexpr int kSlots = 32;
+// Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; a tile is 16 slots.
+// Every (sequence, KV head, eight rows) pair is cut into pieces of a common greatest length, one per warp. A warp walks
+// through its piece without meeting another one; at the end the warps of a CTA add their states of a common pair to one
+// partial record (un-normalised outputs, maximum, sum). The CTA that finds the others' records of the pair complete (a
+// counter) merges them, sixteen at a time; a pair that lies in one CTA needs no record.
+//
+// What bounds a launch of a few microseconds is code that runs once: it is fetched, cold, at about eight cycles per
+// instruction, so loops outside the main one are rolled and both merges are the same code.
+constexpr int kSlots = 16;
 __host__ __device__ inline int tiles_of(int slots) { return (slots + kSlots - 1) / kSlots; }
 
-__host__ __device__ constexpr int kv4_warps(int h) { return h == 256 ? 8 : h == 128 ? 12 : 16; }
+__host__ __device__ constexpr int kv4_warps(int h) { return h == 256 ? 12 : 16; }
 
-template <int H, int BLOCK>
+template <int H, int BLOCK, bool QF32>
 struct Kv4Tile {
   static constexpr int kG = H / BLOCK;                 // blocks of a row
   static constexpr int kNibbleBytes = kSlots * H / 2;  // of the keys (or values) of a tile
   static constexpr int kPairBytes = kSlots * kG * 4;
   static constexpr int kBytes = 2 * (kNibbleBytes + kPairBytes);
+  static constexpr int kQueryBytes = H / 32 * 512 * (QF32 ? 2 : 1);  // a warp's query fragments
   static constexpr int kWarps = kv4_warps(H);
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kRec = H + 4;  // floats of a record per row: outputs, maximum, sum, padding
-  static constexpr int kFit = 220 * 1024 / (kWarps * kBytes);
+  static constexpr int kFit = (220 * 1024 / kWarps - kQueryBytes) / kBytes;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kRing = kWarps * kStages * kBytes;
-  static constexpr int kSmem = kRing + 128;
-  static_assert(8 * kRec * 4 <= kStages * kBytes, "a warp's state fits into its ring");
+  static constexpr int kWarpBytes = kQueryBytes + kStages * kBytes;
+  static constexpr int kRecords = 16 * 8 * kRec * 4;  // sixteen records to merge
+  static constexpr int kSmem = (kWarps * kWarpBytes > kRecords ? kWarps * kWarpBytes : kRecords) + 128;
+  static_assert(8 * kRec * 4 <= kWarpBytes, "a warp's state fits into its part");
   static_assert(kBytes % 128 == 0 && kStages >= 2 && kSmem <= 221 * 1024, "layout");
 };
 
@@ -185,8 +187,12 @@ __host__ __device__ inline Kv4Rows kv4_rows(int t, int n, int nkv) {
   return {group, rows, (rows + 7) / 8};
 }
 
-// Workspace of the tensor-core kernels: a record per piece (of which the first of a pair in each CTA is written), then the
-// logits [pair][slot (rounded up to a tile)][8 rows] where scores are wanted.
+// Workspace: counters (two per piece, zero between calls), then of the tensor-core kernels a record per piece (of which the
+// first of a pair in each CTA is used) and, where scores are wanted, the rows' {maximum, 1 / sum} [pair][8 rows] and the logits
+// [pair][slot (rounded up to a tile)][8 rows].
+constexpr int kMostPieces = 65536;
+constexpr size_t kCounterFloats = 2 * (size_t)kMostPieces;
+constexpr int kFanIn = 16;  // records that one CTA merges in one round trip
 __host__ __device__ inline size_t kv4_records_floats(long long pieces, int h) { return (size_t)pieces * 8 * (h + 4); }
 
 __device__ __forceinline__ int kv4_length(const Kv4Sdpa& p, int b) {
@@ -201,11 +207,19 @@ __device__ __forceinline__ int divide(int a, int b, float inverse) {
   return q;
 }
 
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // How the pairs are cut: into pieces of up to about `size` tiles, each pair's of equal lengths (to a tile), the smallest size
-// that needs no more pieces than there are warps. Every CTA gets an equal number of the pieces (to one). What is rounded
-// here is so in both kernels.
+// that needs no more pieces than there are warps. Every CTA gets an equal number of the pieces (to one).
+// Few tiles are not scattered over more CTAs than they are worth: where every pair has at most four tiles per warp of a CTA, it
+// gets a CTA to itself; up to four tiles per warp of sixteen CTAs, it gets about these.
 struct Kv4Cut {
-  int size, each, longer;  // the first `longer` CTAs have one piece more than `each`
+  bool own_cta;            // a pair is a CTA's, in pieces of equal lengths
+  int size, each, longer;  // otherwise: the first `longer` CTAs have one piece more than `each`
   float inverse;           // 1 / size
   int len;                 // attended slots of sequence `lane`
   __device__ __forceinline__ int pieces_of(int slots) const {
@@ -215,32 +229,41 @@ struct Kv4Cut {
   __device__ __forceinline__ int begin(int cta) const { return cta * each + min(cta, longer); }
   __device__ __forceinline__ int owner(int piece) const {
     const int front = longer * (each + 1);
-    return piece < front ? divide(piece, each + 1, __frcp_rn((float)(each + 1))) : longer + divide(piece - front, each, __frcp_rn((float)each));
+    return piece < front ? divide(piece, each + 1, reciprocal((float)(each + 1))) : longer + divide(piece - front, each, reciprocal((float)each));
   }
 };
-// Pieces of the sequences below `upto`, all pairs. Whole warp.
-__device__ __forceinline__ int count_pieces(const Kv4Sdpa& p, int per, const Kv4Cut& c, int lane, int upto) {
-  int n = lane < upto ? c.pieces_of(c.len) * per : 0;
-  for (int i = lane + 32; i < upto; i += 32) n += c.pieces_of(kv4_length(p, i)) * per;
-  return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
-}
 __device__ __forceinline__ Kv4Cut kv4_cut(const Kv4Sdpa& p, int per, int ctas, int warps, int lane) {
-  const int room = ctas * warps;
-  const float inverse_room = __frcp_rn((float)room), inverse_ctas = __frcp_rn((float)ctas);
+  const int pairs = p.cache.b * per;
   Kv4Cut c;
   c.len = lane < p.cache.b ? kv4_length(p, lane) : 0;
-  int total = tiles_of(c.len) * per;
-  for (int i = lane + 32; i < p.cache.b; i += 32) total += tiles_of(kv4_length(p, i)) * per;
+  int total = tiles_of(c.len) * per, most = tiles_of(c.len);
+#pragma unroll 1
+  for (int i = lane + 32; i < p.cache.b; i += 32) {
+    const int tiles = tiles_of(kv4_length(p, i));
+    total += tiles * per;
+    most = max(most, tiles);
+  }
   total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
-  c.size = max(1, (int)ceilf((float)total * inverse_room));
+  most = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+  c.own_cta = pairs <= ctas && most <= 4 * warps;
+  c.size = c.each = c.longer = 1;
+  c.inverse = 1.0f;
+  if (c.own_cta) return c;
+  if (total <= 4 * kFanIn * pairs * warps) ctas = min(ctas, kFanIn * pairs);
+  const int room = ctas * warps;
+  c.size = max(1, (int)ceilf((float)total * reciprocal((float)room)));
   int n;
+#pragma unroll 1
   while (true) {  // (ends: there is room for twice the pairs, and a large enough size makes a piece of each)
-    c.inverse = __frcp_rn((float)c.size);
-    n = count_pieces(p, per, c, lane, p.cache.b);
+    c.inverse = reciprocal((float)c.size);
+    n = c.pieces_of(c.len) * per;
+#pragma unroll 1
+    for (int i = lane + 32; i < p.cache.b; i += 32) n += c.pieces_of(kv4_length(p, i)) * per;
+    n = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
     if (n <= room) break;
     c.size += 1 + c.size / 16;
   }
-  c.each = divide(n, ctas, inverse_ctas);
+  c.each = divide(n, ctas, reciprocal((float)ctas));
   c.longer = n - c.each * ctas;
   return c;
 }
@@ -261,6 +284,12 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
@@ -299,18 +328,6 @@ __device__ __forceinline__ float power2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-template <int N>
-__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
-  if constexpr (N == 1) {
-    v[0] = lds32(a);
-  } else if constexpr (N == 2) {
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]) : "r"(a + 4 * i));
-  }
 }
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
   uint32_t y;
@@ -351,45 +368,77 @@ __device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t centred_low(uint32_t w) { return half2_sub((w & kLowNibbles) | 0x64006400u, 0x64086408u); }    // - 1032
-__device__ __forceinline__ uint32_t centred_high(uint32_t w) { return half2_sub((w & kHighNibbles) | 0x54005400u, 0x54805480u); }  // - 72
+// (w & mask) | exponent in one instruction: the exponents stay in registers.
+struct Centred {
+  uint32_t unit, eighth;
+  __device__ __forceinline__ Centred() {
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(unit));
+    asm volatile("mov.b32 %0, 0x54005400;" : "=r"(eighth));
+  }
+  __device__ __forceinline__ static uint32_t splice(uint32_t w, uint32_t mask, uint32_t exponent) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(exponent));
+    return r;
+  }
+  __device__ __forceinline__ uint32_t low(uint32_t w) const { return half2_sub(splice(w, kLowNibbles, unit), 0x64086408u); }      // - 1032
+  __device__ __forceinline__ uint32_t high(uint32_t w) const { return half2_sub(splice(w, kHighNibbles, eighth), 0x54805480u); }  // - 72
+};
 
 template <int H, int BLOCK, bool QF32>
-__global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, float* logits_ws) {
-  using T = Kv4Tile<H, BLOCK>;
+__global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, float2* stats_ws, float* logits_ws) {
+  using T = Kv4Tile<H, BLOCK, QF32>;
   constexpr int G = T::kG;
-  constexpr int P = H / 32;           // 16-byte pieces of a row
-  constexpr int kPer = BLOCK / 32;    // of them in a block
+  constexpr int P = H / 32;         // 16-byte pieces of a row
+  constexpr int kPer = BLOCK / 32;  // of them in a block
+  constexpr int kWarps = T::kWarps;
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
-  __shared__ float s_m[T::kWarps][8], s_l[T::kWarps][8];  // maxima and sums of the warps' states
-  __shared__ int s_pair[T::kWarps];                       // and whose these are
-  __shared__ int s_rows[T::kWarps];
+  struct Whose {
+    int pair, count, index, first;  // the pair, its records in all, which of them is this CTA's, the pair's first piece
+  };
+  __shared__ Whose s_of[kWarps];     // whose the warps' states are
+  __shared__ float s_f[kFanIn][8];   // their factors in a sum
+  __shared__ float s_top[8];
+  __shared__ int s_last[kWarps];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int nkv = p.cache.nkv, s_max = p.cache.s;
   const Kv4Rows rw = kv4_rows(p.t, p.n, nkv);
   const int per = nkv * rw.chunks;  // pairs per sequence
-  // this warp's ring; where a lane's copies come from and go to (16-byte piece `lane % P` of rows lane / P + 32 / P j)
-  const uint32_t ring = smem_u32(smem) + (uint32_t)(w * T::kStages * T::kBytes);
+  // this warp's part of the shared memory; where a lane's copies come from and go to (16-byte piece `lane % P` of rows
+  // lane / P + 32 / P j)
+  const uint32_t part_at = smem_u32(smem) + (uint32_t)(w * T::kWarpBytes), ring = part_at + T::kQueryBytes;
   const uint32_t row_pitch = (uint32_t)nkv * (H / 2), pair_pitch = (uint32_t)nkv * G * 4;  // bytes
   const int copy_row = lane / P, copy_piece = lane % P;
   const uint32_t copy_from = (uint32_t)copy_row * row_pitch + copy_piece * 16, pair_from = (uint32_t)(lane / G) * pair_pitch + lane % G * 4;
   const uint32_t row_step = row_pitch * (32 / P), pair_step = pair_pitch * (32 / G);
+  constexpr int kCopies = kSlots * P / 32, kPairCopies = (kSlots * G + 31) / 32;
   // the row that this lane names for a load of matrices: of two pieces, rows 0 .. 15
   const uint32_t matrix_at = piece_at<H>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
-  const float inverse_chunks = __frcp_rn((float)rw.chunks), inverse_group = __frcp_rn((float)rw.group);
+  const float inverse_chunks = reciprocal((float)rw.chunks), inverse_group = reciprocal((float)rw.group), inverse_per = reciprocal((float)per);
   pdl_wait();
   // (only now: what a dependent kernel does ahead of its own wait may then read this kernel's inputs)
   pdl_launch_dependents();
-  // this warp's piece
-  const Kv4Cut cut = kv4_cut(p, per, gridDim.x, T::kWarps, lane);
-  const int first_piece = cut.begin(blockIdx.x), piece = first_piece + w;
-  int seg = 0, b = 0, in_b = 0, unit = 0, len = cut.len;  // seg tiles from `unit` on of pair in_b of sequence b
-  if (w < cut.each + ((int)blockIdx.x < cut.longer ? 1 : 0)) {
+  // this warp's piece: seg tiles from `unit` on of pair in_b of sequence b
+  const Kv4Cut cut = kv4_cut(p, per, gridDim.x, kWarps, lane);
+  int seg = 0, b = 0, in_b = 0, unit = 0, len = cut.len;
+  Whose of{-1, 1, 0, 0};
+  if (cut.own_cta) {
+    if ((int)blockIdx.x < p.cache.b * per) {
+      b = divide(blockIdx.x, per, inverse_per);
+      in_b = blockIdx.x - b * per;
+      len = p.cache.b <= 32 ? __shfl_sync(0xffffffffu, len, b) : kv4_length(p, b);
+      const int tiles = tiles_of(len), each = tiles / kWarps, longer = tiles - each * kWarps;
+      unit = w * each + min(w, longer);
+      seg = each + (w < longer ? 1 : 0);
+      if (w == 0 || seg > 0) of.pair = blockIdx.x;  // (a pair without a slot has zeros to write)
+    }
+  } else if (w < cut.each + ((int)blockIdx.x < cut.longer ? 1 : 0)) {
+    const int piece = cut.begin(blockIdx.x) + w;
+#pragma unroll 1
     for (int b0 = 0, base = 0; b0 < p.cache.b; b0 += 32) {
       if (b0 > 0) len = b0 + lane < p.cache.b ? kv4_length(p, b0 + lane) : 0;
       int n = cut.pieces_of(len), upto = n * per;  // inclusive prefix sum over the lanes
-#pragma unroll
+#pragma unroll 1
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
@@ -401,35 +450,35 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
         len = __shfl_sync(0xffffffffu, len, src);
         n = __shfl_sync(0xffffffffu, n, src);
         b = b0 + src;
-        const float inverse = __frcp_rn((float)n);
+        const float inverse = reciprocal((float)n);
         in_b = divide(rest, n, inverse);
         const int part = rest - in_b * n, tiles = tiles_of(len), each = divide(tiles, n, inverse), longer = tiles - each * n;
         unit = part * each + min(part, longer);
         seg = each + (part < longer ? 1 : 0);
+        of.pair = b * per + in_b;
+        of.first = piece - part;
         break;
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
-  if (lane == 0) s_pair[w] = -1;  // no state yet
 
   if (seg > 0) {
     const int kvh = divide(in_b, rw.chunks, inverse_chunks), chunk = in_b - kvh * rw.chunks;
-    const int pair = b * per + in_b;
     // the queries are asked for first, the tiles arrive meanwhile
-    const int q_row = chunk * 8 + g;
     uint4 q_bits[QF32 ? 2 * P : P];
     {
+      const int q_row = min(chunk * 8 + g, rw.rows - 1);  // (columns without a row repeat the last one and are dropped)
       const int i = divide(q_row, rw.group, inverse_group);
       const size_t at = (((size_t)b * p.t + i) * p.n + kvh * rw.group + (q_row - i * rw.group)) * H + 8 * t;
 #pragma unroll
       for (int sl = 0; sl < P; ++sl) {
         if constexpr (QF32) {
           const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.q) + at + 32 * sl);
-          q_bits[2 * sl] = q_row < rw.rows ? __ldg(src) : make_uint4(0, 0, 0, 0);
-          q_bits[2 * sl + 1] = q_row < rw.rows ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+          q_bits[2 * sl] = __ldg(src);
+          q_bits[2 * sl + 1] = __ldg(src + 1);
         } else {
-          q_bits[sl] = q_row < rw.rows ? __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + at + 32 * sl)) : make_uint4(0, 0, 0, 0);
+          q_bits[sl] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + at + 32 * sl));
         }
       }
     }
@@ -450,18 +499,20 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
           const void* kps = reinterpret_cast<const uint8_t*>(kp_next) + pair_from;
           const void* vps = reinterpret_cast<const uint8_t*>(vp_next) + pair_from;
 #pragma unroll
-          for (int j = 0; j < P; ++j) {
+          for (int j = 0; j < kCopies; ++j) {
             cp_async16(to + piece_at<H>(copy_row + j * (32 / P), copy_piece), advance(ks, j, row_step));
             cp_async16(to + T::kNibbleBytes + piece_at<H>(copy_row + j * (32 / P), copy_piece), advance(vs, j, row_step));
           }
 #pragma unroll
-          for (int j = 0; j < G; ++j) {
-            cp_async4(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, advance(kps, j, pair_step));
-            cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, advance(vps, j, pair_step));
+          for (int j = 0; j < kPairCopies; ++j) {
+            if (lane + 32 * j < kSlots * G) {
+              cp_async4(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, advance(kps, j, pair_step));
+              cp_async4(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, advance(vps, j, pair_step));
+            }
           }
         } else {  // (one tile of a pair at most)
 #pragma unroll 1
-          for (int j = 0; j < P; ++j) {
+          for (int j = 0; j < kCopies; ++j) {
             const int row = copy_row + j * (32 / P);
             const bool ok = row < there;
             const uint32_t from = ok ? copy_from + j * row_step : 0u;
@@ -469,11 +520,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
             cp_async16_or_zero(to + T::kNibbleBytes + piece_at<H>(row, copy_piece), v_next + from, ok);
           }
 #pragma unroll 1
-          for (int j = 0; j < G; ++j) {
-            const bool ok = (lane + 32 * j) / G < there;
-            const uint32_t from = ok ? pair_from + j * pair_step : 0u;
-            cp_async4_or_zero(to + 2 * T::kNibbleBytes + (lane + 32 * j) * 4, reinterpret_cast<const uint8_t*>(kp_next) + from, ok);
-            cp_async4_or_zero(to + 2 * T::kNibbleBytes + T::kPairBytes + (lane + 32 * j) * 4, reinterpret_cast<const uint8_t*>(vp_next) + from, ok);
+          for (int e = lane; e < kSlots * G; e += 32) {
+            const bool ok = e / G < there;
+            const uint32_t from = ok ? (uint32_t)(e / G) * pair_pitch + e % G * 4 : 0u;
+            cp_async4_or_zero(to + 2 * T::kNibbleBytes + e * 4, reinterpret_cast<const uint8_t*>(kp_next) + from, ok);
+            cp_async4_or_zero(to + 2 * T::kNibbleBytes + T::kPairBytes + e * 4, reinterpret_cast<const uint8_t*>(vp_next) + from, ok);
           }
         }
         k_next += (size_t)kSlots * row_pitch;
@@ -488,92 +539,104 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 #pragma unroll 1
     for (int k = 0; k < T::kStages - 1; ++k) request();
 
-    // Queries: thread (g, t) holds row g's elements at its words of a key, as the B operand. They are scaled by a power of
-    // two that brings the row's largest to 2^10 .. 2^11: dividing by 16 then loses nothing above 2^-36 of it, and a float32
-    // query is two fp16 numbers to 22 bits.
-    uint32_t q_high[P][4], q_low[QF32 ? P : 1][4];
+    // Queries: thread (g, t) makes row g's elements at its words of a key, as the B operand: channels 0, 4 | 2, 6 of a word
+    // meet low nibbles, 1, 5 | 3, 7 high ones. They are scaled by a power of two that brings the row's largest to 2^5 ..
+    // 2^6: dividing by 16 then loses nothing above 2^-26 of it, and a float32 query is two fp16 numbers to 22 bits.
+    // They are kept in shared memory, [piece][lane][4 words] (and again for the low halves).
+    const uint32_t query_at = part_at + lane * 16;
     float q_sum[G][2], factor[2];  // of the rows 2 t and 2 t + 1 (the products' columns)
-    int limit[2];
     {
-      float raw[P][8], top = 0.0f;
+      float top;
+      if constexpr (QF32) {
+        top = 0.0f;
 #pragma unroll
-      for (int sl = 0; sl < P; ++sl) {
-        if constexpr (QF32) {
-          const uint4 lo = q_bits[2 * sl], hi = q_bits[2 * sl + 1];
-          raw[sl][0] = __uint_as_float(lo.x), raw[sl][1] = __uint_as_float(lo.y), raw[sl][2] = __uint_as_float(lo.z), raw[sl][3] = __uint_as_float(lo.w);
-          raw[sl][4] = __uint_as_float(hi.x), raw[sl][5] = __uint_as_float(hi.y), raw[sl][6] = __uint_as_float(hi.z), raw[sl][7] = __uint_as_float(hi.w);
-        } else {
-          const uint4 v = q_bits[sl];
-          const float2 f0 = pair_floats(v.x), f1 = pair_floats(v.y), f2 = pair_floats(v.z), f3 = pair_floats(v.w);
-          raw[sl][0] = f0.x, raw[sl][1] = f0.y, raw[sl][2] = f1.x, raw[sl][3] = f1.y;
-          raw[sl][4] = f2.x, raw[sl][5] = f2.y, raw[sl][6] = f3.x, raw[sl][7] = f3.y;
-        }
+        for (int i = 0; i < 2 * P; ++i)
+          top = fmaxf(fmaxf(fmaxf(top, fabsf(__uint_as_float(q_bits[i].x))), fabsf(__uint_as_float(q_bits[i].y))),
+                      fmaxf(fabsf(__uint_as_float(q_bits[i].z)), fabsf(__uint_as_float(q_bits[i].w))));
+      } else {
+        uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(raw[sl][e]));
+        for (int i = 0; i < P; ++i)
+          most = __vmaxu2(__vmaxu2(__vmaxu2(most, q_bits[i].x & 0x7fff7fffu), q_bits[i].y & 0x7fff7fffu),
+                          __vmaxu2(q_bits[i].z & 0x7fff7fffu, q_bits[i].w & 0x7fff7fffu));
+        const float2 f = pair_floats(most);
+        top = fmaxf(f.x, f.y);
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int exponent = __float_as_int(top) >> 23;
-      const int up = exponent == 255 ? 127 : min(264 - exponent, 253);  // (an infinite query stays what it is)
-      const float scale_up = __int_as_float(up << 23), scale_down = __int_as_float((254 - up) << 23);
-      float sums[G];
-#pragma unroll
-      for (int gr = 0; gr < G; ++gr) sums[gr] = 0.0f;
-#pragma unroll
-      for (int sl = 0; sl < P; ++sl) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          raw[sl][e] *= scale_up;
-          sums[sl / kPer] += raw[sl][e];
-        }
-        // channels 0, 4 | 2, 6 meet low nibbles, 1, 5 | 3, 7 high ones
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int c = e < 2 ? 2 * e : 2 * (e - 2) + 1;
-          const float f = e < 2 ? 1.0f : 0.0625f;
-          if constexpr (QF32) {
-            split_halves(raw[sl][c] * f, raw[sl][c + 4] * f, q_high[sl][e], q_low[sl][e]);
-          } else {
-            q_high[sl][e] = halves(raw[sl][c] * f, raw[sl][c + 4] * f);
-          }
-        }
-      }
+      const int field = __float_as_int(top) >> 23;
+      const int up = field == 255 ? 0 : min(132 - field, QF32 ? 126 : 29);  // (an infinite query stays what it is)
+      const float scale_up = __int_as_float((127 + up) << 23), scale_down = __int_as_float((127 - up) << 23);
+      // 2^up as a product of two halves
+      const __half2 one = __float2half2_rn(__int_as_float((127 + min(up, 15)) << 23)), two = __float2half2_rn(__int_as_float((127 + max(up - 15, 0)) << 23));
+      const __half2 sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
-        sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], 1);
-        sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], 2);
-        sums[gr] *= 0x1p-24f;
-        q_sum[gr][0] = __shfl_sync(0xffffffffu, sums[gr], 8 * t);
-        q_sum[gr][1] = __shfl_sync(0xffffffffu, sums[gr], 8 * t + 4);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int sl = gr * kPer; sl < (gr + 1) * kPer; ++sl) {
+          uint32_t high[4], low[4];
+          if constexpr (QF32) {
+            const uint4 lo = q_bits[2 * sl], hi = q_bits[2 * sl + 1];
+            const float even = scale_up, odd = scale_up * 0.0625f;
+            split_halves(__uint_as_float(lo.x) * even, __uint_as_float(hi.x) * even, high[0], low[0]);
+            split_halves(__uint_as_float(lo.z) * even, __uint_as_float(hi.z) * even, high[1], low[1]);
+            split_halves(__uint_as_float(lo.y) * odd, __uint_as_float(hi.y) * odd, high[2], low[2]);
+            split_halves(__uint_as_float(lo.w) * odd, __uint_as_float(hi.w) * odd, high[3], low[3]);
+            sts128(query_at + (P + sl) * 512, low);
+          } else {
+            uint32_t v[4] = {q_bits[sl].x, q_bits[sl].y, q_bits[sl].z, q_bits[sl].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __half2 y = __hmul2(__hmul2(*reinterpret_cast<const __half2*>(&v[e]), one), two);
+              v[e] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              high[e] = __byte_perm(v[e], v[e + 2], 0x5410);
+              const uint32_t odd = __byte_perm(v[e], v[e + 2], 0x7632);
+              const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&odd), sixteenth);
+              high[2 + e] = *reinterpret_cast<const uint32_t*>(&y);
+            }
+          }
+          sts128(query_at + sl * 512, high);
+          // the blocks' sums: products with ones (and sixteens)
+#pragma unroll
+          for (int odd = 0; odd < 2; ++odd) {
+            const uint32_t ones = odd ? 0x4c004c00u : 0x3c003c00u;
+            product(sum, ones, ones, ones, ones, high[2 * odd], high[2 * odd + 1]);
+            if constexpr (QF32) product(sum, ones, ones, ones, ones, low[2 * odd], low[2 * odd + 1]);
+          }
+        }
+        q_sum[gr][0] = sum[0] * 0x1p-24f;
+        q_sum[gr][1] = sum[1] * 0x1p-24f;
       }
       const float f = scale_down * p.scale;
       // (in two steps: 2^24 times a small scale stays within fp32 either way)
       factor[0] = __shfl_sync(0xffffffffu, f, 8 * t) * 0x1p24f;
       factor[1] = __shfl_sync(0xffffffffu, f, 8 * t + 4) * 0x1p24f;
     }
+    int limit[2];
     const float* mask[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = chunk * 8 + 2 * t + e, i = divide(r, rw.group, inverse_group);
-      limit[e] = r < rw.rows ? kv4_limit(len, s_max, p.t, i) : len;  // (columns without a row are computed and dropped)
-      mask[e] = p.mask && r < rw.rows ? p.mask + ((size_t)b * p.t + i) * s_max : nullptr;
+      const int i = divide(min(chunk * 8 + 2 * t + e, rw.rows - 1), rw.group, inverse_group);
+      limit[e] = kv4_limit(len, s_max, p.t, i);
+      mask[e] = p.mask ? p.mask + ((size_t)b * p.t + i) * s_max : nullptr;
     }
     const int least_limit = kv4_limit(len, s_max, p.t, divide(chunk * 8, rw.group, inverse_group));  // of any row
     // masks are requested a tile ahead of their use
-    auto masks = [&](int k, float (&m)[2][4]) {
-      const int first = (unit + k) * kSlots;
+    float next_mask[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto ask_masks = [&](int first) {
 #pragma unroll
-      for (int side = 0; side < 2; ++side)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int slot = first + 16 * side + g + 8 * (e >> 1);
-          m[side][e] = mask[e & 1] && k < seg && slot < limit[e & 1] ? __ldg(mask[e & 1] + slot) : 0.0f;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int slot = first + g + 8 * (e >> 1);
+        if (slot < limit[e & 1]) next_mask[e] = __ldg(mask[e & 1] + slot);
+      }
     };
-    float next_mask[2][4];
-    masks(0, next_mask);
-    const bool guard = p.mask != nullptr || p.t > 1;  // slots that some row does not see may hold anything
-    float* logits = logits_ws ? logits_ws + (size_t)pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
+    if (p.mask) ask_masks(unit * kSlots);
+    const bool guard = p.mask != nullptr || p.t > 1;
+    float* logits = logits_ws ? logits_ws + (size_t)of.pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
 
     // outputs: of piece i and its channels 4 g + {0, 1} and 4 g + {2, 3}, rows 2 t and 2 t + 1
     float o[P][2][4], least_sum[G];
@@ -586,107 +649,108 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
     float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, m_use[2] = {0.0f, 0.0f}, l_run[2] = {0.0f, 0.0f};
     uint32_t exponent = 1;  // fp16 exponent field of the largest value scale so far: weights are in units of 2^(exponent - 23)
 
+    const Centred centred;
     uint32_t at = ring;
+    int first = unit * kSlots;
+    const int behind = first + seg * kSlots;
 #pragma unroll 1
-    for (int k = 0; k < seg; ++k, at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes) {
+    for (; first < behind; first += kSlots, at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes) {
       cp_async_wait<T::kStages - 2>();
       __syncwarp();  // the tile is there, and everybody is done with the one whose place the next request takes
       request();
       const uint32_t pairs_at = at + 2 * T::kNibbleBytes;
-      const int first = (unit + k) * kSlots;
 
-      // -- logits of slots g, g + 8 (+ 16), rows 2 t and 2 t + 1 --
-      float x[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-      // Four pieces and both sides at a time, one product of each chain after the other: a warp waits for a chain's last
-      // product before its next.
-      constexpr int kAtOnce = P < 4 ? P : 4, kChains = kAtOnce / kPer;
+      // -- logits of slots g and g + 8, rows 2 t and 2 t + 1 --
+      // One product of each chain after the other: a warp waits for a chain's last product before its next.
+      constexpr int kAtOnce = P, kChains = kAtOnce / kPer, kApart = kChains < 4 ? 2 : 1;
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i0 = 0; i0 < P; i0 += kAtOnce) {
-        uint32_t words[2][kAtOnce / 2][4];
+        uint32_t words[kAtOnce / 2][4];
 #pragma unroll
-        for (int i = 0; i < kAtOnce; i += 2)
-#pragma unroll
-          for (int side = 0; side < 2; ++side)
-            load_matrices(at + (matrix_at ^ (uint32_t)((i0 + i) * 16)) + side * 8 * H, words[side][i / 2]);
-        float acc[2][kChains][4];
+        for (int i = 0; i < kAtOnce; i += 2) load_matrices(at + (matrix_at ^ (uint32_t)((i0 + i) * 16)), words[i / 2]);
+        float acc[kChains][kApart][4];  // (few chains: low and high nibbles apart)
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
+          uint32_t qs[kChains][4], qls[QF32 ? kChains : 1][4];
 #pragma unroll
-          for (int odd = 0; odd < 2; ++odd)
+          for (int c = 0; c < kChains; ++c) {
+            lds128(query_at + (i0 + c * kPer + j) * 512, qs[c]);
+            if constexpr (QF32) lds128(query_at + (P + i0 + c * kPer + j) * 512, qls[c]);
+          }
 #pragma unroll
-            for (int c = 0; c < kChains; ++c)
+          for (int odd = 0; odd < 2; ++odd) {
 #pragma unroll
-              for (int side = 0; side < 2; ++side) {
-                const int i = c * kPer + j;
-                const uint32_t wa = words[side][i / 2][2 * (i & 1)], wb = words[side][i / 2][2 * (i & 1) + 1];
-                const uint32_t keep = odd ? kHighNibbles : kLowNibbles;
-                const uint32_t a0 = wa & keep, a1 = wb & keep, a2 = (wa >> 8) & keep, a3 = (wb >> 8) & keep;
-                if (j == 0 && odd == 0) {
-                  first_product(acc[side][c], a0, a1, a2, a3, q_high[i0 + i][0], q_high[i0 + i][1]);
-                } else {
-                  product(acc[side][c], a0, a1, a2, a3, q_high[i0 + i][2 * odd], q_high[i0 + i][2 * odd + 1]);
-                }
-                if constexpr (QF32) product(acc[side][c], a0, a1, a2, a3, q_low[i0 + i][2 * odd], q_low[i0 + i][2 * odd + 1]);
+            for (int c = 0; c < kChains; ++c) {
+              const int i = c * kPer + j;
+              const uint32_t (&q)[4] = qs[c];
+              const uint32_t (&ql)[4] = qls[QF32 ? c : 0];
+              const uint32_t wa = words[i / 2][2 * (i & 1)], wb = words[i / 2][2 * (i & 1) + 1];
+              const uint32_t keep = odd ? kHighNibbles : kLowNibbles;
+              const uint32_t a0 = wa & keep, a1 = wb & keep, a2 = (wa >> 8) & keep, a3 = (wb >> 8) & keep;
+              float (&to_acc)[4] = acc[c][odd % kApart];
+              if (j == 0 && odd < kApart) {
+                first_product(to_acc, a0, a1, a2, a3, q[2 * odd], q[2 * odd + 1]);
+              } else {
+                product(to_acc, a0, a1, a2, a3, q[2 * odd], q[2 * odd + 1]);
               }
+              if constexpr (QF32) product(to_acc, a0, a1, a2, a3, ql[2 * odd], ql[2 * odd + 1]);
+            }
+          }
         }
 #pragma unroll
-        for (int c = 0; c < kChains; ++c)
+        for (int c = 0; c < kChains; ++c) {
+          const int gr = i0 / kPer + c;
+          const float2 fa = pair_floats(lds32(pairs_at + (uint32_t)((g * G + gr) * 4)));
+          const float2 fb = pair_floats(lds32(pairs_at + (uint32_t)(((g + 8) * G + gr) * 4)));
 #pragma unroll
-          for (int side = 0; side < 2; ++side) {
-            const int gr = i0 / kPer + c;
-            const float2 fa = pair_floats(lds32(pairs_at + (uint32_t)(((16 * side + g) * G + gr) * 4)));
-            const float2 fb = pair_floats(lds32(pairs_at + (uint32_t)(((16 * side + g + 8) * G + gr) * 4)));
-            x[side][0] = fmaf(fa.x, acc[side][c][0], fmaf(fa.y, q_sum[gr][0], x[side][0]));
-            x[side][1] = fmaf(fa.x, acc[side][c][1], fmaf(fa.y, q_sum[gr][1], x[side][1]));
-            x[side][2] = fmaf(fb.x, acc[side][c][2], fmaf(fb.y, q_sum[gr][0], x[side][2]));
-            x[side][3] = fmaf(fb.x, acc[side][c][3], fmaf(fb.y, q_sum[gr][1], x[side][3]));
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = e < 2 ? fa : fb;
+            x[e] = fmaf(f.x, kApart == 2 ? acc[c][0][e] + acc[c][kApart - 1][e] : acc[c][0][e], fmaf(f.y, q_sum[gr][e & 1], x[e]));
           }
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] *= factor[e & 1];
+      for (int e = 0; e < 4; ++e) x[e] *= factor[e & 1];
       if (p.logit_cap > 0.0f) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = p.logit_cap * tanhf(x[e >> 2][e & 3] / p.logit_cap);
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {  // (the four values in turn: one copy of the function's code)
+          const float y = p.logit_cap * tanhf(x[0] / p.logit_cap);
+          x[0] = x[1], x[1] = x[2], x[2] = x[3], x[3] = y;
+        }
       }
       if (p.mask) {
-        float m[2][4];
+        float m[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m[e >> 2][e & 3] = next_mask[e >> 2][e & 3];
-        masks(k + 1, next_mask);
+        for (int e = 0; e < 4; ++e) m[e] = next_mask[e];
+        ask_masks(first + kSlots);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float a = m[e >> 2][e & 3];
-          x[e >> 2][e & 3] = a == -CUDART_INF_F ? a : x[e >> 2][e & 3] + a;
-        }
+        for (int e = 0; e < 4; ++e) x[e] = m[e] == -CUDART_INF_F ? m[e] : x[e] + m[e];
       }
       if (first + kSlots > least_limit) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int slot = first + 16 * (e >> 2) + g + 8 * ((e >> 1) & 1);
-          x[e >> 2][e & 3] = slot < limit[e & 1] ? x[e >> 2][e & 3] : -CUDART_INF_F;
-        }
+        for (int e = 0; e < 4; ++e) x[e] = first + g + 8 * (e >> 1) < limit[e & 1] ? x[e] : -CUDART_INF_F;
       }
       if (logits) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<float2*>(logits + (size_t)(first + g + 8 * e) * 8 + 2 * t) = make_float2(x[e >> 1][2 * (e & 1)], x[e >> 1][2 * (e & 1) + 1]);
+        float* to_ws = logits + (size_t)(first + g) * 8 + 2 * t;
+        *reinterpret_cast<float2*>(to_ws) = make_float2(x[0], x[1]);
+        *reinterpret_cast<float2*>(to_ws + 64) = make_float2(x[2], x[3]);
       }
 
       // -- running maximum and unit; both rarely change --
       // A weight may exceed 1 by e^kSlack: rescaling the outputs at every new maximum would happen in most tiles while a
       // warp has seen few. The largest value scale of the tile: pairs compared as halves.
       constexpr float kSlack = 4.0f;
-      __half2 largest = __float2half2_rn(0.0f);
+      uint32_t largest = 0;
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const uint32_t pw_ = lds32(pairs_at + T::kPairBytes + (uint32_t)(lane + 32 * j) * 4);
-        largest = __hmax2(largest, *reinterpret_cast<const __half2*>(&pw_));
+      for (int j = 0; j < kPairCopies; ++j) {
+        const int e = (lane + 32 * j) % (kSlots * G);  // (H = 64: every pair twice)
+        largest = __vmaxu2(largest, lds32(pairs_at + T::kPairBytes + (uint32_t)e * 4) & 0x7fff7fffu);
       }
-      const uint32_t largest_bits = *reinterpret_cast<const uint32_t*>(&largest) & 0x7fffu;
-      const uint32_t now = max(exponent, min(__reduce_max_sync(0xffffffffu, largest_bits) >> 10, 30u));
-      float tops[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) tops[e] = fmaxf(fmaxf(x[0][e], x[0][2 + e]), fmaxf(x[1][e], x[1][2 + e]));
+      const uint32_t now = max(exponent, min(__reduce_max_sync(0xffffffffu, largest & 0xffffu) >> 10, 30u));
+      // slots that some row does not see may hold anything: their weights are zero, and so must be their share
+      const bool careful = guard && __any_sync(0xffffffffu, __vcmpgeu2(largest, 0x7c007c00u) != 0u);
+      const float tops[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
       const bool grows = tops[0] > m_run[0] + kSlack || tops[1] > m_run[1] + kSlack;
       if (__any_sync(0xffffffffu, grows) || now != exponent) {
         float alpha[2];
@@ -717,78 +781,62 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i >> 1][i & 1][e] *= alpha[e & 1];
       }
-      // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (+ 16), in units of the value scales
-      float pw[2][4];
-      const float to_units = 23.0f - (float)exponent;
-#pragma unroll
-      for (int side = 0; side < 2; ++side) {
+      // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9, in units of the value scales
+      float pw[4];
+      {
+        const float to_units = 23.0f - (float)exponent;
         float pr[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = power2(fmaf(x[side][e] - m_use[e & 1], kLog2e, to_units));
+        for (int e = 0; e < 4; ++e) pr[e] = power2(fmaf(x[e] - m_use[e & 1], kLog2e, to_units));
         l_run[0] += pr[0] + pr[2];
         l_run[1] += pr[1] + pr[3];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t c0 = __float_as_uint(pr[2 * e]), c1 = __float_as_uint(pr[2 * e + 1]);
           const uint32_t lo = transposed8x8(__byte_perm(c0, c1, 0x5410)), hi = transposed8x8(__byte_perm(c0, c1, 0x7632));
-          pw[side][2 * e] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
-          pw[side][2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+          pw[2 * e] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+          pw[2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
         }
       }
       // -- outputs: channels by slots times slots by rows; a weight is two fp16 numbers --
+      uint32_t high[2], low[2], words[4];
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        uint32_t vp[4][G];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          lds_words(pairs_at + T::kPairBytes + (uint32_t)((16 * side + 2 * t + (j & 1) + 8 * (j >> 1)) * G * 4), vp[j]);
-        if (guard) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) vp[j][gr] = pw[side][j] == 0.0f ? 0u : vp[j][gr];
-        }
-        uint32_t high[G][2], low[G][2];
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
+      for (int i = 0; i < P; ++i) {
+        if (i % kPer == 0) {
+          const int gr = i / kPer;
           float ps[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 f = pair_floats(vp[j][gr]);
-            ps[j] = pw[side][j] * f.x;
-            least_sum[gr] = fmaf(pw[side][j], fmaf(8.0f, f.x, f.y), least_sum[gr]);
+            const uint32_t bits = lds32(pairs_at + T::kPairBytes + (uint32_t)(((2 * t + (j & 1) + 8 * (j >> 1)) * G + gr) * 4));
+            const float2 f = pair_floats(bits);
+            ps[j] = pw[j] * f.x;
+            if (careful && pw[j] == 0.0f) {
+              ps[j] = 0.0f;
+            } else {
+              least_sum[gr] = fmaf(pw[j], fmaf(8.0f, f.x, f.y), least_sum[gr]);
+            }
           }
-          split_halves(ps[0], ps[1], high[gr][0], low[gr][0]);
-          split_halves(ps[2], ps[3], high[gr][1], low[gr][1]);
+          split_halves(ps[0], ps[1], high[0], low[0]);
+          split_halves(ps[2], ps[3], high[1], low[1]);
         }
+        if (i % 2 == 0) load_matrices_transposed(at + T::kNibbleBytes + (matrix_at ^ (uint32_t)(i * 16)), words);
+        uint32_t e[2][4];
 #pragma unroll
-        for (int i = 0; i < P; i += 2) {
-          uint32_t words[4], e[4][4];
-          load_matrices_transposed(at + T::kNibbleBytes + (matrix_at ^ (uint32_t)(i * 16)) + side * 8 * H, words);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t a = j & 1 ? words[j & 2] >> 8 : words[j & 2], c = j & 1 ? words[(j & 2) + 1] >> 8 : words[(j & 2) + 1];
-            e[j][0] = centred_low(a), e[j][1] = centred_high(a), e[j][2] = centred_low(c), e[j][3] = centred_high(c);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int gr = (i + (j >> 1)) / kPer;
-            product(o[i + (j >> 1)][j & 1], e[j][0], e[j][1], e[j][2], e[j][3], high[gr][0], high[gr][1]);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int gr = (i + (j >> 1)) / kPer;
-            product(o[i + (j >> 1)][j & 1], e[j][0], e[j][1], e[j][2], e[j][3], low[gr][0], low[gr][1]);
-          }
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t a = j ? words[2 * (i & 1)] >> 8 : words[2 * (i & 1)], c = j ? words[2 * (i & 1) + 1] >> 8 : words[2 * (i & 1) + 1];
+          e[j][0] = centred.low(a), e[j][1] = centred.high(a), e[j][2] = centred.low(c), e[j][3] = centred.high(c);
         }
+        product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], high[0], high[1]);
+        product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], high[0], high[1]);
+        product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], low[0], low[1]);
+        product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], low[0], low[1]);
       }
     }
     cp_async_wait<0>();
 
-    // -- this pair's state: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
+    // -- the warp's state, as a record: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
     const float from_units = __int_as_float((int)(104 + exponent) << 23);  // 2^(exponent - 23)
-    const int rows = min(8, rw.rows - chunk * 8);
-    float* state = reinterpret_cast<float*>(smem + w * T::kStages * T::kBytes);
+    float* state = reinterpret_cast<float*>(smem + w * T::kWarpBytes);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -804,228 +852,215 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK>::kThreads, 1) kv4_sdpa_kerne
       for (int i = gr * kPer; i < (gr + 1) * kPer; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (2 * t + e < rows)
-            *reinterpret_cast<float4*>(state + (2 * t + e) * T::kRec + i * 32 + g * 4) =
-                make_float4((o[i][0][e] + least[e]) * from_units, (o[i][0][2 + e] + least[e]) * from_units, (o[i][1][e] + least[e]) * from_units,
-                            (o[i][1][2 + e] + least[e]) * from_units);
+          *reinterpret_cast<float4*>(state + (2 * t + e) * T::kRec + i * 32 + g * 4) =
+              make_float4((o[i][0][e] + least[e]) * from_units, (o[i][0][2 + e] + least[e]) * from_units, (o[i][1][e] + least[e]) * from_units,
+                          (o[i][1][2 + e] + least[e]) * from_units);
     }
-    if (g < 2) {
-      s_m[w][2 * t + g] = g ? m_run[1] : m_run[0];
-      s_l[w][2 * t + g] = (g ? l_run[1] : l_run[0]) * from_units;
+    if (g < 2) *reinterpret_cast<float2*>(state + (2 * t + g) * T::kRec + H) = make_float2(g ? m_run[1] : m_run[0], (g ? l_run[1] : l_run[0]) * from_units);
+  } else if (of.pair >= 0 && lane < 8) {  // (no slot)
+    float* state = reinterpret_cast<float*>(smem + w * T::kWarpBytes) + lane * T::kRec;
+    for (int d = 0; d < H; ++d) state[d] = 0.0f;
+    *reinterpret_cast<float2*>(state + H) = make_float2(-CUDART_INF_F, 0.0f);
+  }
+  if (lane == 0) {
+    if (of.pair >= 0 && !cut.own_cta) {
+      const int n = cut.pieces_of(len), cta = cut.owner(of.first);
+      of.count = cut.owner(of.first + n - 1) - cta + 1;
+      of.index = blockIdx.x - cta;
     }
-    if (lane == 0) {
-      s_pair[w] = pair;
-      s_rows[w] = rows;
-    }
+    s_of[w] = of;
   }
 
-  // -- neighbouring warps of one pair: one record, under the first one's piece --
-  __syncthreads();
-  for (int first = 0; first < T::kWarps;) {
-    const int pair = s_pair[first];
-    if (pair < 0) break;  // (pieces are in order: behind a warp without one there is none)
-    int end = first + 1;
-    while (end < T::kWarps && s_pair[end] == pair) ++end;
-    float* rec = p.ws + (size_t)(first_piece + first) * 8 * T::kRec;
-    for (int i = threadIdx.x; i < s_rows[first] * (H / 4); i += T::kThreads) {
+  // -- the states of a CTA's pairs, and then the pairs' records, are added up --
+  // Where record `index` of a pair lies: under its first piece, and under the first piece of every further CTA.
+  auto record = [&](const Whose& o, int index) {
+    return p.ws + kCounterFloats + (size_t)(index == 0 ? o.first : cut.begin((int)blockIdx.x - o.index + index)) * 8 * T::kRec;
+  };
+  // Adds up n records in shared memory, `bytes` apart, to the pair's outputs or to the record at `to`. All threads.
+  auto add_up = [&](const uint8_t* from, int bytes, int n, int pair, float* to_record) {
+    const int in_b = pair - divide(pair, per, inverse_per) * per, kvh = divide(in_b, rw.chunks, inverse_chunks);
+    const int row0 = (in_b - kvh * rw.chunks) * 8, rows = min(8, rw.rows - row0);
+    auto ml = [&](int j, int row) { return *reinterpret_cast<const float2*>(from + j * bytes + (row * T::kRec + H) * 4); };
+    // (a fourth of the records at a time, and records without a weight up to a multiple of four: no code for remainders)
+    if (threadIdx.x < 8 * kFanIn) {
+      const int j = threadIdx.x >> 3, row = threadIdx.x & 7;
+      float top = -CUDART_INF_F;
+#pragma unroll 1
+      for (int i = 0; i < n; i += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, ml(min(i + e, n - 1), row).x);
+      }
+      s_f[j][row] = j < n ? power2((ml(min(j, n - 1), row).x - (top == -CUDART_INF_F ? 0.0f : top)) * kLog2e) : 0.0f;
+      if (j == 0) s_top[row] = top;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < rows * (H / 4); i += T::kThreads) {
       const int row = i / (H / 4), d = i % (H / 4) * 4;
-      float top = -CUDART_INF_F, sum = 0.0f;
+      const float top = s_top[row];
+      float sum = 0.0f;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+      for (int j0 = 0; j0 < n; j0 += 4) {
 #pragma unroll
-      for (int j = 0; j < T::kWarps; ++j)
-        if (j >= first && j < end) top = fmaxf(top, s_m[j][row]);
-      const float use = top == -CUDART_INF_F ? 0.0f : top;
-#pragma unroll
-      for (int j = 0; j < T::kWarps; ++j) {
-        if (j >= first && j < end) {
-          const float f = power2((s_m[j][row] - use) * kLog2e);
-          const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + j * T::kStages * T::kBytes) + row * T::kRec + d);
+        for (int e = 0; e < 4; ++e) {
+          const float f = s_f[j0 + e][row];
+          const uint8_t* at = from + min(j0 + e, n - 1) * bytes + row * T::kRec * 4;
+          const float4 v = *reinterpret_cast<const float4*>(at + d * 4);
+          sum = fmaf(f, *reinterpret_cast<const float*>(at + (H + 1) * 4), sum);
           acc.x = fmaf(f, v.x, acc.x);
           acc.y = fmaf(f, v.y, acc.y);
           acc.z = fmaf(f, v.z, acc.z);
           acc.w = fmaf(f, v.w, acc.w);
-          sum = fmaf(f, s_l[j][row], sum);
         }
       }
-      *reinterpret_cast<float4*>(rec + row * T::kRec + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(rec + row * T::kRec + H) = make_float2(top, sum);
-    }
-    first = end;
-  }
-}
-
-// Merges the records of one query row, H >> part_log2 channels per CTA (the first n t << part_log2 CTAs of a sequence), or
-// adds the weights that 1024 slots of a KV head got to the scores (the others). What it costs are L2 round trips, so the
-// records are requested before their weights are known.
-constexpr int kMergeThreads = 256;
-constexpr int kScoreSlots = 1024;
-
-__device__ __forceinline__ float merge_reduce(float v, bool max, float* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float y = __shfl_xor_sync(0xffffffffu, v, o);
-    v = max ? fmaxf(v, y) : v + y;
-  }
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int i = 1; i < kMergeThreads / 32; ++i) v = max ? fmaxf(v, red[i]) : v + red[i];
-  return v;
-}
-
-template <int H, bool QF32>
-__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa p, const int ctas, const int part_log2, const float* logits_ws) {
-  constexpr int kRec = H + 4, kBatch = 8;
-  constexpr size_t kStride = 8 * (size_t)kRec;
-  extern __shared__ float merge_w[];  // per record a weight, then per record a sum
-  __shared__ float4 s_part[kMergeThreads];
-  __shared__ float s_stat[16];
-  pdl_launch_dependents();
-  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Kv4Rows rw = kv4_rows(p.t, p.n, p.cache.nkv);
-  const int per = p.cache.nkv * rw.chunks;
-  // what does not depend on the kernel before: it has waited for whatever wrote the lengths
-  const Kv4Cut cut = kv4_cut(p, per, ctas, kv4_warps(H), lane);
-  const int length = kv4_length(p, b), pieces = cut.pieces_of(length), below = count_pieces(p, per, cut, lane, b);
-  // Records of a pair: under its first piece, and under the first piece of every further CTA.
-  struct Records {
-    const float* base;  // of piece 0
-    int first, cta, count;
-  };
-  auto records = [&](int in_b) {
-    const int first = below + in_b * pieces;
-    if (pieces == 0) return Records{p.ws, 0, 0, 0};
-    const int cta = cut.owner(first);
-    return Records{p.ws, first, cta, cut.owner(first + pieces - 1) - cta + 1};
-  };
-  auto record_at = [&](const Records& r, int j) { return r.base + (j == 0 ? r.first : cut.begin(r.cta + j)) * kStride; };
-  if ((int)blockIdx.x < (p.n * p.t) << part_log2) {
-    const int row = blockIdx.x >> part_log2, part = blockIdx.x & ((1 << part_log2) - 1);
-    const int i = row / p.n, head = row % p.n, kvh = head / rw.group, r = i * rw.group + head % rw.group;
-    const int quads = (H / 4) >> part_log2, groups = kMergeThreads / quads;
-    const int quad = tid % quads, grp = tid / quads, channel = 4 * (part * quads + quad);
-    const Records rec = records(kvh * rw.chunks + r / 8);
-    const int count = rec.count, in_rec = (r % 8) * kRec;
-    pdl_wait();
-    float4 first[kBatch];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int c = grp + j * groups;
-      first[j] = c < count ? __ldcg(reinterpret_cast<const float4*>(record_at(rec, c) + in_rec + channel)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    float* sums = merge_w + ctas;
-    float top = -CUDART_INF_F, l = 0.0f;
-    for (int c = tid; c < count; c += kMergeThreads) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(record_at(rec, c) + in_rec + H));
-      merge_w[c] = v.x;
-      sums[c] = v.y;
-      top = fmaxf(top, v.x);
-    }
-    top = merge_reduce(top, true, s_stat);
-    top = top == -CUDART_INF_F ? 0.0f : top;
-    for (int c = tid; c < count; c += kMergeThreads) {
-      const float f = exp2f((merge_w[c] - top) * kLog2e);
-      merge_w[c] = f;
-      l += f * sums[c];
-    }
-    l = merge_reduce(l, false, s_stat + 8);  // (its barrier also publishes the weights)
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c0 = grp; c0 < count; c0 += kBatch * groups) {
-      if (c0 > grp) {
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (c0 + j * groups < count) first[j] = __ldcg(reinterpret_cast<const float4*>(record_at(rec, c0 + j * groups) + in_rec + channel));
+      if (to_record) {
+        *reinterpret_cast<float4*>(to_record + row * T::kRec + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(to_record + row * T::kRec + H) = make_float2(top, sum);
+        continue;
       }
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (c0 + j * groups < count) {
-          const float f = merge_w[c0 + j * groups];
-          acc.x = fmaf(f, first[j].x, acc.x);
-          acc.y = fmaf(f, first[j].y, acc.y);
-          acc.z = fmaf(f, first[j].z, acc.z);
-          acc.w = fmaf(f, first[j].w, acc.w);
-        }
+      const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;  // (0: no slot, and zeros)
+      const int i_q = divide(row0 + row, rw.group, inverse_group), head = kvh * rw.group + (row0 + row - i_q * rw.group);
+      const size_t at = (((size_t)divide(pair, per, inverse_per) * p.t + i_q) * p.n + head) * H + d;
+      if constexpr (QF32) {
+        float* o = static_cast<float*>(p.out) + at;
+        o[0] = acc.x * inverse, o[1] = acc.y * inverse, o[2] = acc.z * inverse, o[3] = acc.w * inverse;
+      } else {
+        __half* o = static_cast<__half*>(p.out) + at;
+        o[0] = __float2half_rn(acc.x * inverse), o[1] = __float2half_rn(acc.y * inverse);
+        o[2] = __float2half_rn(acc.z * inverse), o[3] = __float2half_rn(acc.w * inverse);
       }
+      if (stats_ws && d == 0) stats_ws[(size_t)pair * 8 + row] = make_float2(top == -CUDART_INF_F ? 0.0f : top, inverse);
     }
-    s_part[tid] = acc;
     __syncthreads();
-    if (grp > 0) return;
-#pragma unroll 4
-    for (int j = 1; j < groups; ++j) {
-      const float4 v = s_part[j * quads + quad];
-      acc.x += v.x;
-      acc.y += v.y;
-      acc.z += v.z;
-      acc.w += v.w;
-    }
-    if (l == 0.0f) {
-      acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // no slot
-    } else {
-      acc = make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
-    }
-    const size_t at = (((size_t)b * p.t + i) * p.n + head) * H + channel;
-    if constexpr (QF32) {
-      float* o = static_cast<float*>(p.out) + at;
-      o[0] = acc.x, o[1] = acc.y, o[2] = acc.z, o[3] = acc.w;
-    } else {
-      __half* o = static_cast<__half*>(p.out) + at;
-      o[0] = __float2half_rn(acc.x), o[1] = __float2half_rn(acc.y), o[2] = __float2half_rn(acc.z), o[3] = __float2half_rn(acc.w);
-    }
-    return;
+  };
+  // One arrival of `all` at a counter; true for the last, which leaves it zero.
+  int* counters = reinterpret_cast<int*>(p.ws);
+  auto arrive = [&](int* counter, int all) {
+    int before;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    const bool last = before == all - 1;
+    if (last) *counter = 0;
+    return last;
+  };
+  __syncthreads();
+  bool records = false;
+#pragma unroll 1
+  for (int j = 0; j < kWarps;) {
+    const Whose o = s_of[j];
+    if (o.pair < 0) break;  // (pieces are in order: behind a warp without one there is none)
+    int end = j + 1;
+#pragma unroll 1
+    while (end < kWarps && s_of[end].pair == o.pair) ++end;
+    add_up(smem + j * T::kWarpBytes, T::kWarpBytes, end - j, o.pair, o.count == 1 ? nullptr : record(o, o.index));
+    records = records || o.count > 1;
+    j = end;
   }
-  const int ranges = (p.cache.s + kScoreSlots - 1) / kScoreSlots;
-  const int at = blockIdx.x - ((p.n * p.t) << part_log2), kvh = at / ranges, slot0 = at % ranges * kScoreSlots;
+  if (records) {
+    if (threadIdx.x < kWarps) {
+      const int j = threadIdx.x;
+      const Whose o = s_of[j];
+      bool last = false;
+      if (o.pair >= 0 && o.count > 1 && (j == 0 || s_of[j - 1].pair != o.pair)) {
+        const int base = o.index / kFanIn * kFanIn;
+        last = arrive(counters + (base == 0 ? o.first : cut.begin((int)blockIdx.x - o.index + base)), min(kFanIn, o.count - base));
+      }
+      s_last[j] = last ? 1 : 0;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int j = 0; j < kWarps; ++j) {
+      if (!s_last[j]) continue;
+      const Whose o = s_of[j];
+      int base = o.index / kFanIn * kFanIn, stride = 1, n = min(kFanIn, o.count - base);
+#pragma unroll 1
+      while (true) {
+        // records base, base + stride, ...: sixteen at a time
+        const bool more = o.count > kFanIn && stride == 1;  // this is one of several sums: it goes where the first record is
+        const int rest = n - kFanIn;
+        n = min(n, kFanIn);
+#pragma unroll 1
+        for (int e = threadIdx.x; e < n * (2 * T::kRec); e += T::kThreads) {  // 16-byte pieces
+          const int r = e / (2 * T::kRec), piece = e - r * (2 * T::kRec);
+          cp_async16(smem_u32(smem) + e * 16, record(o, base + r * stride) + piece * 4);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncthreads();
+        add_up(smem, 8 * T::kRec * 4, n, o.pair, more ? record(o, base) : rest > 0 ? record(o, base + (n - 1) * stride) : nullptr);
+        if (rest > 0) {  // (over 256 records: the sum so far, where the last one was, is the first of the next sixteen)
+          base += (kFanIn - 1) * stride;
+          n = rest + 1;
+          continue;
+        }
+        if (!more) break;
+        n = (o.count + kFanIn - 1) / kFanIn;
+        if (threadIdx.x == 0) s_last[j] = arrive(counters + kMostPieces + o.first, n) ? 2 : 1;
+        __syncthreads();
+        if (s_last[j] != 2) break;
+        base = 0;
+        stride = kFanIn;
+      }
+    }
+  }
+  // a sequence without a slot is in no piece: its rows are zeros
+  if (!cut.own_cta) {
+#pragma unroll 1
+    for (int e = blockIdx.x; e < p.cache.b; e += gridDim.x) {
+      if (kv4_length(p, e) > 0) continue;
+      const size_t words = (size_t)p.t * p.n * H * (QF32 ? 4 : 2) / 16;
+      uint4* o = static_cast<uint4*>(p.out) + (size_t)e * words;
+#pragma unroll 1
+      for (size_t i = threadIdx.x; i < words; i += T::kThreads) o[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// Adds the weights that 1024 slots of a KV head got to the scores.
+constexpr int kScoreThreads = 256;
+constexpr int kScoreSlots = 1024;
+__global__ void __launch_bounds__(kScoreThreads) kv4_scores_kernel(const Kv4Sdpa p, const float2* stats_ws, const float* logits_ws) {
+  __shared__ float2 s_stat[8];
+  pdl_launch_dependents();
+  const int b = blockIdx.z, kvh = blockIdx.y, slot0 = blockIdx.x * kScoreSlots;
+  const Kv4Rows rw = kv4_rows(p.t, p.n, p.cache.nkv);
+  const size_t pitch = (size_t)tiles_of(p.cache.s) * kSlots * 8;
+  const int length = kv4_length(p, b);  // (the kernel before has waited for whatever wrote it)
+  float* scores = p.scores + ((size_t)b * p.cache.nkv + kvh) * p.cache.s;
   pdl_wait();
   if (slot0 >= length) return;
-  const size_t pitch = (size_t)tiles_of(p.cache.s) * kSlots * 8;
-  float sums[kScoreSlots / kMergeThreads];
+  float sums[kScoreSlots / kScoreThreads];
 #pragma unroll
-  for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) sums[j] = 0.0f;
+  for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) sums[j] = 0.0f;
   for (int c = 0; c < rw.chunks; ++c) {
-    const int in_b = kvh * rw.chunks + c, rows = min(8, rw.rows - 8 * c);
-    const Records rec = records(in_b);
-    const int in_rec = warp * kRec + H;
+    const size_t pair = ((size_t)b * p.cache.nkv + kvh) * rw.chunks + c;
+    const int rows = min(8, rw.rows - 8 * c);
     __syncthreads();
-    if (warp < rows) {
-      float top = -CUDART_INF_F, l = 0.0f;
-      for (int j = lane; j < rec.count; j += 32) top = fmaxf(top, __ldcg(record_at(rec, j) + in_rec));
+    if (threadIdx.x < 8) s_stat[threadIdx.x] = (int)threadIdx.x < rows ? __ldcg(stats_ws + pair * 8 + threadIdx.x) : make_float2(0.0f, 0.0f);
+    const float* logits = logits_ws + pair * pitch;
+    float4 x[kScoreSlots / kScoreThreads][2];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = top == -CUDART_INF_F ? 0.0f : top;
-      for (int j = lane; j < rec.count; j += 32) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(record_at(rec, j) + in_rec));
-        l += exp2f((v.x - top) * kLog2e) * v.y;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      if (lane == 0) {
-        s_stat[warp] = top;
-        s_stat[8 + warp] = l == 0.0f ? 0.0f : 1.0f / l;
-      }
-    } else if (lane == 0) {
-      s_stat[warp] = 0.0f;
-      s_stat[8 + warp] = 0.0f;
+    for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) {
+      const int slot = slot0 + threadIdx.x + j * kScoreThreads;
+      const float4* from = reinterpret_cast<const float4*>(logits + (size_t)slot * 8);
+      x[j][0] = x[j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (slot < length) x[j][0] = __ldcg(from), x[j][1] = __ldcg(from + 1);
     }
     __syncthreads();
-    const float* logits = logits_ws + ((size_t)b * per + in_b) * pitch;
 #pragma unroll
-    for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) {
-      const int slot = slot0 + threadIdx.x + j * kMergeThreads;
-      if (slot < length) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(logits + (size_t)slot * 8)), y = __ldcg(reinterpret_cast<const float4*>(logits + (size_t)slot * 8) + 1);
-        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    for (int e = 0; e < 8; ++e) {
+      const float2 st = s_stat[e];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < rows) sums[j] = fmaf(exp2f((v[e] - s_stat[e]) * kLog2e), s_stat[8 + e], sums[j]);
+      for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) {
+        const float4 y = x[j][e / 4];
+        const float v = e % 4 == 0 ? y.x : e % 4 == 1 ? y.y : e % 4 == 2 ? y.z : y.w;
+        if (e < rows) sums[j] = fmaf(power2((v - st.x) * kLog2e), st.y, sums[j]);
       }
     }
   }
-  float* scores = p.scores + ((size_t)b * p.cache.nkv + kvh) * p.cache.s;
 #pragma unroll
-  for (int j = 0; j < kScoreSlots / kMergeThreads; ++j) {
-    const int slot = slot0 + threadIdx.x + j * kMergeThreads;
+  for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) {
+    const int slot = slot0 + threadIdx.x + j * kScoreThreads;
     if (slot < length) scores[slot] += sums[j];
   }
 }
@@ -1040,16 +1075,18 @@ int kv4_ctas(long long pairs, int s, int h) {
 
 bool kv4_tensor_shape(int b, int t, int n, int nkv, int h, int s) {
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
-  return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX / 2 && pairs <= (1 << 19) && tiles_of(s) < (1 << 22) &&
-         4ll * n * t + (long long)nkv * ((s + kScoreSlots - 1) / kScoreSlots) <= INT32_MAX;
+  return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX / 2 && tiles_of(s) < (1 << 22) &&
+         (long long)kv4_ctas(pairs, s, h) * kv4_warps(h) <= kMostPieces;
 }
 
 template <int H, int BLOCK, bool QF32>
 cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
-  using T = Kv4Tile<H, BLOCK>;
+  using T = Kv4Tile<H, BLOCK, QF32>;
   const long long pairs = (long long)p.cache.b * p.cache.nkv * kv4_rows(p.t, p.n, p.cache.nkv).chunks;
   const int ctas = kv4_ctas(pairs, p.cache.s, H);
-  float* logits = p.scores ? p.ws + kv4_records_floats((long long)ctas * T::kWarps, H) : nullptr;
+  float* behind = p.ws + kCounterFloats + kv4_records_floats((long long)ctas * T::kWarps, H);
+  float2* stats = p.scores ? reinterpret_cast<float2*>(behind) : nullptr;
+  float* logits = p.scores ? behind + 16 * pairs : nullptr;
   static bool done[64] = {false};
   int device = 0;
   cudaGetDevice(&device);
@@ -1059,14 +1096,10 @@ cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     done[device] = true;
   }
-  const cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, logits);
-  if (e != cudaSuccess) return e;
-  const int scores = p.scores ? p.cache.nkv * ((p.cache.s + kScoreSlots - 1) / kScoreSlots) : 0;
-  // few rows are cut by channels too: their records are many
-  int part_log2 = 0;
-  while (part_log2 < 2 && ((long long)p.cache.b * p.n * p.t << part_log2) < device_sm_count()) ++part_log2;
-  return launch_chained(kv4_merge_kernel<H, QF32>, dim3(((p.n * p.t) << part_log2) + scores, p.cache.b), dim3(kMergeThreads),
-                        2 * sizeof(float) * (size_t)ctas, s, p, ctas, part_log2, (const float*)logits);
+  const cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, stats, logits);
+  if (e != cudaSuccess || !p.scores) return e;
+  return launch_chained(kv4_scores_kernel, dim3((p.cache.s + kScoreSlots - 1) / kScoreSlots, p.cache.nkv, p.cache.b), dim3(kScoreThreads), 0, s, p,
+                        (const float2*)stats, (const float*)logits);
 }
 template <int H, int BLOCK>
 cudaError_t launch_tensor_q(const Kv4Sdpa& p, cudaStream_t s) {
@@ -1082,16 +1115,21 @@ cudaError_t launch_tensor_block(const Kv4Sdpa& p, cudaStream_t s) {
 size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int scores) {
   const size_t rows = (size_t)b * t * n;
   const size_t any = 2 * rows + rows * s;  // (also what queries off a 16-byte boundary need)
-  if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return any * sizeof(float);
+  if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return (kCounterFloats + any) * sizeof(float);
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
   const size_t tensor = kv4_records_floats((long long)kv4_ctas(pairs, s, h) * kv4_warps(h), h) +
-                        (scores ? (size_t)pairs * tiles_of(s) * kSlots * 8 : 0);
-  return (any > tensor ? any : tensor) * sizeof(float);
+                        (scores ? 16 * (size_t)pairs + (size_t)pairs * tiles_of(s) * kSlots * 8 : 0);
+  return (kCounterFloats + (any > tensor ? any : tensor)) * sizeof(float);
 }
+size_t kv4_sdpa_counter_bytes() { return kCounterFloats * sizeof(float); }
 
 cudaError_t launch_kv4_sdpa(const Kv4Sdpa& p, cudaStream_t s) {
   const Kv4Cache& c = p.cache;
-  if (!kv4_tensor_shape(c.b, p.t, p.n, c.nkv, c.h, c.s) || (reinterpret_cast<uintptr_t>(p.q) & 15) != 0) return launch_rows(p, s);
+  if (!kv4_tensor_shape(c.b, p.t, p.n, c.nkv, c.h, c.s) || (reinterpret_cast<uintptr_t>(p.q) & 15) != 0) {
+    Kv4Sdpa behind = p;
+    behind.ws += kCounterFloats;
+    return launch_rows(behind, s);
+  }
   return c.h == 256 ? launch_tensor_block<256>(p, s) : c.h == 128 ? launch_tensor_block<128>(p, s) : launch_tensor_block<64>(p, s);
 }
 
