@@ -409,11 +409,9 @@ B200_API int b200_kv4_read(const void* d_k_cache, const void* d_v_cache, const v
  * none) as in b200_sdpa_decode, never negative.
  * d_scores [b, nkv, s_max] f32 (optional): += the softmax weights that each slot got from its KV
  * head's n / nkv * t queries (what b200_kv4_evict ranks by); slots beyond the length are left
- * alone. Any number of query heads per KV head. Workspace: on a 16-byte boundary, for calls on one
- * stream; b200_kv4_sdpa_workspace_init clears the counters at its start once (512 KiB), every call
- * leaves them cleared, whatever its sizes are. */
+ * alone. Any number of query heads per KV head. Workspace: on a 16-byte boundary, no initial
+ * contents. */
 B200_API size_t b200_kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int block, int s_max, int with_scores);
-B200_API int b200_kv4_sdpa_workspace_init(void* d_workspace, void* stream);
 B200_API int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache, const void* d_k_scale,
                            const void* d_v_scale, const int32_t* d_lengths, const float* d_mask, float* d_scores, void* d_out,
                            int b, int t, int n, int nkv, int h, int block, int s_max, int q_dtype, float scale,

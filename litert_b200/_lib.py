@@ -78,7 +78,6 @@ SIGNATURES = {
     "b200_kv4_append": (_i, [_vp, _vp, _i, _ll, _ll, _ll, _ll, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "b200_kv4_read": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "b200_kv4_sdpa_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
-    "b200_kv4_sdpa_workspace_init": (_i, [_vp, _vp]),
     "b200_kv4_sdpa": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _sz,
                            _vp]),
     "b200_kv4_evict": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp,

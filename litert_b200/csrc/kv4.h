@@ -62,7 +62,6 @@ struct Kv4Sdpa {
   float scale, logit_cap;
   float* ws;
 };
-size_t kv4_sdpa_counter_bytes();  // of the workspace's start, zero between calls
 size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int scores);
 cudaError_t launch_kv4_sdpa(const Kv4Sdpa& p, cudaStream_t s);
 

@@ -141,11 +141,6 @@ size_t b200_kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int bl
   return b200::kv4_sdpa_workspace_bytes(b, t, n, nkv, h, s_max, with_scores);
 }
 
-int b200_kv4_sdpa_workspace_init(void* d_workspace, void* stream) {
-  if (!d_workspace || !aligned(d_workspace, 16)) return fail(B200_ERR_INVALID_ARGUMENT, "b200_kv4_sdpa_workspace_init: workspace on a 16-byte boundary needed");
-  return done(cudaMemsetAsync(d_workspace, 0, b200::kv4_sdpa_counter_bytes(), static_cast<cudaStream_t>(stream)), "b200_kv4_sdpa_workspace_init");
-}
-
 int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache, const void* d_k_scale, const void* d_v_scale,
                   const int32_t* d_lengths, const float* d_mask, float* d_scores, void* d_out, int b, int t, int n, int nkv, int h,
                   int block, int s_max, int q_dtype, float scale, float logit_cap, void* d_workspace, size_t workspace_bytes,

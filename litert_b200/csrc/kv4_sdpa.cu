@@ -150,15 +150,18 @@ cudaError_t launch_rows(const Kv4Sdpa& p, cudaStream_t s) {
 // Up to eight query rows of a KV head (query heads x query tokens) are the 8-wide side of mma.m16n8k16; a tile is 16 slots.
 // Every (sequence, KV head, eight rows) pair is cut into pieces of a common greatest length, one per warp. A warp walks
 // through its piece without meeting another one; at the end the warps of a CTA add their states of a common pair to one
-// partial record (un-normalised outputs, maximum, sum). The CTA that finds the others' records of the pair complete (a
-// counter) merges them, sixteen at a time; a pair that lies in one CTA needs no record.
+// partial record (un-normalised outputs, maximum, sum), and a second kernel merges a pair's records. A pair of few tiles
+// belongs to one CTA, which writes the outputs itself.
 //
 // What bounds a launch of a few microseconds is code that runs once: it is fetched, cold, at about eight cycles per
-// instruction, so loops outside the main one are rolled and both merges are the same code.
+// instruction, so loops outside the main one are rolled. Measured with 16 ragged sequences of up to 8192 tokens, 8 heads x
+// 256, replayed: the CTA that completes a pair (a counter) merges it 20.1 us, second kernel 16.1; pieces that run on from one
+// pair to the next (all of one length) 17.5, 4 of them in the warps that had parts of two pairs; such pieces per CTA 19.4; a
+// record for every warp 20.3 (9.8 MB to merge).
 constexpr int kSlots = 16;
 __host__ __device__ inline int tiles_of(int slots) { return (slots + kSlots - 1) / kSlots; }
 
-__host__ __device__ constexpr int kv4_warps(int h) { return h == 256 ? 12 : 16; }
+__host__ __device__ constexpr int kv4_warps(int h) { return h == 256 ? 8 : 16; }
 
 template <int H, int BLOCK, bool QF32>
 struct Kv4Tile {
@@ -173,10 +176,9 @@ struct Kv4Tile {
   static constexpr int kFit = (220 * 1024 / kWarps - kQueryBytes) / kBytes;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kWarpBytes = kQueryBytes + kStages * kBytes;
-  static constexpr int kRecords = 16 * 8 * kRec * 4;  // sixteen records to merge
-  static constexpr int kSmem = (kWarps * kWarpBytes > kRecords ? kWarps * kWarpBytes : kRecords) + 128;
+  static constexpr int kSmem = kWarps * kWarpBytes + 128;
   static_assert(8 * kRec * 4 <= kWarpBytes, "a warp's state fits into its part");
-  static_assert(kBytes % 128 == 0 && kStages >= 2 && kSmem <= 221 * 1024, "layout");
+  static_assert(kBytes % 128 == 0 && kStages >= 3 && kSmem <= 221 * 1024, "layout");
 };
 
 struct Kv4Rows {
@@ -187,12 +189,9 @@ __host__ __device__ inline Kv4Rows kv4_rows(int t, int n, int nkv) {
   return {group, rows, (rows + 7) / 8};
 }
 
-// Workspace: counters (two per piece, zero between calls), then of the tensor-core kernels a record per piece (of which the
-// first of a pair in each CTA is used) and, where scores are wanted, the rows' {maximum, 1 / sum} [pair][8 rows] and the logits
-// [pair][slot (rounded up to a tile)][8 rows].
-constexpr int kMostPieces = 65536;
-constexpr size_t kCounterFloats = 2 * (size_t)kMostPieces;
-constexpr int kFanIn = 16;  // records that one CTA merges in one round trip
+// Workspace of the tensor-core kernels: a record per piece (of which the first of a pair in each CTA is used), then, where
+// scores are wanted, the rows' {maximum, 1 / sum} [pair][8 rows] and the logits [pair][slot (rounded up to a tile)][8 rows].
+constexpr int kFewRecords = 16;
 __host__ __device__ inline size_t kv4_records_floats(long long pieces, int h) { return (size_t)pieces * 8 * (h + 4); }
 
 __device__ __forceinline__ int kv4_length(const Kv4Sdpa& p, int b) {
@@ -249,7 +248,7 @@ __device__ __forceinline__ Kv4Cut kv4_cut(const Kv4Sdpa& p, int per, int ctas, i
   c.size = c.each = c.longer = 1;
   c.inverse = 1.0f;
   if (c.own_cta) return c;
-  if (total <= 4 * kFanIn * pairs * warps) ctas = min(ctas, kFanIn * pairs);
+  if (total <= 4 * kFewRecords * pairs * warps) ctas = min(ctas, kFewRecords * pairs);
   const int room = ctas * warps;
   c.size = max(1, (int)ceilf((float)total * reciprocal((float)room)));
   int n;
@@ -384,6 +383,23 @@ struct Centred {
   __device__ __forceinline__ uint32_t high(uint32_t w) const { return half2_sub(splice(w, kHighNibbles, eighth), 0x54805480u); }  // - 72
 };
 
+// Four channels of a query row's result, from its sums; with the first ones, what the scores need of the row.
+template <int H, bool QF32>
+__device__ __forceinline__ void kv4_output(const Kv4Sdpa& p, float2* stats_ws, int b, int i, int head, int pair, int row, int d, float top, float sum,
+                                           const float4& acc) {
+  const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;  // (0: no slot, and zeros)
+  const size_t at = (((size_t)b * p.t + i) * p.n + head) * H + d;
+  if constexpr (QF32) {
+    float* o = static_cast<float*>(p.out) + at;
+    o[0] = acc.x * inverse, o[1] = acc.y * inverse, o[2] = acc.z * inverse, o[3] = acc.w * inverse;
+  } else {
+    __half* o = static_cast<__half*>(p.out) + at;
+    o[0] = __float2half_rn(acc.x * inverse), o[1] = __float2half_rn(acc.y * inverse);
+    o[2] = __float2half_rn(acc.z * inverse), o[3] = __float2half_rn(acc.w * inverse);
+  }
+  if (stats_ws && d == 0) stats_ws[(size_t)pair * 8 + row] = make_float2(top == -CUDART_INF_F ? 0.0f : top, inverse);
+}
+
 template <int H, int BLOCK, bool QF32>
 __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa_kernel(const Kv4Sdpa p, float2* stats_ws, float* logits_ws) {
   using T = Kv4Tile<H, BLOCK, QF32>;
@@ -393,13 +409,9 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
   constexpr int kWarps = T::kWarps;
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
-  struct Whose {
-    int pair, count, index, first;  // the pair, its records in all, which of them is this CTA's, the pair's first piece
-  };
-  __shared__ Whose s_of[kWarps];     // whose the warps' states are
-  __shared__ float s_f[kFanIn][8];   // their factors in a sum
-  __shared__ float s_top[8];
-  __shared__ int s_last[kWarps];
+  __shared__ int s_pair[kWarps];                       // whose the warps' states are
+  __shared__ float s_m[kWarps][8], s_l[kWarps][8];     // their maxima and sums
+  __shared__ float s_f[kWarps][8];                     // and factors in the sum
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int nkv = p.cache.nkv, s_max = p.cache.s;
   const Kv4Rows rw = kv4_rows(p.t, p.n, nkv);
@@ -421,7 +433,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
   // this warp's piece: seg tiles from `unit` on of pair in_b of sequence b
   const Kv4Cut cut = kv4_cut(p, per, gridDim.x, kWarps, lane);
   int seg = 0, b = 0, in_b = 0, unit = 0, len = cut.len;
-  Whose of{-1, 1, 0, 0};
+  int pair = -1;
   if (cut.own_cta) {
     if ((int)blockIdx.x < p.cache.b * per) {
       b = divide(blockIdx.x, per, inverse_per);
@@ -430,7 +442,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
       const int tiles = tiles_of(len), each = tiles / kWarps, longer = tiles - each * kWarps;
       unit = w * each + min(w, longer);
       seg = each + (w < longer ? 1 : 0);
-      if (w == 0 || seg > 0) of.pair = blockIdx.x;  // (a pair without a slot has zeros to write)
+      if (w == 0 || seg > 0) pair = blockIdx.x;  // (a pair without a slot has zeros to write)
     }
   } else if (w < cut.each + ((int)blockIdx.x < cut.longer ? 1 : 0)) {
     const int piece = cut.begin(blockIdx.x) + w;
@@ -455,8 +467,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
         const int part = rest - in_b * n, tiles = tiles_of(len), each = divide(tiles, n, inverse), longer = tiles - each * n;
         unit = part * each + min(part, longer);
         seg = each + (part < longer ? 1 : 0);
-        of.pair = b * per + in_b;
-        of.first = piece - part;
+        pair = b * per + in_b;
         break;
       }
       base += __shfl_sync(0xffffffffu, upto, 31);
@@ -636,7 +647,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     };
     if (p.mask) ask_masks(unit * kSlots);
     const bool guard = p.mask != nullptr || p.t > 1;
-    float* logits = logits_ws ? logits_ws + (size_t)of.pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
+    float* logits = logits_ws ? logits_ws + (size_t)pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
 
     // outputs: of piece i and its channels 4 g + {0, 1} and 4 g + {2, 3}, rows 2 t and 2 t + 1
     float o[P][2][4], least_sum[G];
@@ -650,20 +661,12 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     uint32_t exponent = 1;  // fp16 exponent field of the largest value scale so far: weights are in units of 2^(exponent - 23)
 
     const Centred centred;
-    uint32_t at = ring;
-    int first = unit * kSlots;
-    const int behind = first + seg * kSlots;
-#pragma unroll 1
-    for (; first < behind; first += kSlots, at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes) {
-      cp_async_wait<T::kStages - 2>();
-      __syncwarp();  // the tile is there, and everybody is done with the one whose place the next request takes
-      request();
+    // The logits of a tile's slots g and g + 8, rows 2 t and 2 t + 1, without factor, cap and mask.
+    auto dot = [&](uint32_t at, float (&x)[4]) {
       const uint32_t pairs_at = at + 2 * T::kNibbleBytes;
-
-      // -- logits of slots g and g + 8, rows 2 t and 2 t + 1 --
       // One product of each chain after the other: a warp waits for a chain's last product before its next.
       constexpr int kAtOnce = P, kChains = kAtOnce / kPer, kApart = kChains < 4 ? 2 : 1;
-      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      x[0] = x[1] = x[2] = x[3] = 0.0f;
 #pragma unroll
       for (int i0 = 0; i0 < P; i0 += kAtOnce) {
         uint32_t words[kAtOnce / 2][4];
@@ -710,6 +713,8 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
           }
         }
       }
+    };
+    auto finish = [&](int first, float (&x)[4]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] *= factor[e & 1];
       if (p.logit_cap > 0.0f) {
@@ -737,6 +742,23 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
         *reinterpret_cast<float2*>(to_ws + 64) = make_float2(x[2], x[3]);
       }
 
+    };
+    // A tile's weights and outputs stand in one block of code with the next tile's products with the queries, so that the
+    // chains of the one fill the waits of the other.
+    uint32_t at = ring;
+    int first = unit * kSlots;
+    const int behind = first + seg * kSlots;
+    float x[4];
+    cp_async_wait<T::kStages - 2>();
+    __syncwarp();
+    dot(at, x);
+    finish(first, x);
+#pragma unroll 1
+    for (; first < behind; first += kSlots) {
+      cp_async_wait<T::kStages - 3>();
+      __syncwarp();  // the next tile is there, and everybody is done with the one before this, whose place the next request takes
+      request();
+      const uint32_t pairs_at = at + 2 * T::kNibbleBytes, next_at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes;
       // -- running maximum and unit; both rarely change --
       // A weight may exceed 1 by e^kSlack: rescaling the outputs at every new maximum would happen in most tiles while a
       // warp has seen few. The largest value scale of the tile: pairs compared as halves.
@@ -798,6 +820,8 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
           pw[2 * e + 1] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
         }
       }
+      float y[4];
+      dot(next_at, y);  // (behind the last tile: of whatever lies there, and not used)
       // -- outputs: channels by slots times slots by rows; a weight is two fp16 numbers --
       uint32_t high[2], low[2], words[4];
 #pragma unroll
@@ -831,6 +855,10 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
         product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], low[0], low[1]);
         product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], low[0], low[1]);
       }
+      at = next_at;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = y[e];
+      if (first + kSlots < behind) finish(first + kSlots, x);
     }
     cp_async_wait<0>();
 
@@ -856,164 +884,148 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
               make_float4((o[i][0][e] + least[e]) * from_units, (o[i][0][2 + e] + least[e]) * from_units, (o[i][1][e] + least[e]) * from_units,
                           (o[i][1][2 + e] + least[e]) * from_units);
     }
-    if (g < 2) *reinterpret_cast<float2*>(state + (2 * t + g) * T::kRec + H) = make_float2(g ? m_run[1] : m_run[0], (g ? l_run[1] : l_run[0]) * from_units);
-  } else if (of.pair >= 0 && lane < 8) {  // (no slot)
-    float* state = reinterpret_cast<float*>(smem + w * T::kWarpBytes) + lane * T::kRec;
-    for (int d = 0; d < H; ++d) state[d] = 0.0f;
-    *reinterpret_cast<float2*>(state + H) = make_float2(-CUDART_INF_F, 0.0f);
-  }
-  if (lane == 0) {
-    if (of.pair >= 0 && !cut.own_cta) {
-      const int n = cut.pieces_of(len), cta = cut.owner(of.first);
-      of.count = cut.owner(of.first + n - 1) - cta + 1;
-      of.index = blockIdx.x - cta;
+    if (g < 2) {
+      s_m[w][2 * t + g] = g ? m_run[1] : m_run[0];
+      s_l[w][2 * t + g] = (g ? l_run[1] : l_run[0]) * from_units;
     }
-    s_of[w] = of;
+  } else if (lane < 8) {  // (no slot)
+    s_m[w][lane] = -CUDART_INF_F;
+    s_l[w][lane] = 0.0f;
   }
+  if (lane == 0) s_pair[w] = pair;
 
-  // -- the states of a CTA's pairs, and then the pairs' records, are added up --
-  // Where record `index` of a pair lies: under its first piece, and under the first piece of every further CTA.
-  auto record = [&](const Whose& o, int index) {
-    return p.ws + kCounterFloats + (size_t)(index == 0 ? o.first : cut.begin((int)blockIdx.x - o.index + index)) * 8 * T::kRec;
-  };
-  // Adds up n records in shared memory, `bytes` apart, to the pair's outputs or to the record at `to`. All threads.
-  auto add_up = [&](const uint8_t* from, int bytes, int n, int pair, float* to_record) {
-    const int in_b = pair - divide(pair, per, inverse_per) * per, kvh = divide(in_b, rw.chunks, inverse_chunks);
-    const int row0 = (in_b - kvh * rw.chunks) * 8, rows = min(8, rw.rows - row0);
-    auto ml = [&](int j, int row) { return *reinterpret_cast<const float2*>(from + j * bytes + (row * T::kRec + H) * 4); };
-    // (a fourth of the records at a time, and records without a weight up to a multiple of four: no code for remainders)
-    if (threadIdx.x < 8 * kFanIn) {
-      const int j = threadIdx.x >> 3, row = threadIdx.x & 7;
-      float top = -CUDART_INF_F;
-#pragma unroll 1
-      for (int i = 0; i < n; i += 4) {
+  // -- the states of a CTA's pairs become records, or outputs --
+  __syncthreads();
+  if (threadIdx.x < 8 * kWarps) {
+    const int j = threadIdx.x >> 3, row = threadIdx.x & 7, mine = s_pair[j];
+    float top = -CUDART_INF_F;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, ml(min(i + e, n - 1), row).x);
-      }
-      s_f[j][row] = j < n ? power2((ml(min(j, n - 1), row).x - (top == -CUDART_INF_F ? 0.0f : top)) * kLog2e) : 0.0f;
-      if (j == 0) s_top[row] = top;
-    }
-    __syncthreads();
+    for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_pair[i] == mine ? s_m[i][row] : -CUDART_INF_F);
+    s_f[j][row] = power2((s_m[j][row] - (top == -CUDART_INF_F ? 0.0f : top)) * kLog2e);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int first = 0; first < kWarps;) {
+    const int mine = s_pair[first];
+    if (mine < 0) break;  // (pieces are in order: behind a warp without one there is none)
+    int end = first + 1;
+#pragma unroll 1
+    while (end < kWarps && s_pair[end] == mine) ++end;
+    const int of_b = divide(mine, per, inverse_per), of_in_b = mine - of_b * per, of_kvh = divide(of_in_b, rw.chunks, inverse_chunks);
+    const int row0 = (of_in_b - of_kvh * rw.chunks) * 8, rows = min(8, rw.rows - row0);
+    float* rec = p.ws + (size_t)(cut.begin(blockIdx.x) + first) * 8 * T::kRec;
 #pragma unroll 1
     for (int i = threadIdx.x; i < rows * (H / 4); i += T::kThreads) {
       const int row = i / (H / 4), d = i % (H / 4) * 4;
-      const float top = s_top[row];
-      float sum = 0.0f;
+      float sum = 0.0f, top = -CUDART_INF_F;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 1
-      for (int j0 = 0; j0 < n; j0 += 4) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f = s_f[j0 + e][row];
-          const uint8_t* at = from + min(j0 + e, n - 1) * bytes + row * T::kRec * 4;
-          const float4 v = *reinterpret_cast<const float4*>(at + d * 4);
-          sum = fmaf(f, *reinterpret_cast<const float*>(at + (H + 1) * 4), sum);
-          acc.x = fmaf(f, v.x, acc.x);
-          acc.y = fmaf(f, v.y, acc.y);
-          acc.z = fmaf(f, v.z, acc.z);
-          acc.w = fmaf(f, v.w, acc.w);
-        }
+      for (int j = 0; j < kWarps; ++j) {
+        const bool here = j >= first && j < end && s_l[j][row] != 0.0f;  // (else there is no state, or nothing in it)
+        const float f = s_f[j][row];
+        const float4 v = *reinterpret_cast<const float4*>(smem + j * T::kWarpBytes + (row * T::kRec + d) * 4);
+        top = fmaxf(top, here ? s_m[j][row] : -CUDART_INF_F);
+        acc.x += here ? f * v.x : 0.0f;
+        acc.y += here ? f * v.y : 0.0f;
+        acc.z += here ? f * v.z : 0.0f;
+        acc.w += here ? f * v.w : 0.0f;
+        sum += here ? f * s_l[j][row] : 0.0f;
       }
-      if (to_record) {
-        *reinterpret_cast<float4*>(to_record + row * T::kRec + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(to_record + row * T::kRec + H) = make_float2(top, sum);
-        continue;
-      }
-      const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;  // (0: no slot, and zeros)
-      const int i_q = divide(row0 + row, rw.group, inverse_group), head = kvh * rw.group + (row0 + row - i_q * rw.group);
-      const size_t at = (((size_t)divide(pair, per, inverse_per) * p.t + i_q) * p.n + head) * H + d;
-      if constexpr (QF32) {
-        float* o = static_cast<float*>(p.out) + at;
-        o[0] = acc.x * inverse, o[1] = acc.y * inverse, o[2] = acc.z * inverse, o[3] = acc.w * inverse;
+      if (!cut.own_cta) {
+        *reinterpret_cast<float4*>(rec + row * T::kRec + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(rec + row * T::kRec + H) = make_float2(top, sum);
       } else {
-        __half* o = static_cast<__half*>(p.out) + at;
-        o[0] = __float2half_rn(acc.x * inverse), o[1] = __float2half_rn(acc.y * inverse);
-        o[2] = __float2half_rn(acc.z * inverse), o[3] = __float2half_rn(acc.w * inverse);
+        const int i_q = divide(row0 + row, rw.group, inverse_group), head = of_kvh * rw.group + (row0 + row - i_q * rw.group);
+        kv4_output<H, QF32>(p, stats_ws, of_b, i_q, head, mine, row, d, top, sum, acc);
       }
-      if (stats_ws && d == 0) stats_ws[(size_t)pair * 8 + row] = make_float2(top == -CUDART_INF_F ? 0.0f : top, inverse);
     }
-    __syncthreads();
-  };
-  // One arrival of `all` at a counter; true for the last, which leaves it zero.
-  int* counters = reinterpret_cast<int*>(p.ws);
-  auto arrive = [&](int* counter, int all) {
-    int before;
-    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
-    const bool last = before == all - 1;
-    if (last) *counter = 0;
-    return last;
-  };
+    first = end;
+  }
+}
+
+// Merges the records of one query row, H >> part_log2 channels per CTA. What it costs are its start and L2 round trips, so
+// there is one for all records up to 32 (64, 128 where the channels are parted), requested before their weights are known.
+constexpr int kMergeThreads = 128;
+template <int H, bool QF32>
+__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa p, const int ctas, const int part_log2, float2* stats_ws) {
+  constexpr int kRec = H + 4, kBatch = H / 16;
+  __shared__ float4 s_part[kMergeThreads];
+  __shared__ float s_sum[kMergeThreads];
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const Kv4Rows rw = kv4_rows(p.t, p.n, p.cache.nkv);
+  const int per = p.cache.nkv * rw.chunks;
+  const int row = blockIdx.x >> part_log2, part = blockIdx.x & ((1 << part_log2) - 1);
+  const int i = row / p.n, head = row - i * p.n, kvh = head / rw.group, r = i * rw.group + head - kvh * rw.group;
+  const int quads = (H / 4) >> part_log2, groups = kMergeThreads / quads;  // powers of two
+  const int quad = tid & (quads - 1), grp = tid / quads, d = 4 * (part * quads + quad);
+  // what does not depend on the kernel before: it has waited for whatever wrote the lengths
+  const Kv4Cut cut = kv4_cut(p, per, ctas, kv4_warps(H), lane);
+  int below = 0, pieces = 0;  // pieces of the sequences before b, and of each pair of b
+#pragma unroll 1
+  for (int j = lane; j < b; j += 32) below += cut.pieces_of(j == lane ? cut.len : kv4_length(p, j)) * per;
+  below = (int)__reduce_add_sync(0xffffffffu, (unsigned)below);
+  pieces = cut.pieces_of(kv4_length(p, b));
+  const int in_b = kvh * rw.chunks + (r >> 3), first = below + in_b * pieces, cta = cut.owner(first);
+  const int count = pieces == 0 ? 0 : cut.owner(first + pieces - 1) - cta + 1;  // under the first piece, and that of every further CTA
+  const float* base = p.ws + (r & 7) * kRec;
+  pdl_launch_dependents();
+  pdl_wait();
+  if (cut.own_cta) return;
+  float sum = 0.0f, top = -CUDART_INF_F;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+  for (int j0 = 0; j0 < count; j0 += kBatch * groups) {
+    float2 ml[kBatch];
+    float4 v[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {  // (all in flight at once; without a weight where there are fewer)
+      const int at = j0 + grp + j * groups, to = min(at, count - 1);
+      const float* rec = base + (size_t)(to == 0 ? first : cut.begin(cta + to)) * (8 * kRec);
+      ml[j] = __ldcg(reinterpret_cast<const float2*>(rec + H));
+      v[j] = __ldcg(reinterpret_cast<const float4*>(rec + d));
+    }
+    float now = top;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) now = fmaxf(now, ml[j].x);
+    const float use = now == -CUDART_INF_F ? 0.0f : now;
+    const float keep = top == -CUDART_INF_F ? 0.0f : power2((top - use) * kLog2e);
+    top = now;
+    acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+    sum *= keep;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const float f = j0 + grp + j * groups < count ? power2((ml[j].x - use) * kLog2e) : 0.0f;
+      acc.x = fmaf(f, v[j].x, acc.x);
+      acc.y = fmaf(f, v[j].y, acc.y);
+      acc.z = fmaf(f, v[j].z, acc.z);
+      acc.w = fmaf(f, v[j].w, acc.w);
+      sum = fmaf(f, ml[j].y, sum);
+    }
+  }
+  // the groups' sums, each under its own maximum
+  __shared__ float s_top[kMergeThreads];
+  s_part[tid] = acc;
+  s_sum[tid] = sum;
+  s_top[tid] = top;
   __syncthreads();
-  bool records = false;
+  if (grp > 0) return;
 #pragma unroll 1
-  for (int j = 0; j < kWarps;) {
-    const Whose o = s_of[j];
-    if (o.pair < 0) break;  // (pieces are in order: behind a warp without one there is none)
-    int end = j + 1;
+  for (int j = 1; j < groups; ++j) top = fmaxf(top, s_top[j * quads + quad]);
+  const float use = top == -CUDART_INF_F ? 0.0f : top;
+  acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  sum = 0.0f;
 #pragma unroll 1
-    while (end < kWarps && s_of[end].pair == o.pair) ++end;
-    add_up(smem + j * T::kWarpBytes, T::kWarpBytes, end - j, o.pair, o.count == 1 ? nullptr : record(o, o.index));
-    records = records || o.count > 1;
-    j = end;
+  for (int j = 0; j < groups; ++j) {
+    const int at = j * quads + quad;
+    const float f = power2((s_top[at] - use) * kLog2e);
+    const float4 v = s_part[at];
+    acc.x = fmaf(f, v.x, acc.x);
+    acc.y = fmaf(f, v.y, acc.y);
+    acc.z = fmaf(f, v.z, acc.z);
+    acc.w = fmaf(f, v.w, acc.w);
+    sum = fmaf(f, s_sum[at], sum);
   }
-  if (records) {
-    if (threadIdx.x < kWarps) {
-      const int j = threadIdx.x;
-      const Whose o = s_of[j];
-      bool last = false;
-      if (o.pair >= 0 && o.count > 1 && (j == 0 || s_of[j - 1].pair != o.pair)) {
-        const int base = o.index / kFanIn * kFanIn;
-        last = arrive(counters + (base == 0 ? o.first : cut.begin((int)blockIdx.x - o.index + base)), min(kFanIn, o.count - base));
-      }
-      s_last[j] = last ? 1 : 0;
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (int j = 0; j < kWarps; ++j) {
-      if (!s_last[j]) continue;
-      const Whose o = s_of[j];
-      int base = o.index / kFanIn * kFanIn, stride = 1, n = min(kFanIn, o.count - base);
-#pragma unroll 1
-      while (true) {
-        // records base, base + stride, ...: sixteen at a time
-        const bool more = o.count > kFanIn && stride == 1;  // this is one of several sums: it goes where the first record is
-        const int rest = n - kFanIn;
-        n = min(n, kFanIn);
-#pragma unroll 1
-        for (int e = threadIdx.x; e < n * (2 * T::kRec); e += T::kThreads) {  // 16-byte pieces
-          const int r = e / (2 * T::kRec), piece = e - r * (2 * T::kRec);
-          cp_async16(smem_u32(smem) + e * 16, record(o, base + r * stride) + piece * 4);
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        __syncthreads();
-        add_up(smem, 8 * T::kRec * 4, n, o.pair, more ? record(o, base) : rest > 0 ? record(o, base + (n - 1) * stride) : nullptr);
-        if (rest > 0) {  // (over 256 records: the sum so far, where the last one was, is the first of the next sixteen)
-          base += (kFanIn - 1) * stride;
-          n = rest + 1;
-          continue;
-        }
-        if (!more) break;
-        n = (o.count + kFanIn - 1) / kFanIn;
-        if (threadIdx.x == 0) s_last[j] = arrive(counters + kMostPieces + o.first, n) ? 2 : 1;
-        __syncthreads();
-        if (s_last[j] != 2) break;
-        base = 0;
-        stride = kFanIn;
-      }
-    }
-  }
-  // a sequence without a slot is in no piece: its rows are zeros
-  if (!cut.own_cta) {
-#pragma unroll 1
-    for (int e = blockIdx.x; e < p.cache.b; e += gridDim.x) {
-      if (kv4_length(p, e) > 0) continue;
-      const size_t words = (size_t)p.t * p.n * H * (QF32 ? 4 : 2) / 16;
-      uint4* o = static_cast<uint4*>(p.out) + (size_t)e * words;
-#pragma unroll 1
-      for (size_t i = threadIdx.x; i < words; i += T::kThreads) o[i] = make_uint4(0, 0, 0, 0);
-    }
-  }
+  kv4_output<H, QF32>(p, stats_ws, b, i, head, b * per + in_b, r & 7, d, top, sum, acc);
 }
 
 // Adds the weights that 1024 slots of a KV head got to the scores.
@@ -1075,8 +1087,7 @@ int kv4_ctas(long long pairs, int s, int h) {
 
 bool kv4_tensor_shape(int b, int t, int n, int nkv, int h, int s) {
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
-  return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX / 2 && tiles_of(s) < (1 << 22) &&
-         (long long)kv4_ctas(pairs, s, h) * kv4_warps(h) <= kMostPieces;
+  return (h == 64 || h == 128 || h == 256) && pairs * tiles_of(s) <= INT32_MAX / 2 && pairs <= (1 << 19) && tiles_of(s) < (1 << 22);
 }
 
 template <int H, int BLOCK, bool QF32>
@@ -1084,7 +1095,7 @@ cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
   using T = Kv4Tile<H, BLOCK, QF32>;
   const long long pairs = (long long)p.cache.b * p.cache.nkv * kv4_rows(p.t, p.n, p.cache.nkv).chunks;
   const int ctas = kv4_ctas(pairs, p.cache.s, H);
-  float* behind = p.ws + kCounterFloats + kv4_records_floats((long long)ctas * T::kWarps, H);
+  float* behind = p.ws + kv4_records_floats((long long)ctas * T::kWarps, H);
   float2* stats = p.scores ? reinterpret_cast<float2*>(behind) : nullptr;
   float* logits = p.scores ? behind + 16 * pairs : nullptr;
   static bool done[64] = {false};
@@ -1096,8 +1107,15 @@ cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     done[device] = true;
   }
-  const cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, stats, logits);
-  if (e != cudaSuccess || !p.scores) return e;
+  cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, stats, logits);
+  if (e != cudaSuccess) return e;
+  if (pairs > ctas || tiles_of(p.cache.s) > 4 * T::kWarps) {  // (else every pair is a CTA's: kv4_cut)
+    int part_log2 = 0;  // few rows are cut by channels too: their records are many
+    while (part_log2 < 2 && ((long long)p.cache.b * p.n * p.t << part_log2) < 2 * device_sm_count()) ++part_log2;
+    e = launch_chained(kv4_merge_kernel<H, QF32>, dim3((p.n * p.t) << part_log2, p.cache.b), dim3(kMergeThreads), 0, s, p, ctas, part_log2, stats);
+    if (e != cudaSuccess) return e;
+  }
+  if (!p.scores) return cudaSuccess;
   return launch_chained(kv4_scores_kernel, dim3((p.cache.s + kScoreSlots - 1) / kScoreSlots, p.cache.nkv, p.cache.b), dim3(kScoreThreads), 0, s, p,
                         (const float2*)stats, (const float*)logits);
 }
@@ -1115,21 +1133,16 @@ cudaError_t launch_tensor_block(const Kv4Sdpa& p, cudaStream_t s) {
 size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int scores) {
   const size_t rows = (size_t)b * t * n;
   const size_t any = 2 * rows + rows * s;  // (also what queries off a 16-byte boundary need)
-  if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return (kCounterFloats + any) * sizeof(float);
+  if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return any * sizeof(float);
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
   const size_t tensor = kv4_records_floats((long long)kv4_ctas(pairs, s, h) * kv4_warps(h), h) +
                         (scores ? 16 * (size_t)pairs + (size_t)pairs * tiles_of(s) * kSlots * 8 : 0);
-  return (kCounterFloats + (any > tensor ? any : tensor)) * sizeof(float);
+  return (any > tensor ? any : tensor) * sizeof(float);
 }
-size_t kv4_sdpa_counter_bytes() { return kCounterFloats * sizeof(float); }
 
 cudaError_t launch_kv4_sdpa(const Kv4Sdpa& p, cudaStream_t s) {
   const Kv4Cache& c = p.cache;
-  if (!kv4_tensor_shape(c.b, p.t, p.n, c.nkv, c.h, c.s) || (reinterpret_cast<uintptr_t>(p.q) & 15) != 0) {
-    Kv4Sdpa behind = p;
-    behind.ws += kCounterFloats;
-    return launch_rows(behind, s);
-  }
+  if (!kv4_tensor_shape(c.b, p.t, p.n, c.nkv, c.h, c.s) || (reinterpret_cast<uintptr_t>(p.q) & 15) != 0) return launch_rows(p, s);
   return c.h == 256 ? launch_tensor_block<256>(p, s) : c.h == 128 ? launch_tensor_block<128>(p, s) : launch_tensor_block<64>(p, s);
 }
 

@@ -48,7 +48,6 @@ class Workspace:
             check(lib.b200_zero_workspace_init(_ptr(self.zero), _stream()))
         self.scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=self.device)
         self.sdpa = None
-        self.kv4 = None  # of the attention over 4-bit caches
 
     def scratch_for(self, m, k):
         need = _lib.load().b200_fc_scratch_bytes(m, k)
@@ -57,17 +56,12 @@ class Workspace:
         return self.scratch
 
     def sdpa_for(self, b, n, nkv, h, s_max):
-        need = _lib.load().b200_sdpa_workspace_bytes(b, n, nkv, h, s_max)
+        return self.sdpa_bytes(_lib.load().b200_sdpa_workspace_bytes(b, n, nkv, h, s_max))
+
+    def sdpa_bytes(self, need):
         if self.sdpa is None or self.sdpa.numel() < need:
             self.sdpa = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self.sdpa
-
-    def kv4_for(self, need):
-        if self.kv4 is None or self.kv4.numel() < need:
-            self.kv4 = torch.empty(need, dtype=torch.uint8, device=self.device)
-            with torch.cuda.device(self.device):
-                _kcheck(_lib.load().b200_kv4_sdpa_workspace_init(_ptr(self.kv4), _stream()))
-        return self.kv4
 
     def check_status(self):
         """Synchronises and raises if a device-side bounded wait ran out."""
@@ -506,11 +500,7 @@ def sdpa_decode_int4(q, k_cache, v_cache, k_scale, v_scale, lengths=None, mask=N
     lib = _lib.load()
     need = lib.b200_kv4_sdpa_workspace_bytes(b, t, n, nkv, h, block, s_max, int(scores is not None))
     with torch.cuda.device(q.device):
-        if ws is None:
-            wsb = torch.empty(need, dtype=torch.uint8, device=q.device)
-            _kcheck(lib.b200_kv4_sdpa_workspace_init(_ptr(wsb), _stream()))
-        else:
-            wsb = ws.kv4_for(need)
+        wsb = torch.empty(need, dtype=torch.uint8, device=q.device) if ws is None else ws.sdpa_bytes(need)
         _kcheck(lib.b200_kv4_sdpa(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(lengths), _ptr(mask),
                                   _ptr(scores), _ptr(out), b, t, n, nkv, h, block, s_max, _DT[q.dtype],
                                   float(scale) if scale else 0.0, float(logit_cap), _ptr(wsb), wsb.numel(), _stream()))
