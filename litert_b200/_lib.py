@@ -160,6 +160,7 @@ class _GeneralPath:
         return None
 
     fc_hybrid = fc_w4 = sdpa_decode = fc_int8
+    kv_append_int4 = kv_read_int4 = sdpa_decode_int4 = kv_evict_int4 = fc_int8
 
 
 def host_ops():

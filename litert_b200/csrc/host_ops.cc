@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -240,11 +241,172 @@ PyObject* sdpa_decode(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   }
 }
 
+// A cache in 4 bits: nibbles uint8 [b, s, nkv, h / 2], pairs f16 [b, s, nkv, h / block, 2], contiguous, on the current device.
+struct Int4Cache {
+  In k, v, ks, vs;
+  int b = 0, s = 0, nkv = 0, h = 0, block = 0;
+  bool ok = false;
+  explicit Int4Cache(PyObject* const* a) : k(a[0], at::kByte), v(a[1], at::kByte), ks(a[2], at::kHalf), vs(a[3], at::kHalf) {
+    if (!k.ok || !v.ok || !ks.ok || !vs.ok || k.t->dim() != 4 || ks.t->dim() != 5 || v.t->sizes() != k.t->sizes() || vs.t->sizes() != ks.t->sizes())
+      return;
+    const auto n = k.t->sizes(), m = ks.t->sizes();
+    if (n[0] != m[0] || n[1] != m[1] || n[2] != m[2] || m[4] != 2 || m[3] == 0 || 2 * n[3] % m[3] != 0) return;
+    if (n[0] > INT32_MAX || n[1] > INT32_MAX || n[2] > INT32_MAX || n[3] > 1 << 20) return;
+    const at::Device d = k.t->device();
+    if (d.index() != c10::cuda::current_device() || v.t->device() != d || ks.t->device() != d || vs.t->device() != d) return;
+    b = (int)n[0], s = (int)n[1], nkv = (int)n[2], h = 2 * (int)n[3], block = h / (int)m[3];
+    ok = true;
+  }
+  bool here(const In& x) const { return x.ok && (!x.t || x.t->device() == k.t->device()); }
+  bool per_sequence(const In& x) const { return here(x) && (!x.t || x.t->numel() == b); }
+};
+
+// Rows [b, t, nkv, h] of a cache, heads and channels contiguous.
+bool rows_of(PyObject* o, const Int4Cache& c, at::ScalarType type, const at::Tensor** out) {
+  if (!THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  *out = &t;
+  return t.is_cuda() && t.device() == c.k.t->device() && t.scalar_type() == type && t.dim() == 4 && t.size(0) == c.b && t.size(2) == c.nkv &&
+         t.size(3) == c.h && t.size(1) <= INT32_MAX && t.stride(3) == 1 && (c.nkv == 1 || t.stride(2) == c.h);
+}
+
+bool float_type(PyObject* o, at::ScalarType* type) {
+  if (!THPVariable_CheckExact(o)) return false;
+  *type = THPVariable_Unpack(o).scalar_type();
+  return *type == at::kHalf || *type == at::kFloat;
+}
+int float_code(at::ScalarType t) { return t == at::kHalf ? B200_DTYPE_F16 : B200_DTYPE_F32; }
+
+// (k, v, positions, k_cache, v_cache, k_scale, v_scale, counts)
+PyObject* kv_append_int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  if (nargs != 8) Py_RETURN_NONE;
+  try {
+    const Int4Cache c(a + 3);
+    at::ScalarType type;
+    const at::Tensor *k, *v;
+    if (!c.ok || !float_type(a[0], &type) || !rows_of(a[0], c, type, &k) || !rows_of(a[1], c, type, &v) || v->size(1) != k->size(1)) Py_RETURN_NONE;
+    In positions(a[2], at::kInt), counts(a[7], at::kInt, true);
+    if (!c.per_sequence(positions) || !c.per_sequence(counts)) Py_RETURN_NONE;
+    void* s = stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_kv4_append(k->data_ptr(), v->data_ptr(), float_code(type), k->stride(0), k->stride(1), v->stride(0), v->stride(1),
+                         positions.ptr<int32_t>(), counts.ptr<int32_t>(), c.b, (int)k->size(1), c.nkv, c.h, c.block, c.s, c.k.ptr<void>(),
+                         c.v.ptr<void>(), c.ks.ptr<void>(), c.vs.ptr<void>(), s);
+    Py_END_ALLOW_THREADS
+    if (rc != B200_OK) Py_RETURN_NONE;
+    Py_RETURN_TRUE;
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// (k_cache, v_cache, k_scale, v_scale, tokens, positions, counts, half)
+PyObject* kv_read_int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  if (nargs != 8) Py_RETURN_NONE;
+  try {
+    const Int4Cache c(a);
+    int tokens = c.s;
+    In positions(a[5], at::kInt, true), counts(a[6], at::kInt, true);
+    if (!c.ok || (a[4] != Py_None && !as_int(a[4], &tokens)) || tokens < 0 || !c.per_sequence(positions) || !c.per_sequence(counts)) Py_RETURN_NONE;
+    const at::ScalarType type = a[7] == Py_True ? at::kHalf : at::kFloat;
+    const std::array<int64_t, 4> shape{c.b, tokens, c.nkv, c.h};
+    at::Tensor k(at::detail::empty_cuda(shape, type, c.k.t->device(), std::nullopt)), v(at::detail::empty_cuda(shape, type, c.k.t->device(), std::nullopt));
+    void* s = stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_kv4_read(c.k.ptr<void>(), c.v.ptr<void>(), c.ks.ptr<void>(), c.vs.ptr<void>(), c.b, c.s, c.nkv, c.h, c.block,
+                       positions.ptr<int32_t>(), counts.ptr<int32_t>(), tokens, float_code(type), k.data_ptr(), v.data_ptr(), s);
+    Py_END_ALLOW_THREADS
+    if (rc != B200_OK) Py_RETURN_NONE;
+    PyObject* ko = THPVariable_Wrap(std::move(k));
+    PyObject* vo = THPVariable_Wrap(std::move(v));
+    PyObject* both = ko && vo ? PyTuple_Pack(2, ko, vo) : nullptr;
+    Py_XDECREF(ko);
+    Py_XDECREF(vo);
+    return both;
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// (q, k_cache, v_cache, k_scale, v_scale, lengths, mask, scale, logit_cap, scores, ws)
+PyObject* sdpa_decode_int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  if (nargs != 11 || a[10] == Py_None || a[8] == Py_None) Py_RETURN_NONE;
+  try {
+    const Int4Cache c(a + 1);
+    at::ScalarType type;
+    if (!c.ok || !float_type(a[0], &type)) Py_RETURN_NONE;
+    Attr ws_o(a[10], s_sdpa);
+    In q(a[0], type), lengths(a[5], at::kInt, true), mask(a[6], at::kFloat, true), scores(a[9], at::kFloat, true), ws(ws_o.o, at::kByte);
+    float scale, cap;
+    if (!c.here(q) || !c.per_sequence(lengths) || !c.here(mask) || !c.here(scores) || !c.here(ws) || !as_float(a[7], &scale) || !as_float(a[8], &cap) ||
+        q.t->dim() != 4 || q.t->size(0) != c.b || q.t->size(3) != c.h || q.t->numel() == 0 || q.t->size(1) > 65535 || q.t->size(2) > 1 << 20)
+      Py_RETURN_NONE;
+    const int t = (int)q.t->size(1), n = (int)q.t->size(2);
+    if (n % c.nkv != 0 || (mask.t && mask.t->sizes() != at::IntArrayRef{c.b, 1, t, c.s}) ||
+        (scores.t && scores.t->sizes() != at::IntArrayRef{c.b, c.nkv, c.s}))
+      Py_RETURN_NONE;
+    if ((size_t)ws.t->numel() < b200_kv4_sdpa_workspace_bytes(c.b, t, n, c.nkv, c.h, c.block, c.s, scores.t ? 1 : 0)) Py_RETURN_NONE;
+    at::Tensor y = result(Py_None, q.t->sizes(), type, *q.t);
+    void* s = stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_kv4_sdpa(q.ptr<void>(), c.k.ptr<void>(), c.v.ptr<void>(), c.ks.ptr<void>(), c.vs.ptr<void>(), lengths.ptr<int32_t>(),
+                       mask.ptr<float>(), scores.ptr<float>(), y.data_ptr(), c.b, t, n, c.nkv, c.h, c.block, c.s, float_code(type), scale, cap,
+                       ws.ptr<void>(), (size_t)ws.t->numel(), s);
+    Py_END_ALLOW_THREADS
+    return give(Py_None, std::move(y), rc);
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// (k_cache, v_cache, k_scale, v_scale, scores, lengths, budget, sinks, recent, into: None or a tuple of four tensors)
+PyObject* kv_evict_int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  if (nargs != 10 || (a[9] != Py_None && (!PyTuple_CheckExact(a[9]) || PyTuple_GET_SIZE(a[9]) != 4))) Py_RETURN_NONE;
+  try {
+    const Int4Cache c(a);
+    PyObject* into[4] = {a[0], a[1], a[2], a[3]};
+    if (a[9] != Py_None)
+      for (int i = 0; i < 4; ++i) into[i] = PyTuple_GET_ITEM(a[9], i);
+    const Int4Cache to(into);
+    In scores(a[4], at::kFloat), lengths(a[5], at::kInt);
+    int budget, sinks, recent;
+    if (!c.ok || !to.ok || to.b != c.b || to.nkv != c.nkv || to.h != c.h || to.block != c.block || !c.here(scores) || !c.per_sequence(lengths) ||
+        scores.t->sizes() != at::IntArrayRef{c.b, c.nkv, c.s} || !as_int(a[6], &budget) || !as_int(a[7], &sinks) || !as_int(a[8], &recent) || budget <= 0)
+      Py_RETURN_NONE;
+    const at::Device d = c.k.t->device();
+    at::Tensor kept(at::detail::empty_cuda(std::array<int64_t, 3>{c.b, c.nkv, budget}, at::kInt, d, std::nullopt)),
+        new_scores(at::detail::empty_cuda(std::array<int64_t, 3>{c.b, c.nkv, to.s}, at::kFloat, d, std::nullopt)),
+        new_lengths(at::detail::empty_cuda(std::array<int64_t, 1>{c.b}, at::kInt, d, std::nullopt));
+    void* s = stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_kv4_evict(c.k.ptr<void>(), c.v.ptr<void>(), c.ks.ptr<void>(), c.vs.ptr<void>(), c.b, c.s, c.nkv, c.h, c.block, scores.ptr<float>(),
+                        lengths.ptr<int32_t>(), budget, sinks, recent, to.k.ptr<void>(), to.v.ptr<void>(), to.ks.ptr<void>(), to.vs.ptr<void>(),
+                        to.s, static_cast<int32_t*>(kept.data_ptr()), static_cast<float*>(new_scores.data_ptr()),
+                        static_cast<int32_t*>(new_lengths.data_ptr()), s);
+    Py_END_ALLOW_THREADS
+    if (rc != B200_OK) Py_RETURN_NONE;
+    PyObject* o[3] = {THPVariable_Wrap(std::move(kept)), THPVariable_Wrap(std::move(new_scores)), THPVariable_Wrap(std::move(new_lengths))};
+    PyObject* all = o[0] && o[1] && o[2] ? PyTuple_Pack(3, o[0], o[1], o[2]) : nullptr;
+    for (PyObject* x : o) Py_XDECREF(x);
+    return all;
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
 PyMethodDef kMethods[] = {
     {"fc_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fc_int8)), METH_FASTCALL, nullptr},
     {"fc_hybrid", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fc_hybrid)), METH_FASTCALL, nullptr},
     {"fc_w4", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fc_w4)), METH_FASTCALL, nullptr},
     {"sdpa_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(sdpa_decode)), METH_FASTCALL, nullptr},
+    {"kv_append_int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(kv_append_int4)), METH_FASTCALL, nullptr},
+    {"kv_read_int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(kv_read_int4)), METH_FASTCALL, nullptr},
+    {"sdpa_decode_int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(sdpa_decode_int4)), METH_FASTCALL, nullptr},
+    {"kv_evict_int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(kv_evict_int4)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

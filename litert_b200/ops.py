@@ -435,6 +435,8 @@ def kv_append_int4(k, v, positions, k_cache, v_cache, k_scale, v_scale, counts=N
     """Quantizes k and v [b, t, nkv, h] (float16 or float32; slices of a fused projection are read where they lie) and
     stores token i of sequence b in slot positions[b] + i of the cache. Slots outside the cache and tokens
     i >= counts[b] (a padded batch) are left alone."""
+    if _host.kv_append_int4(k, v, positions, k_cache, v_cache, k_scale, v_scale, counts) is not None:
+        return
     b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
     if k.dtype not in (torch.float16, torch.float32):
         raise B200Error("kv_append_int4 takes float16 or float32 rows")
@@ -460,9 +462,12 @@ def kv_read_int4(k_cache, v_cache, k_scale, v_scale, tokens=None, positions=None
     """The values of slots positions[b] (default 0) .. + tokens - 1 (default: the cache's length) as two tensors
     [b, tokens, nkv, h]: what a prompt chunk's attention (sdpa_rows) reads. Slots outside the cache and rows
     i >= counts[b] are zeros."""
-    b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
     if dtype not in (torch.float16, torch.float32):
         raise B200Error("kv_read_int4 gives float16 or float32 rows")
+    rows = _host.kv_read_int4(k_cache, v_cache, k_scale, v_scale, tokens, positions, counts, dtype == torch.float16)
+    if rows is not None:
+        return rows
+    b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
     tokens = s_max if tokens is None else int(tokens)
     if tokens < 0:
         raise B200Error("tokens must not be negative")
@@ -482,6 +487,9 @@ def sdpa_decode_int4(q, k_cache, v_cache, k_scale, v_scale, lengths=None, mask=N
     attends over all of these but the last t - 1 - i. mask float32 [b, 1, t, s_max] is added; -inf hides a slot whatever
     it holds. scores float32 [b, nkv, s_max], where given, grows by the softmax weights that every slot got from the
     queries of its KV head (kv_evict_int4 ranks by it)."""
+    y = _host.sdpa_decode_int4(q, k_cache, v_cache, k_scale, v_scale, lengths, mask, scale, logit_cap, scores, ws)
+    if y is not None:
+        return y
     b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
     if q.dtype not in (torch.float16, torch.float32) or not q.is_cuda or q.device != k_cache.device:
         raise B200Error("q must be float16 or float32, on the cache's device")
@@ -513,8 +521,12 @@ def kv_evict_int4(k_cache, v_cache, k_scale, v_scale, scores, lengths, budget, s
     order, to the first slots of the cache itself, or of the cache `into` (the four tensors of another one with at least
     `budget` slots). Returns (kept int32 [b, nkv, budget], -1 behind the last; scores [b, nkv, slots of the
     destination], zeros behind; lengths int32 [b]): what the next steps go on with."""
+    into = None if into is None else tuple(into)
+    done = _host.kv_evict_int4(k_cache, v_cache, k_scale, v_scale, scores, lengths, budget, sinks, recent, into)
+    if done is not None:
+        return done
     b, s_max, nkv, h, block = _int4_cache(k_cache, v_cache, k_scale, v_scale)
-    to = (k_cache, v_cache, k_scale, v_scale) if into is None else tuple(into)
+    to = (k_cache, v_cache, k_scale, v_scale) if into is None else into
     if len(to) != 4:
         raise B200Error("into must be the four tensors of a cache")
     b_to, s_to, nkv_to, h_to, block_to = _int4_cache(*to)
