@@ -68,8 +68,8 @@ int b200_kv4_append(const void* d_k, const void* d_v, int dtype, long long k_bat
   if (!d_k || !d_v || !d_positions) return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
   if (!aligned(d_k, dtype == B200_DTYPE_F32 ? 4 : 2) || !aligned(d_v, dtype == B200_DTYPE_F32 ? 4 : 2))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: keys and values lie on boundaries of their elements", name);
-  if ((long long)b * t * nkv * (h / 8) > (long long)INT32_MAX * 256ll)
-    return fail(B200_ERR_UNSUPPORTED, "%s: too many tokens for one call", name);
+  if ((long long)t * nkv * (h / 8) > INT32_MAX - 1024)
+    return fail(B200_ERR_UNSUPPORTED, "%s: too many tokens of a sequence for one call", name);
   b200::Kv4Append p;
   p.cache = cache_of(d_k_cache, d_v_cache, d_k_scale, d_v_scale, b, s_max, nkv, h, block);
   p.k = d_k, p.v = d_v;
@@ -89,8 +89,8 @@ int b200_kv4_read(const void* d_k_cache, const void* d_v_cache, const void* d_k_
   if (b == 0 || t == 0) return B200_OK;
   if (!d_k || !d_v) return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
   if (!aligned(d_k, 16) || !aligned(d_v, 16)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: outputs lie on 16-byte boundaries", name);
-  if ((long long)b * t * nkv * (h / 8) > (long long)INT32_MAX * 256ll)
-    return fail(B200_ERR_UNSUPPORTED, "%s: too many tokens for one call", name);
+  if ((long long)t * nkv * (h / 8) > INT32_MAX - 1024)
+    return fail(B200_ERR_UNSUPPORTED, "%s: too many tokens of a sequence for one call", name);
   b200::Kv4Read p;
   p.cache = cache_of(const_cast<void*>(d_k_cache), const_cast<void*>(d_v_cache), const_cast<void*>(d_k_scale),
                      const_cast<void*>(d_v_scale), b, s_max, nkv, h, block);

@@ -15,134 +15,207 @@ namespace cg = cooperative_groups;
 
 constexpr int kRowThreads = 256;
 
+// n / d for n below 2^31: a product and a shift, the factor made on the host.
+struct Divisor {
+  uint32_t d, factor, shift;
+};
+Divisor divisor(uint32_t d) {
+  uint32_t bits = 0;
+  while ((1ull << bits) < d) ++bits;
+  return {d, (uint32_t)(((1ull << (31 + bits)) + d - 1) / d), 31 + bits};
+}
+__device__ __forceinline__ uint32_t operator/(uint32_t n, const Divisor& by) { return (uint32_t)(((uint64_t)n * by.factor) >> by.shift); }
+
 // ---- storing ---------------------------------------------------------------------------------------------
 // Per block of channels: least = fp16(min), scale = fp16((max - least) / 15) with difference and quotient rounded to
 // fp32, u = the integer nearest to (x - least) / scale (ties to even), clamped to 0 .. 15. Both roundings to fp16 happen
 // before the nibbles are chosen, so that these are the best ones for the pair that is kept.
-// Which integer is nearest is decided exactly: the fp32 quotient is off by 15 * 3 * 2^-24 at most, so only quotients that
-// near to a border are looked at again, in 64 bits where difference and border are exact.
-__device__ __forceinline__ uint32_t nearest_nibble(float x, float least, float scale, float inverse) {
-  const float f = (x - least) * inverse;
-  const float below = floorf(f);
-  float u = rintf(f);
-  if (fabsf(f - below - 0.5f) < 1e-5f) {
-    const double d = (double)x - (double)least, border = ((double)below + 0.5) * (double)scale;
-    u = d > border ? below + 1.0f : d < border ? below : u;
-    if (d == border) u = 2.0f * rintf(0.5f * (below + 0.5f));  // the even neighbour
-  }
-  return (uint32_t)fminf(fmaxf(u, 0.0f), 15.0f);
+// Which integer is nearest is decided exactly: y = (x - least) / (15 scale), clamped for free by the product's saturation,
+// is off by 2^-22 of itself at most, so 15 y by 3.6e-6; only what comes within 1e-5 of a border is looked at again, in 64
+// bits where difference and border are exact.
+//
+// Memory-bound by its bytes, and nearly by instruction issue: 67 M elements at 36 T lane operations per second leave 12
+// operations for each in the time that HBM takes. So 16 channels per thread (block / 16 neighbouring lanes have one block),
+// the minimum and the negated maximum of fp16 rows as one pair of halves, nibbles put together by fused products.
+__device__ __forceinline__ float nearest_float(float n, float x, float least, float scale) {
+  const double d = (double)x - (double)least;
+  const float below = n * scale > (float)d ? n - 1.0f : n;  // the border lies above it
+  const double border = ((double)below + 0.5) * (double)scale;
+  const float u = d > border ? below + 1.0f : d < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));  // (ties: the even neighbour)
+  return fminf(fmaxf(u, 0.0f), 15.0f);
+}
+__device__ __forceinline__ float min_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
 }
 
-// A thread takes 8 channels (one word of nibbles), block / 8 neighbouring lanes one block. Memory-bound.
 template <bool F32>
-__global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append p, const long long items, const int vec) {
+__global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append p, const uint32_t items, const Divisor per_token, const int lanes_log2,
+                                                                 const int vec) {
   pdl_enter();
-  const long long item = (long long)blockIdx.x * kRowThreads + threadIdx.x;
-  const int words = p.cache.h / 8, lanes = p.cache.block / 8;
-  const bool is_v = blockIdx.y != 0;
+  const uint32_t item = blockIdx.x * kRowThreads + threadIdx.x;  // of a sequence's (token, 16 channels)
+  const int b = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
   bool live = item < items;
-  long long row = live ? item / words : 0;  // (sequence, token, head)
-  const int word = live ? (int)(item % words) : 0;
-  const int kvh = (int)(row % p.cache.nkv);
-  row /= p.cache.nkv;
-  const int i = (int)(row % p.t), b = (int)(row / p.t);
+  const uint32_t i = live ? item / per_token : 0, rest = live ? item - i * per_token.d : 0;
   const long long slot = (long long)p.positions[b] + i;
-  live = live && slot >= 0 && slot < p.cache.s && (!p.counts || i < p.counts[b]);
-  float x[8];
-  if (live) {
-    const long long at = (is_v ? b * p.v_batch + i * p.v_token : b * p.k_batch + i * p.k_token) + (long long)kvh * p.cache.h + 8 * word;
-    if constexpr (F32) {
-      const float* src = static_cast<const float*>(is_v ? p.v : p.k) + at;
-      if (vec) {
-        const float4 lo = __ldg(reinterpret_cast<const float4*>(src)), hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
-        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-      } else {
+  live = live && slot >= 0 && slot < p.cache.s && (!p.counts || (int)i < p.counts[b]);  // (alike for the lanes of a block)
+  float x[16];
+  float lo, hi;
+  const long long at = (is_v ? b * p.v_batch + i * p.v_token : b * p.k_batch + i * p.k_token) + (long long)rest * 16;
+  if constexpr (F32) {
+    const float* src = static_cast<const float*>(is_v ? p.v : p.k) + at;
+    if (!live) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __ldg(src + e);
+      for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+    } else if (vec) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(src) + e);
+        x[4 * e] = v.x, x[4 * e + 1] = v.y, x[4 * e + 2] = v.z, x[4 * e + 3] = v.w;
       }
     } else {
-      const __half* src = static_cast<const __half*>(is_v ? p.v : p.k) + at;
-      if (vec) {
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(src));
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-          x[2 * e] = f.x, x[2 * e + 1] = f.y;
-        }
-      } else {
+      for (int e = 0; e < 16; ++e) x[e] = __ldg(src + e);
+    }
+    lo = hi = x[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __half2float(src[e]);
-      }
+    for (int e = 1; e < 16; ++e) {
+      lo = min_nan(lo, x[e]);
+      hi = max_nan(hi, x[e]);
+    }
+    for (int o = 1; o < 1 << lanes_log2; o <<= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
   } else {
+    const __half* src = static_cast<const __half*>(is_v ? p.v : p.k) + at;
+    uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (!live) {
+    } else if (vec) {
+      const uint4 r0 = __ldg(reinterpret_cast<const uint4*>(src)), r1 = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+      w[0] = r0.x, w[1] = r0.y, w[2] = r0.z, w[3] = r0.w, w[4] = r1.x, w[5] = r1.y, w[6] = r1.z, w[7] = r1.w;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-  }
-  float lo = x[0], hi = x[0], bad = 0.0f;  // bad: NaN once any element is infinite or NaN
+      for (int e = 0; e < 8; ++e) {
+        const __half2 v = __halves2half2(src[2 * e], src[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+    __half2 least2 = *reinterpret_cast<const __half2*>(&w[0]), most2 = least2;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = fminf(lo, x[e]);
-    hi = fmaxf(hi, x[e]);
-    bad = fmaf(0.0f, x[e], bad);
+    for (int e = 1; e < 8; ++e) {
+      least2 = __hmin2_nan(least2, *reinterpret_cast<const __half2*>(&w[e]));
+      most2 = __hmax2_nan(most2, *reinterpret_cast<const __half2*>(&w[e]));
+    }
+    // (minimum, -maximum)
+    __half2 both = __halves2half2(__hmin_nan(__low2half(least2), __high2half(least2)), __hneg(__hmax_nan(__low2half(most2), __high2half(most2))));
+    for (int o = 1; o < 1 << lanes_log2; o <<= 1) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&both), o);
+      both = __hmin2_nan(both, *reinterpret_cast<const __half2*>(&other));
+    }
+    lo = __low2float(both);
+    hi = -__high2float(both);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      x[2 * e] = f.x, x[2 * e + 1] = f.y;
+    }
   }
-  for (int o = 1; o < lanes; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad += __shfl_xor_sync(0xffffffffu, bad, o);
-  }
+  const bool bad = !(fabsf(lo) < CUDART_INF_F && fabsf(hi) < CUDART_INF_F);  // an infinity or NaN is not hidden: the block reads back as NaN
   __half least_h = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
   const float least = __half2float(least_h);
   __half scale_h = __float2half_rn(fminf(fmaxf(__fdiv_rn(__fsub_rn(hi, least), 15.0f), 0.0f), 65504.0f));
   const float scale = __half2float(scale_h);
-  uint32_t bits = 0;
-  if (bad != bad) {  // an infinity or NaN is not hidden: the block reads back as NaN
+  uint32_t word[2] = {0, 0};
+  if (bad) {
     least_h = scale_h = __ushort_as_half(0x7fff);
   } else if (scale > 0.0f) {
-    const float inverse = 1.0f / scale;
+    const float inverse = __fdividef(1.0f, 15.0f * scale);
+    float n[16], far = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) bits |= nearest_nibble(x[e], least, scale, inverse) << (4 * e);
+    for (int e = 0; e < 16; ++e) {
+      const float y = __saturatef((x[e] - least) * inverse);
+      n[e] = fmaf(y, 15.0f, 12582912.0f) - 12582912.0f;  // rounded by the sum's last place
+      far = fmaxf(far, fabsf(fmaf(y, 15.0f, -n[e])));
+    }
+    if (far > 0.49999f) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) n[e] = nearest_float(n[e], x[e], least, scale);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float* m = n + 8 * e;
+      // (sums below 2^16, exact; a number added to 2^23 is its low bits)
+      const float low = fmaf(fmaf(m[3], 16.0f, m[2]), 256.0f, fmaf(m[1], 16.0f, m[0])) + 8388608.0f;
+      const float high = fmaf(fmaf(m[7], 16.0f, m[6]), 256.0f, fmaf(m[5], 16.0f, m[4])) + 8388608.0f;
+      word[e] = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+    }
   }
   if (!live) return;
-  const size_t to = ((size_t)b * p.cache.s + (size_t)slot) * p.cache.nkv + kvh;
-  reinterpret_cast<uint32_t*>(is_v ? p.cache.v : p.cache.k)[to * words + word] = bits;
-  if (word % lanes == 0) (is_v ? p.cache.v_pairs : p.cache.k_pairs)[to * (p.cache.h / p.cache.block) + word / lanes] = __halves2half2(scale_h, least_h);
+  const size_t to = ((size_t)b * p.cache.s + (size_t)slot) * per_token.d + rest;
+  *reinterpret_cast<uint2*>((is_v ? p.cache.v : p.cache.k) + to * 8) = make_uint2(word[0], word[1]);
+  if ((rest & ((1u << lanes_log2) - 1)) == 0) (is_v ? p.cache.v_pairs : p.cache.k_pairs)[to >> lanes_log2] = __halves2half2(scale_h, least_h);
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------
+// A thread takes two words of nibbles, 256 apart, so that a warp's stores are whole lines. fp16 values are fused products
+// of halves: one rounding.
 template <bool F32>
-__global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Read p, const long long items) {
+__global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Read p, const uint32_t items, const Divisor per_token, const int words_log2) {
   pdl_enter();
-  const long long item = (long long)blockIdx.x * kRowThreads + threadIdx.x;
-  if (item >= items) return;
-  const int words = p.cache.h / 8, lanes = p.cache.block / 8;
-  const bool is_v = blockIdx.y != 0;
-  long long row = item / words;
-  const int word = (int)(item % words), kvh = (int)(row % p.cache.nkv);
-  row /= p.cache.nkv;
-  const int i = (int)(row % p.t), b = (int)(row / p.t);
-  const long long slot = (p.positions ? (long long)p.positions[b] : 0) + i;
-  const bool there = slot >= 0 && slot < p.cache.s && (!p.counts || i < p.counts[b]);
-  float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  if (there) {
-    const size_t from = ((size_t)b * p.cache.s + (size_t)slot) * p.cache.nkv + kvh;
-    const uint32_t bits = __ldg(reinterpret_cast<const uint32_t*>(is_v ? p.cache.v : p.cache.k) + from * words + word);
-    const float2 sm = __half22float2(__ldg((is_v ? p.cache.v_pairs : p.cache.k_pairs) + from * (p.cache.h / p.cache.block) + word / lanes));
+  const int b = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  const uint32_t* nibbles = reinterpret_cast<const uint32_t*>(is_v ? p.cache.v : p.cache.k);
+  const __half2* pairs = is_v ? p.cache.v_pairs : p.cache.k_pairs;
+  const long long position = p.positions ? (long long)p.positions[b] : 0;
+  const int count = p.counts ? p.counts[b] : p.t;
+  uint32_t w[2];
+  __half2 pair[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((bits >> (4 * e)) & 15u), sm.x, sm.y);
-  }
-  if constexpr (F32) {
-    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(is_v ? p.v : p.k) + item * 8);
-    dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-    dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const __half2 h = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-      w[e] = *reinterpret_cast<const uint32_t*>(&h);
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t item = blockIdx.x * (2 * kRowThreads) + e * kRowThreads + threadIdx.x;
+    const uint32_t i = item / per_token, rest = item - i * per_token.d;
+    const long long slot = position + i;
+    w[e] = 0;
+    pair[e] = __float2half2_rn(0.0f);
+    if (item < items && slot >= 0 && slot < p.cache.s && (int)i < count) {
+      const size_t from = ((size_t)b * p.cache.s + (size_t)slot) * per_token.d + rest;
+      w[e] = __ldg(nibbles + from);
+      pair[e] = __ldg(pairs + (from >> words_log2));
     }
-    *reinterpret_cast<uint4*>(static_cast<__half*>(is_v ? p.v : p.k) + item * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t item = blockIdx.x * (2 * kRowThreads) + e * kRowThreads + threadIdx.x;
+    if (item >= items) return;
+    const size_t to = ((size_t)b * items + item) * 8;
+    if constexpr (F32) {
+      const float2 sm = __half22float2(pair[e]);
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = fmaf(__uint_as_float(((w[e] >> (4 * k)) & 15u) | 0x4b000000u) - 8388608.0f, sm.x, sm.y);
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(is_v ? p.v : p.k) + to);
+      dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+      dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      const __half2 s2 = __low2half2(pair[e]), m2 = __high2half2(pair[e]), bias = __float2half2_rn(1024.0f);
+      uint32_t v[4];  // nibbles k and k + 4
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t bits = ((w[e] >> (4 * k)) & 0x000f000fu) | 0x64006400u;
+        const __half2 y = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&bits), bias), s2, m2);
+        v[k] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+      *reinterpret_cast<uint4*>(static_cast<__half*>(is_v ? p.v : p.k) + to) =
+          make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
+    }
   }
 }
 
@@ -173,7 +246,7 @@ struct EvictShared {
 // In place, rows move down (slot kept[j] >= j), so a pass of the cluster reads the rows of as many destinations as fit
 // into its CTAs' shared memory, waits for the cluster, and writes them: what it overwrites has been read in this pass or
 // an earlier one.
-__global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Evict p, const int in_place) {
+__global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Evict p, const int in_place, const int row_log2) {
   extern __shared__ __align__(16) uint8_t rows_smem[];
   __shared__ EvictShared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -318,66 +391,86 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Ev
   __threadfence();
   cluster.sync();  // the list is complete; no CTA's shared memory is read any more
   // ---- rows ----
+  // A row's 16-byte pieces of nibbles and its 4-byte pairs lie side by side over 2^row_log2 lanes (row_log2 may be 6: two
+  // turns of a warp); a thread asks for eight before it puts down the first.
   const int nibbles = p.from.h / 2, groups = p.from.h / p.from.block;
   const int row_bytes = 2 * nibbles + 8 * groups, row_pad = (row_bytes + 15) / 16 * 16;
-  const int chunks = nibbles / 16, parts = 2 * chunks + 2 * groups;  // 16-byte pieces of nibbles, then 4-byte pairs
+  const int chunks = nibbles / 16, parts = 2 * chunks + 2 * groups;
+  const int part = tid & ((1 << row_log2) - 1), row_of = tid >> row_log2, rows_at_once = kEvictThreads >> row_log2;
+  const bool is_pair = part >= 2 * chunks, is_v = is_pair ? part - 2 * chunks >= groups : part >= chunks;
+  const int within = is_pair ? (part - 2 * chunks) % groups * 4 : part % chunks * 16, pitch = is_pair ? 4 * groups : nibbles;
+  const uint8_t* from = is_pair ? reinterpret_cast<const uint8_t*>(is_v ? p.from.v_pairs : p.from.k_pairs) : is_v ? p.from.v : p.from.k;
+  uint8_t* to = is_pair ? reinterpret_cast<uint8_t*>(is_v ? p.to.v_pairs : p.to.k_pairs) : is_v ? p.to.v : p.to.k;
+  const size_t from_step = (size_t)p.from.nkv * pitch, to_step = (size_t)p.to.nkv * pitch;
+  from += ((size_t)b * p.from.s * p.from.nkv + kvh) * pitch + within;
+  to += ((size_t)b * p.to.s * p.to.nkv + kvh) * pitch + within;
+  uint8_t* mine = rows_smem + (is_pair ? 2 * nibbles + (part - 2 * chunks) * 4 : part * 16);
   const int fit = kEvictRowSmem / row_pad;
+  const bool live = part < parts;
+  constexpr int kAtOnce = 8;
   for (int j0 = in_place ? p.sinks : 0; j0 < left; j0 += ctas * fit) {
     const int r0 = j0 + rank * fit, rows = max(0, min(fit, left - r0));
-    for (int e = tid; e < rows * parts; e += kEvictThreads) {
-      const int r = e / parts, part = e % parts;
-      const size_t at = ((size_t)b * p.from.s + (size_t)__ldcg(kept + r0 + r)) * p.from.nkv + kvh;
-      uint8_t* dst = rows_smem + (size_t)r * row_pad;
-      if (part < 2 * chunks) {
-        const uint8_t* src = (part < chunks ? p.from.k : p.from.v) + at * nibbles + (part % chunks) * 16;
-        *reinterpret_cast<uint4*>(dst + part * 16) = __ldcg(reinterpret_cast<const uint4*>(src));
-      } else {
-        const int g = part - 2 * chunks;
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(g < groups ? p.from.k_pairs : p.from.v_pairs) + at * groups + g % groups;
-        *reinterpret_cast<uint32_t*>(dst + 2 * nibbles + 4 * g) = __ldcg(src);
+    for (int r = row_of; r < rows; r += kAtOnce * rows_at_once) {
+      int slot[kAtOnce];
+      uint4 v[kAtOnce];
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) slot[e] = r + e * rows_at_once < rows ? __ldcg(kept + r0 + r + e * rows_at_once) : -1;
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) {
+        if (!live || slot[e] < 0) continue;
+        const uint8_t* at = from + slot[e] * from_step;
+        if (is_pair) {
+          v[e].x = __ldcg(reinterpret_cast<const uint32_t*>(at));
+        } else {
+          v[e] = __ldcg(reinterpret_cast<const uint4*>(at));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) {
+        if (!live || slot[e] < 0) continue;
+        // (out of place a row goes straight on)
+        uint8_t* at = in_place ? mine + (size_t)(r + e * rows_at_once) * row_pad : to + (size_t)(r0 + r + e * rows_at_once) * to_step;
+        if (is_pair) {
+          *reinterpret_cast<uint32_t*>(at) = v[e].x;
+        } else {
+          *reinterpret_cast<uint4*>(at) = v[e];
+        }
       }
     }
-    if (in_place) {
-      cluster.sync();
-    } else {
-      __syncthreads();
-    }
-    for (int e = tid; e < rows * parts; e += kEvictThreads) {
-      const int r = e / parts, part = e % parts;
-      const size_t at = ((size_t)b * p.to.s + (size_t)(r0 + r)) * p.to.nkv + kvh;
-      const uint8_t* src = rows_smem + (size_t)r * row_pad;
-      if (part < 2 * chunks) {
-        uint8_t* dst = (part < chunks ? p.to.k : p.to.v) + at * nibbles + (part % chunks) * 16;
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + part * 16);
+    if (!in_place) continue;
+    cluster.sync();  // every row of this pass has been read
+    for (int r = row_of; r < rows && live; r += rows_at_once) {
+      const uint8_t* src = mine + (size_t)r * row_pad;
+      uint8_t* at = to + (size_t)(r0 + r) * to_step;
+      if (is_pair) {
+        *reinterpret_cast<uint32_t*>(at) = *reinterpret_cast<const uint32_t*>(src);
       } else {
-        const int g = part - 2 * chunks;
-        reinterpret_cast<uint32_t*>(g < groups ? p.to.k_pairs : p.to.v_pairs)[at * groups + g % groups] =
-            *reinterpret_cast<const uint32_t*>(src + 2 * nibbles + 4 * g);
+        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(src);
       }
     }
-    __syncthreads();
+    // (a thread's own pieces of the shared memory: no barrier before the next pass)
   }
 }
 
 }  // namespace
 
 cudaError_t launch_kv4_append(const Kv4Append& p, cudaStream_t s) {
-  const long long items = (long long)p.cache.b * p.t * p.cache.nkv * (p.cache.h / 8);
-  if (items == 0) return cudaSuccess;
+  const uint32_t per_token = (uint32_t)p.cache.nkv * (p.cache.h / 16), items = (uint32_t)p.t * per_token;
   const int elem = p.f32 ? 4 : 2, per = 16 / elem;  // elements of a 16-byte load
   const bool vec = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0 &&
                    p.k_batch % per == 0 && p.k_token % per == 0 && p.v_batch % per == 0 && p.v_token % per == 0;
-  const dim3 grid((unsigned)((items + kRowThreads - 1) / kRowThreads), 2);
-  return p.f32 ? launch_chained(kv4_append_kernel<true>, grid, dim3(kRowThreads), 0, s, p, items, vec ? 1 : 0)
-               : launch_chained(kv4_append_kernel<false>, grid, dim3(kRowThreads), 0, s, p, items, vec ? 1 : 0);
+  const dim3 grid((items + kRowThreads - 1) / kRowThreads, p.cache.b, 2);
+  const int lanes_log2 = p.cache.block == 64 ? 2 : 1;
+  return p.f32 ? launch_chained(kv4_append_kernel<true>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), lanes_log2, vec ? 1 : 0)
+               : launch_chained(kv4_append_kernel<false>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), lanes_log2, vec ? 1 : 0);
 }
 
 cudaError_t launch_kv4_read(const Kv4Read& p, cudaStream_t s) {
-  const long long items = (long long)p.cache.b * p.t * p.cache.nkv * (p.cache.h / 8);
-  if (items == 0) return cudaSuccess;
-  const dim3 grid((unsigned)((items + kRowThreads - 1) / kRowThreads), 2);
-  return p.f32 ? launch_chained(kv4_read_kernel<true>, grid, dim3(kRowThreads), 0, s, p, items)
-               : launch_chained(kv4_read_kernel<false>, grid, dim3(kRowThreads), 0, s, p, items);
+  const uint32_t per_token = (uint32_t)p.cache.nkv * (p.cache.h / 8), items = (uint32_t)p.t * per_token;
+  const dim3 grid((items + 2 * kRowThreads - 1) / (2 * kRowThreads), p.cache.b, 2);
+  const int words_log2 = p.cache.block == 64 ? 3 : 2;
+  return p.f32 ? launch_chained(kv4_read_kernel<true>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), words_log2)
+               : launch_chained(kv4_read_kernel<false>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), words_log2);
 }
 
 cudaError_t launch_kv4_evict(const Kv4Evict& p, cudaStream_t s) {
@@ -392,10 +485,13 @@ cudaError_t launch_kv4_evict(const Kv4Evict& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     done[dev] = true;
   }
+  const int parts = 2 * (p.from.h / 32) + 2 * (p.from.h / p.from.block);
+  int row_log2 = 0;
+  while ((1 << row_log2) < parts) ++row_log2;
   int ctas = 8;
   while (ctas > 1 && (long long)pairs * ctas > 2ll * device_sm_count()) ctas /= 2;
   return launch_chained_cluster(kv4_evict_kernel, dim3((unsigned)(pairs * ctas)), dim3(kEvictThreads), (size_t)kEvictRowSmem, ctas, s, p,
-                                p.from.k == p.to.k ? 1 : 0);
+                                p.from.k == p.to.k ? 1 : 0, row_log2);
 }
 
 }  // namespace b200
