@@ -229,24 +229,28 @@ __device__ __forceinline__ uint32_t score_key(float score) {
 
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
-constexpr int kEvictRowSmem = 160 * 1024;  // rows on their way
+constexpr int kEvictSmem = 104 * 1024, kEvictMostSmem = 216 * 1024;  // rows on their way; before that two histograms
+constexpr int kDigitBits = 11, kDigits = 1 << kDigitBits, kPerThread = kDigits / kEvictThreads;
+constexpr int kWholeSlots = 8192;
 
 struct EvictShared {
-  uint32_t hist[2][256];
   uint32_t digit, above;       // the digit that the threshold has, and how many keys lie above it
   uint32_t more, equal;        // this CTA's keys above / at the threshold
   uint32_t scan[2][kEvictWarps];
 };
 
 // One cluster per (sequence, KV head): its CTAs share the slots between them. The slots that neither the first `sinks`
-// nor the last `recent` protect are ranked by a radix selection, 8 bits of the key a time: every CTA counts its slots'
-// digits, the cluster adds the counts through distributed shared memory, and after four rounds the threshold and the
-// number of slots at the threshold that stay (the lowest) are known. The kept slots' list is made by a scan in slot
-// order.
+// nor the last `recent` protect are ranked by a radix selection, 11 bits of the key a time (the first digit is sign,
+// exponent and two bits more: scores of one order of magnitude do not all count in one word): every CTA counts its slots'
+// digits, adds the cluster's counts of a share of the digits through distributed shared memory and hands the sums round,
+// and after three rounds the threshold and the number of slots at the threshold that stay (the lowest) are known. (All
+// digits' counts read from all CTAs by everybody: 20 us a round.) Up to 8192 slots every CTA counts all of them instead:
+// they stay in its L1, and no round waits for the cluster. The kept slots' list is made by a scan in slot order.
 // In place, rows move down (slot kept[j] >= j), so a pass of the cluster reads the rows of as many destinations as fit
 // into its CTAs' shared memory, waits for the cluster, and writes them: what it overwrites has been read in this pass or
 // an earlier one.
-__global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Evict p, const int in_place, const int row_log2) {
+// Bound by round trips: (MEASURED)
+__global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Evict p, const int in_place, const int row_log2, const int smem_bytes) {
   extern __shared__ __align__(16) uint8_t rows_smem[];
   __shared__ EvictShared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -281,50 +285,68 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Ev
   const int wanted = choose ? p.budget - p.sinks - p.recent : 0;
   if (wanted > 0) {  // (uniform over the cluster)
     const int n = behind - first, share = (n + ctas - 1) / ctas;
-    const int begin = first + min(n, rank * share), end = first + min(n, (rank + 1) * share);
+    const int begin = first + min(n, rank * share), end = first + min(n, (rank + 1) * share);  // this CTA's slots
+    const bool whole = n <= kWholeSlots || ctas == 1;
+    const int count_begin = whole ? first : begin, count_end = whole ? behind : end;
     uint32_t prefix = 0, to_find = (uint32_t)wanted;  // the threshold is the to_find-th largest of the keys with this prefix
-    for (int round = 0; round < 4; ++round) {
-      const int shift = 24 - 8 * round;
-      uint32_t* hist = sh.hist[round & 1];
-      for (int i = tid; i < 256; i += kEvictThreads) hist[i] = 0;
+    int shift = 32;
+#pragma unroll 1
+    for (int round = 0; round < 3; ++round) {
+      const int above = shift;
+      shift = max(0, shift - kDigitBits);
+      const uint32_t mask = (1u << (above - shift)) - 1u;
+      uint32_t *hist = reinterpret_cast<uint32_t*>(rows_smem), *sums = hist + kDigits;
+      for (int i = tid; i < kDigits; i += kEvictThreads) hist[i] = 0;
       __syncthreads();
-      for (int i = begin + tid; i < end; i += kEvictThreads) {
+      for (int i = count_begin + tid; i < count_end; i += kEvictThreads) {
         const uint32_t key = score_key(__ldg(scores + i));
-        if (round == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+        if (round == 0 || (key ^ prefix) >> above == 0) atomicAdd(&hist[(key >> shift) & mask], 1u);
       }
-      cluster.sync();
-      if (warp == 0) {
-        // lane l holds the digits 255 - 8 l .. 248 - 8 l: counts from the largest digit down
-        uint32_t mine[8], sum = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          mine[e] = 0;
-          for (int c = 0; c < ctas; ++c) mine[e] += cluster.map_shared_rank(hist, c)[255 - 8 * lane - e];
-          sum += mine[e];
+      if (whole) {
+        __syncthreads();
+        sums = hist;
+      } else {
+        cluster.sync();
+        const int slice = kDigits / ctas;
+        for (int i = rank * slice + tid; i < (rank + 1) * slice; i += kEvictThreads) {
+          uint32_t all = 0;
+          for (int c = 0; c < ctas; ++c) all += cluster.map_shared_rank(hist, c)[i];
+          for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(sums, c)[i] = all;
         }
-        uint32_t upto = sum;
+        cluster.sync();
+      }
+      // thread t holds the digits 2047 - 4 t .. 2044 - 4 t: counts from the largest digit down
+      uint32_t mine[kPerThread], sum = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += y;
-        }
-        uint32_t above = upto - sum;
+      for (int e = 0; e < kPerThread; ++e) mine[e] = sums[kDigits - 1 - kPerThread * tid - e];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (above < to_find && to_find <= above + mine[e]) {
-            sh.digit = 255u - 8u * lane - e;
-            sh.above = above;
-          }
-          above += mine[e];
+      for (int e = 0; e < kPerThread; ++e) sum += mine[e];
+      uint32_t upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      if (lane == 31) sh.scan[0][warp] = upto;
+      __syncthreads();
+      uint32_t greater = upto - sum;
+#pragma unroll
+      for (int w = 0; w < kEvictWarps; ++w) greater += w < warp ? sh.scan[0][w] : 0u;
+#pragma unroll
+      for (int e = 0; e < kPerThread; ++e) {
+        if (greater < to_find && to_find <= greater + mine[e]) {
+          sh.digit = (uint32_t)(kDigits - 1 - kPerThread * tid - e);
+          sh.above = greater;
         }
+        greater += mine[e];
       }
       __syncthreads();
       prefix |= sh.digit << shift;
       to_find -= sh.above;
     }
-    // slots above and at the threshold, here and in the CTAs before
+    // slots above and at the threshold: this CTA's (whole: those in front of its own)
     uint32_t more = 0, equal = 0;
-    for (int i = begin + tid; i < end; i += kEvictThreads) {
+    for (int i = (whole ? first : begin) + tid; i < (whole ? begin : end); i += kEvictThreads) {
       const uint32_t key = score_key(__ldg(scores + i));
       more += key > prefix;
       equal += key == prefix;
@@ -336,25 +358,28 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Ev
       sh.scan[1][warp] = equal;
     }
     __syncthreads();
-    if (tid == 0) {
-      more = equal = 0;
-      for (int w = 0; w < kEvictWarps; ++w) {
-        more += sh.scan[0][w];
-        equal += sh.scan[1][w];
-      }
-      sh.more = more;
-      sh.equal = equal;
+    more = equal = 0;
+#pragma unroll
+    for (int w = 0; w < kEvictWarps; ++w) {
+      more += sh.scan[0][w];
+      equal += sh.scan[1][w];
     }
-    cluster.sync();
-    uint32_t more_before = 0, equal_before = 0;
-    for (int c = 0; c < rank; ++c) {
-      const EvictShared* other = cluster.map_shared_rank(&sh, c);
-      more_before += other->more;
-      equal_before += other->equal;
+    if (!whole) {
+      if (tid == 0) {
+        sh.more = more;
+        sh.equal = equal;
+      }
+      cluster.sync();
+      more = equal = 0;
+      for (int c = 0; c < rank; ++c) {
+        const EvictShared* other = cluster.map_shared_rank(&sh, c);
+        more += other->more;
+        equal += other->equal;
+      }
     }
     // (of the equal ones the first to_find stay)
-    uint32_t taken = (uint32_t)first + more_before + min(equal_before, to_find);
-    uint32_t equals = equal_before;
+    uint32_t taken = (uint32_t)first + more + min(equal, to_find);
+    uint32_t equals = equal;
     for (int i0 = begin; i0 < end; i0 += kEvictThreads) {
       const int i = i0 + tid;
       const float score = i < end ? __ldg(scores + i) : 0.0f;
@@ -392,7 +417,7 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Ev
   cluster.sync();  // the list is complete; no CTA's shared memory is read any more
   // ---- rows ----
   // A row's 16-byte pieces of nibbles and its 4-byte pairs lie side by side over 2^row_log2 lanes (row_log2 may be 6: two
-  // turns of a warp); a thread asks for eight before it puts down the first.
+  // turns of a warp); all of a pass are asked for before the first is put down.
   const int nibbles = p.from.h / 2, groups = p.from.h / p.from.block;
   const int row_bytes = 2 * nibbles + 8 * groups, row_pad = (row_bytes + 15) / 16 * 16;
   const int chunks = nibbles / 16, parts = 2 * chunks + 2 * groups;
@@ -404,43 +429,30 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Ev
   const size_t from_step = (size_t)p.from.nkv * pitch, to_step = (size_t)p.to.nkv * pitch;
   from += ((size_t)b * p.from.s * p.from.nkv + kvh) * pitch + within;
   to += ((size_t)b * p.to.s * p.to.nkv + kvh) * pitch + within;
-  uint8_t* mine = rows_smem + (is_pair ? 2 * nibbles + (part - 2 * chunks) * 4 : part * 16);
-  const int fit = kEvictRowSmem / row_pad;
+  const int fit = smem_bytes / (row_pad + 4);  // rows, and their slots
+  int32_t* slots = reinterpret_cast<int32_t*>(rows_smem + (size_t)fit * row_pad);
+  const uint32_t mine = smem_u32(rows_smem) + (uint32_t)(is_pair ? 2 * nibbles + (part - 2 * chunks) * 4 : part * 16);
   const bool live = part < parts;
-  constexpr int kAtOnce = 8;
   for (int j0 = in_place ? p.sinks : 0; j0 < left; j0 += ctas * fit) {
     const int r0 = j0 + rank * fit, rows = max(0, min(fit, left - r0));
-    for (int r = row_of; r < rows; r += kAtOnce * rows_at_once) {
-      int slot[kAtOnce];
-      uint4 v[kAtOnce];
-#pragma unroll
-      for (int e = 0; e < kAtOnce; ++e) slot[e] = r + e * rows_at_once < rows ? __ldcg(kept + r0 + r + e * rows_at_once) : -1;
-#pragma unroll
-      for (int e = 0; e < kAtOnce; ++e) {
-        if (!live || slot[e] < 0) continue;
-        const uint8_t* at = from + slot[e] * from_step;
+    __syncthreads();  // (the slots of the pass before have been used)
+    for (int r = tid; r < rows; r += kEvictThreads) slots[r] = __ldcg(kept + r0 + r);
+    __syncthreads();
+    if (live) {
+      for (int r = row_of; r < rows; r += rows_at_once) {
+        const uint8_t* src = from + slots[r] * from_step;
+        const uint32_t dst = mine + (uint32_t)(r * row_pad);
         if (is_pair) {
-          v[e].x = __ldcg(reinterpret_cast<const uint32_t*>(at));
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
         } else {
-          v[e] = __ldcg(reinterpret_cast<const uint4*>(at));
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < kAtOnce; ++e) {
-        if (!live || slot[e] < 0) continue;
-        // (out of place a row goes straight on)
-        uint8_t* at = in_place ? mine + (size_t)(r + e * rows_at_once) * row_pad : to + (size_t)(r0 + r + e * rows_at_once) * to_step;
-        if (is_pair) {
-          *reinterpret_cast<uint32_t*>(at) = v[e].x;
-        } else {
-          *reinterpret_cast<uint4*>(at) = v[e];
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
         }
       }
     }
-    if (!in_place) continue;
-    cluster.sync();  // every row of this pass has been read
+    asm volatile("cp.async.wait_all;" ::: "memory");  // (a thread puts down what it asked for)
+    if (in_place) cluster.sync();                      // every row of this pass has been read
     for (int r = row_of; r < rows && live; r += rows_at_once) {
-      const uint8_t* src = mine + (size_t)r * row_pad;
+      const uint8_t* src = rows_smem + (mine - smem_u32(rows_smem)) + (size_t)r * row_pad;
       uint8_t* at = to + (size_t)(r0 + r) * to_step;
       if (is_pair) {
         *reinterpret_cast<uint32_t*>(at) = *reinterpret_cast<const uint32_t*>(src);
@@ -448,7 +460,6 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv4_evict_kernel(const Kv4Ev
         *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(src);
       }
     }
-    // (a thread's own pieces of the shared memory: no barrier before the next pass)
   }
 }
 
@@ -473,25 +484,45 @@ cudaError_t launch_kv4_read(const Kv4Read& p, cudaStream_t s) {
                : launch_chained(kv4_read_kernel<false>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), words_log2);
 }
 
+// Clusters of eight CTAs with an SM each that fit on the current device at once.
+static int evict_clusters_alone() {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(8);
+  cfg.blockDim = dim3(kEvictThreads);
+  cfg.dynamicSmemBytes = kEvictMostSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 8, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, kv4_evict_kernel, &cfg) == cudaSuccess ? n : 0;
+}
+
 cudaError_t launch_kv4_evict(const Kv4Evict& p, cudaStream_t s) {
   const int pairs = p.from.b * p.from.nkv;
   if (pairs == 0) return cudaSuccess;
   static bool done[64] = {false};
+  static int alone[64];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
   if (!done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictRowSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictMostSmem);
     if (e != cudaSuccess) return e;
+    alone[dev] = evict_clusters_alone();
     done[dev] = true;
   }
   const int parts = 2 * (p.from.h / 32) + 2 * (p.from.h / p.from.block);
   int row_log2 = 0;
   while ((1 << row_log2) < parts) ++row_log2;
+  const bool in_place = p.from.k == p.to.k;
   int ctas = 8;
-  while (ctas > 1 && (long long)pairs * ctas > 2ll * device_sm_count()) ctas /= 2;
-  return launch_chained_cluster(kv4_evict_kernel, dim3((unsigned)(pairs * ctas)), dim3(kEvictThreads), (size_t)kEvictRowSmem, ctas, s, p,
-                                p.from.k == p.to.k ? 1 : 0, row_log2);
+  while (ctas > 1 && (long long)pairs * ctas > device_sm_count()) ctas /= 2;
+  // a whole SM for each CTA, where the clusters find them: two on one SM share its way to memory while others idle
+  const int smem = ctas == 8 && pairs <= alone[dev] ? kEvictMostSmem : kEvictSmem;
+  return launch_chained_cluster(kv4_evict_kernel, dim3((unsigned)(pairs * ctas)), dim3(kEvictThreads), (size_t)smem, ctas, s, p, in_place ? 1 : 0,
+                                row_log2, smem);
 }
 
 }  // namespace b200
