@@ -288,6 +288,10 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Ev
     const int begin = first + min(n, rank * share), end = first + min(n, (rank + 1) * share);  // this CTA's slots
     const bool whole = n <= kWholeSlots || ctas == 1;
     const int count_begin = whole ? first : begin, count_end = whole ? behind : end;
+    // the first count leaves the keys in shared memory for the others, where they fit
+    uint32_t* keys = reinterpret_cast<uint32_t*>(rows_smem) + 2 * kDigits;
+    const bool keep = 4 * (long long)(count_end - count_begin) + 8 * kDigits <= smem_bytes;
+    auto key_of = [&](int i) { return keep ? keys[i - count_begin] : score_key(__ldg(scores + i)); };
     uint32_t prefix = 0, to_find = (uint32_t)wanted;  // the threshold is the to_find-th largest of the keys with this prefix
     int shift = 32;
 #pragma unroll 1
@@ -298,17 +302,27 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Ev
       uint32_t *hist = reinterpret_cast<uint32_t*>(rows_smem), *sums = hist + kDigits;
       for (int i = tid; i < kDigits; i += kEvictThreads) hist[i] = 0;
       __syncthreads();
-      for (int i = count_begin + tid; i < count_end; i += kEvictThreads) {
-        const uint32_t key = score_key(__ldg(scores + i));
-        if (round == 0 || (key ^ prefix) >> above == 0) atomicAdd(&hist[(key >> shift) & mask], 1u);
+      if (round == 0) {
+#pragma unroll 4
+        for (int i = count_begin + tid; i < count_end; i += kEvictThreads) {
+          const uint32_t key = score_key(__ldg(scores + i));
+          if (keep) keys[i - count_begin] = key;
+          atomicAdd(&hist[key >> shift], 1u);
+        }
+      } else {
+#pragma unroll 4
+        for (int i = count_begin + tid; i < count_end; i += kEvictThreads) {
+          const uint32_t key = key_of(i);  // (a thread's own)
+          if ((key ^ prefix) >> above == 0) atomicAdd(&hist[(key >> shift) & mask], 1u);
+        }
       }
       if (whole) {
         __syncthreads();
         sums = hist;
       } else {
         cluster.sync();
-        const int slice = kDigits / ctas;
-        for (int i = rank * slice + tid; i < (rank + 1) * slice; i += kEvictThreads) {
+        const int slice = (kDigits + ctas - 1) / ctas;
+        for (int i = rank * slice + tid; i < min(kDigits, (rank + 1) * slice); i += kEvictThreads) {
           uint32_t all = 0;
           for (int c = 0; c < ctas; ++c) all += cluster.map_shared_rank(hist, c)[i];
           for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(sums, c)[i] = all;
@@ -346,8 +360,9 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Ev
     }
     // slots above and at the threshold: this CTA's (whole: those in front of its own)
     uint32_t more = 0, equal = 0;
+#pragma unroll 4
     for (int i = (whole ? first : begin) + tid; i < (whole ? begin : end); i += kEvictThreads) {
-      const uint32_t key = score_key(__ldg(scores + i));
+      const uint32_t key = key_of(i);
       more += key > prefix;
       equal += key == prefix;
     }
@@ -380,36 +395,47 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Ev
     // (of the equal ones the first to_find stay)
     uint32_t taken = (uint32_t)first + more + min(equal, to_find);
     uint32_t equals = equal;
-    for (int i0 = begin; i0 < end; i0 += kEvictThreads) {
-      const int i = i0 + tid;
-      const float score = i < end ? __ldg(scores + i) : 0.0f;
-      const uint32_t key = i < end ? score_key(score) : 0u;
-      const bool is_equal = i < end && key == prefix, is_more = i < end && key > prefix;
-      const uint32_t eq_mask = __ballot_sync(0xffffffffu, is_equal), more_mask = __ballot_sync(0xffffffffu, is_more);
-      __syncthreads();
-      if (lane == 0) {
-        sh.scan[0][warp] = __popc(more_mask);
-        sh.scan[1][warp] = __popc(eq_mask);
+    // four neighbouring slots per thread; counts of slots above (low half) and at the threshold (high half) as one number
+    for (int i0 = begin; i0 < end; i0 += 4 * kEvictThreads) {
+      const int mine = i0 + 4 * tid;
+      float score[4];
+      uint32_t kind[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        score[e] = mine + e < end ? __ldg(scores + mine + e) : 0.0f;
+        const uint32_t key = score_key(score[e]);
+        kind[e] = mine + e >= end ? 0u : key > prefix ? 1u : key == prefix ? 0x10000u : 0u;
+        sum += kind[e];
+      }
+      uint32_t upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
       }
       __syncthreads();
-      uint32_t m_before = 0, e_before = 0, m_all = 0, e_all = 0;
+      if (lane == 31) sh.scan[0][warp] = upto;
+      __syncthreads();
+      uint32_t before = upto - sum, all = 0;
 #pragma unroll
       for (int w = 0; w < kEvictWarps; ++w) {
-        if (w == warp) m_before = m_all, e_before = e_all;
-        m_all += sh.scan[0][w];
-        e_all += sh.scan[1][w];
+        const uint32_t v = sh.scan[0][w];
+        before += w < warp ? v : 0u;
+        all += v;
       }
-      const uint32_t lower = (1u << lane) - 1u;
-      m_before += __popc(more_mask & lower);
-      e_before += __popc(eq_mask & lower);
       const uint32_t room = to_find > equals ? to_find - equals : 0u;  // equal ones that may still stay
-      if (is_more || (is_equal && e_before < room)) {
-        const uint32_t to = taken + m_before + min(e_before, room);
-        kept[to] = i;
-        scores_out[to] = score;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t m_before = before & 0xffffu, e_before = before >> 16;
+        if (kind[e] == 1u || (kind[e] != 0u && e_before < room)) {
+          const uint32_t to = taken + m_before + min(e_before, room);
+          kept[to] = mine + e;
+          scores_out[to] = score[e];
+        }
+        before += kind[e];
       }
-      taken += m_all + min(e_all, room);
-      equals += e_all;
+      taken += (all & 0xffffu) + min(all >> 16, room);
+      equals += all >> 16;
     }
   }
   if (in_place && !choose) return;  // (uniform over the cluster, and before any barrier of it)
@@ -433,8 +459,9 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Ev
   int32_t* slots = reinterpret_cast<int32_t*>(rows_smem + (size_t)fit * row_pad);
   const uint32_t mine = smem_u32(rows_smem) + (uint32_t)(is_pair ? 2 * nibbles + (part - 2 * chunks) * 4 : part * 16);
   const bool live = part < parts;
-  for (int j0 = in_place ? p.sinks : 0; j0 < left; j0 += ctas * fit) {
-    const int r0 = j0 + rank * fit, rows = max(0, min(fit, left - r0));
+  const int j_first = in_place ? p.sinks : 0, each = min(fit, (left - j_first + ctas - 1) / ctas);
+  for (int j0 = j_first; j0 < left; j0 += ctas * each) {
+    const int r0 = j0 + rank * each, rows = max(0, min(each, left - r0));
     __syncthreads();  // (the slots of the pass before have been used)
     for (int r = tid; r < rows; r += kEvictThreads) slots[r] = __ldcg(kept + r0 + r);
     __syncthreads();
@@ -484,15 +511,15 @@ cudaError_t launch_kv4_read(const Kv4Read& p, cudaStream_t s) {
                : launch_chained(kv4_read_kernel<false>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), words_log2);
 }
 
-// Clusters of eight CTAs with an SM each that fit on the current device at once.
-static int evict_clusters_alone() {
+// Clusters of `ctas` CTAs with an SM each that fit on the current device at once.
+static int evict_clusters_alone(int ctas) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(8);
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kEvictThreads);
   cfg.dynamicSmemBytes = kEvictMostSmem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 8, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.x = (unsigned)ctas, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
@@ -503,26 +530,26 @@ cudaError_t launch_kv4_evict(const Kv4Evict& p, cudaStream_t s) {
   const int pairs = p.from.b * p.from.nkv;
   if (pairs == 0) return cudaSuccess;
   static bool done[64] = {false};
-  static int alone[64];
+  static int alone[64][9];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
   if (!done[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictMostSmem);
     if (e != cudaSuccess) return e;
-    alone[dev] = evict_clusters_alone();
+    for (int c = 1; c <= 8; ++c) alone[dev][c] = evict_clusters_alone(c);
     done[dev] = true;
   }
   const int parts = 2 * (p.from.h / 32) + 2 * (p.from.h / p.from.block);
   int row_log2 = 0;
   while ((1 << row_log2) < parts) ++row_log2;
-  const bool in_place = p.from.k == p.to.k;
+  // The largest clusters that find an SM for each CTA: two CTAs on one SM share its way to memory while others idle, and a
+  // second turn of clusters waits for the first (16 x 4352 to 4096 in place on clusters of 8, for which 15 find room: 33 us).
   int ctas = 8;
-  while (ctas > 1 && (long long)pairs * ctas > device_sm_count()) ctas /= 2;
-  // a whole SM for each CTA, where the clusters find them: two on one SM share its way to memory while others idle
-  const int smem = ctas == 8 && pairs <= alone[dev] ? kEvictMostSmem : kEvictSmem;
-  return launch_chained_cluster(kv4_evict_kernel, dim3((unsigned)(pairs * ctas)), dim3(kEvictThreads), (size_t)smem, ctas, s, p, in_place ? 1 : 0,
-                                row_log2, smem);
+  while (ctas > 1 && pairs > alone[dev][ctas]) --ctas;
+  const int smem = pairs <= alone[dev][ctas] ? kEvictMostSmem : kEvictSmem;
+  return launch_chained_cluster(kv4_evict_kernel, dim3((unsigned)(pairs * ctas)), dim3(kEvictThreads), (size_t)smem, ctas, s, p,
+                                p.from.k == p.to.k ? 1 : 0, row_log2, smem);
 }
 
 }  // namespace b200
