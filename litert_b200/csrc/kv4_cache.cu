@@ -56,34 +56,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 template <bool F32>
-__global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append p, const uint32_t items, const Divisor per_token, const int lanes_log2,
-                                                                 const int vec) {
-  pdl_enter();
-  const uint32_t item = blockIdx.x * kRowThreads + threadIdx.x;  // of a sequence's (token, 16 channels)
-  const int b = blockIdx.y;
-  const bool is_v = blockIdx.z != 0;
-  bool live = item < items;
-  const uint32_t i = live ? item / per_token : 0, rest = live ? item - i * per_token.d : 0;
-  const long long slot = (long long)p.positions[b] + i;
-  live = live && slot >= 0 && slot < p.cache.s && (!p.counts || (int)i < p.counts[b]);  // (alike for the lanes of a block)
-  float x[16];
-  float lo, hi;
-  const long long at = (is_v ? b * p.v_batch + i * p.v_token : b * p.k_batch + i * p.k_token) + (long long)rest * 16;
+struct Sixteen {  // channels, as they lie in memory
+  uint32_t w[F32 ? 16 : 8];
+};
+
+// One block's nibbles of a thread's 16 channels, and the block's pair. `lanes_log2`: log2 of the lanes that have the block.
+template <bool F32>
+__device__ __forceinline__ void quantize_sixteen(const Sixteen<F32>& in, int lanes_log2, uint2& word, __half2& pair) {
+  float x[16], lo, hi;
   if constexpr (F32) {
-    const float* src = static_cast<const float*>(is_v ? p.v : p.k) + at;
-    if (!live) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = 0.0f;
-    } else if (vec) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(src) + e);
-        x[4 * e] = v.x, x[4 * e + 1] = v.y, x[4 * e + 2] = v.z, x[4 * e + 3] = v.w;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = __ldg(src + e);
-    }
+    for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(in.w[e]);
     lo = hi = x[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) {
@@ -95,24 +78,11 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append
       hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
   } else {
-    const __half* src = static_cast<const __half*>(is_v ? p.v : p.k) + at;
-    uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (!live) {
-    } else if (vec) {
-      const uint4 r0 = __ldg(reinterpret_cast<const uint4*>(src)), r1 = __ldg(reinterpret_cast<const uint4*>(src) + 1);
-      w[0] = r0.x, w[1] = r0.y, w[2] = r0.z, w[3] = r0.w, w[4] = r1.x, w[5] = r1.y, w[6] = r1.z, w[7] = r1.w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const __half2 v = __halves2half2(src[2 * e], src[2 * e + 1]);
-        w[e] = *reinterpret_cast<const uint32_t*>(&v);
-      }
-    }
-    __half2 least2 = *reinterpret_cast<const __half2*>(&w[0]), most2 = least2;
+    __half2 least2 = *reinterpret_cast<const __half2*>(&in.w[0]), most2 = least2;
 #pragma unroll
     for (int e = 1; e < 8; ++e) {
-      least2 = __hmin2_nan(least2, *reinterpret_cast<const __half2*>(&w[e]));
-      most2 = __hmax2_nan(most2, *reinterpret_cast<const __half2*>(&w[e]));
+      least2 = __hmin2_nan(least2, *reinterpret_cast<const __half2*>(&in.w[e]));
+      most2 = __hmax2_nan(most2, *reinterpret_cast<const __half2*>(&in.w[e]));
     }
     // (minimum, -maximum)
     __half2 both = __halves2half2(__hmin_nan(__low2half(least2), __high2half(least2)), __hneg(__hmax_nan(__low2half(most2), __high2half(most2))));
@@ -124,7 +94,7 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append
     hi = -__high2float(both);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&in.w[e]));
       x[2 * e] = f.x, x[2 * e + 1] = f.y;
     }
   }
@@ -133,35 +103,95 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append
   const float least = __half2float(least_h);
   __half scale_h = __float2half_rn(fminf(fmaxf(__fdiv_rn(__fsub_rn(hi, least), 15.0f), 0.0f), 65504.0f));
   const float scale = __half2float(scale_h);
-  uint32_t word[2] = {0, 0};
-  if (bad) {
-    least_h = scale_h = __ushort_as_half(0x7fff);
-  } else if (scale > 0.0f) {
-    const float inverse = __fdividef(1.0f, 15.0f * scale);
-    float n[16], far = 0.0f;
+  if (bad) least_h = scale_h = __ushort_as_half(0x7fff);
+  pair = __halves2half2(scale_h, least_h);
+  // (a factor of zero, and whatever it meets, saturates to zero)
+  const float inverse = bad || scale == 0.0f ? 0.0f : __fdividef(1.0f, 15.0f * scale);
+  float n[16], far = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float y = __saturatef((x[e] - least) * inverse);
+    n[e] = fmaf(y, 15.0f, 12582912.0f) - 12582912.0f;  // rounded by the sum's last place
+    far = fmaxf(far, fabsf(fmaf(y, 15.0f, -n[e])));
+  }
+  if (far > 0.49999f) {  // (a quarter of the warps of fp16 rows: exact ties among 512 elements; each of them seldom)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float y = __saturatef((x[e] - least) * inverse);
-      n[e] = fmaf(y, 15.0f, 12582912.0f) - 12582912.0f;  // rounded by the sum's last place
-      far = fmaxf(far, fabsf(fmaf(y, 15.0f, -n[e])));
-    }
-    if (far > 0.49999f) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) n[e] = nearest_float(n[e], x[e], least, scale);
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float* m = n + 8 * e;
-      // (sums below 2^16, exact; a number added to 2^23 is its low bits)
-      const float low = fmaf(fmaf(m[3], 16.0f, m[2]), 256.0f, fmaf(m[1], 16.0f, m[0])) + 8388608.0f;
-      const float high = fmaf(fmaf(m[7], 16.0f, m[6]), 256.0f, fmaf(m[5], 16.0f, m[4])) + 8388608.0f;
-      word[e] = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+      if (fabsf(fmaf(y, 15.0f, -n[e])) > 0.49999f) n[e] = nearest_float(n[e], x[e], least, scale);
     }
   }
-  if (!live) return;
-  const size_t to = ((size_t)b * p.cache.s + (size_t)slot) * per_token.d + rest;
-  *reinterpret_cast<uint2*>((is_v ? p.cache.v : p.cache.k) + to * 8) = make_uint2(word[0], word[1]);
-  if ((rest & ((1u << lanes_log2) - 1)) == 0) (is_v ? p.cache.v_pairs : p.cache.k_pairs)[to >> lanes_log2] = __halves2half2(scale_h, least_h);
+  uint32_t out[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float* m = n + 8 * e;
+    // (sums below 2^16, exact; a number added to 2^23 is its low bits)
+    const float low = fmaf(fmaf(m[3], 16.0f, m[2]), 256.0f, fmaf(m[1], 16.0f, m[0])) + 8388608.0f;
+    const float high = fmaf(fmaf(m[7], 16.0f, m[6]), 256.0f, fmaf(m[5], 16.0f, m[4])) + 8388608.0f;
+    out[e] = __byte_perm(__float_as_uint(low), __float_as_uint(high), 0x5410);
+  }
+  word = make_uint2(out[0], out[1]);
+}
+
+// A thread walks over a sequence's pieces of 16 channels, the next one asked for before this one is used: what does not
+// depend on the piece is a third of the instructions otherwise.
+template <bool F32>
+__global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append p, const uint32_t items, const Divisor per_token, const int lanes_log2,
+                                                                 const int vec) {
+  constexpr int kElem = F32 ? 4 : 2;
+  pdl_enter();
+  const int b = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  const uint8_t* src = static_cast<const uint8_t*>(is_v ? p.v : p.k) + (is_v ? p.v_batch : p.k_batch) * b * kElem;
+  const long long token = (is_v ? p.v_token : p.k_token) * kElem;
+  const long long position = p.positions[b];
+  const int count = p.counts ? min(p.counts[b], p.t) : p.t;
+  // tokens that have a slot
+  const int first = (int)max(0ll, min((long long)INT32_MAX, -position)), behind = (int)max(0ll, min((long long)count, (long long)p.cache.s - position));
+  uint8_t* nibbles = (is_v ? p.cache.v : p.cache.k) + ((long long)b * p.cache.s + position) * per_token.d * 8;
+  __half2* pairs = (is_v ? p.cache.v_pairs : p.cache.k_pairs) + ((((long long)b * p.cache.s + position) * per_token.d) >> lanes_log2);
+  auto ask = [&](uint32_t item, Sixteen<F32>& in) {
+    const uint32_t i = item / per_token, rest = item - i * per_token.d;
+    const bool live = item < items && (int)i >= first && (int)i < behind;  // (alike for the lanes of a block)
+    if (live) {
+      const uint8_t* at = src + i * token + (size_t)rest * 16 * kElem;
+      if (vec) {
+#pragma unroll
+        for (int e = 0; e < (F32 ? 4 : 2); ++e) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + e);
+          in.w[4 * e] = v.x, in.w[4 * e + 1] = v.y, in.w[4 * e + 2] = v.z, in.w[4 * e + 3] = v.w;
+        }
+      } else if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) in.w[e] = __ldg(reinterpret_cast<const uint32_t*>(at) + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          in.w[e] = __ldg(reinterpret_cast<const unsigned short*>(at) + 2 * e) | (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(at) + 2 * e + 1) << 16;
+      }
+    }
+    return live;
+  };
+  const uint32_t step = gridDim.x * kRowThreads;
+  uint32_t item = blockIdx.x * kRowThreads + threadIdx.x;
+  Sixteen<F32> next;
+#pragma unroll
+  for (int e = 0; e < (F32 ? 16 : 8); ++e) next.w[e] = 0;
+  bool next_live = ask(item, next);
+  for (uint32_t front = blockIdx.x * kRowThreads; front < items; front += step) {  // (the block's first: all lanes stay)
+    const Sixteen<F32> in = next;
+    const bool live = next_live;
+    const uint32_t now = item;
+    item += step;
+    next_live = ask(item, next);
+    uint2 word;
+    __half2 pair;
+    quantize_sixteen<F32>(in, lanes_log2, word, pair);
+    if (live) {
+      *reinterpret_cast<uint2*>(nibbles + (size_t)now * 8) = word;
+      if ((now & ((1u << lanes_log2) - 1)) == 0) pairs[now >> lanes_log2] = pair;
+    }
+  }
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------
@@ -497,7 +527,8 @@ cudaError_t launch_kv4_append(const Kv4Append& p, cudaStream_t s) {
   const int elem = p.f32 ? 4 : 2, per = 16 / elem;  // elements of a 16-byte load
   const bool vec = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0 &&
                    p.k_batch % per == 0 && p.k_token % per == 0 && p.v_batch % per == 0 && p.v_token % per == 0;
-  const dim3 grid((items + kRowThreads - 1) / kRowThreads, p.cache.b, 2);
+  const unsigned blocks = (items + kRowThreads - 1) / kRowThreads, enough = (unsigned)(6 * device_sm_count() + 2 * p.cache.b - 1) / (2 * p.cache.b);
+  const dim3 grid(blocks < enough ? blocks : enough, p.cache.b, 2);  // three blocks per SM
   const int lanes_log2 = p.cache.block == 64 ? 2 : 1;
   return p.f32 ? launch_chained(kv4_append_kernel<true>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), lanes_log2, vec ? 1 : 0)
                : launch_chained(kv4_append_kernel<false>, grid, dim3(kRowThreads), 0, s, p, items, divisor(per_token), lanes_log2, vec ? 1 : 0);
