@@ -57,7 +57,7 @@ def values(cache, i):
     return u * wide[..., 0] + wide[..., 1], u * np.abs(wide[..., 0]) + np.abs(wide[..., 1])
 
 
-def attention(q, k, v, k_mag, v_mag, limits, scale, cap, mask):
+def attention(q, k, v, k_mag, v_mag, limits, scale, cap, mask, v_half=None):
     """One sequence in float64: q [t, n, h], k / v [s, nkv, h]. Returns outputs, weights per KV head [nkv, s], and bounds
     of what float32 sums may be off by in either.
 
@@ -66,7 +66,8 @@ def attention(q, k, v, k_mag, v_mag, limits, scale, cap, mask):
     magnitudes (tensor cores may truncate); the cap's tanh and division add four steps of the cap's value, scaling and
     mask four of the logit's. A weight is off by twice its logit's error (numerator and maximum's share) and by eight steps
     of (1 + |x - top| log2 e): exponent, exponential, division. Sums over s slots add s + 64 steps of the magnitudes; the
-    weights' split into two fp16 numbers 2^-21."""
+    weights' split into two fp16 numbers 2^-21. For fp16 queries a weight times its value
+    scale a is one fp16 number, off by half a step, which counts (u - 8) times: v_half = 8 |a| bounds |u - 8| |a|."""
     t, n, h = q.shape
     s, nkv = k.shape[:2]
     step = 2 * EPS32
@@ -99,6 +100,8 @@ def attention(q, k, v, k_mag, v_mag, limits, scale, cap, mask):
             mag = np.where(keep[:, None], v_mag[:limits[i], j], 0.0)
             out[i, head] = w @ vv
             out_off[i, head] = (rel + (s + 64) * step + 2.0 ** -21) * (w @ mag)
+            if v_half is not None:
+                out_off[i, head] += EPS16 * (w @ np.where(keep[:, None], v_half[:limits[i], j], 0.0))
             weights[j, :limits[i]] += w
             weights_off[j, :limits[i]] += w * rel + 1e-30
     return out, weights, out_off, weights_off
@@ -119,12 +122,13 @@ def check_attention(ops, ws, q, cache, lengths=None, mask=None, scale=None, cap=
     assert got.dtype == q.dtype and got.shape == q.shape
     got = got.cpu().numpy().astype(np.float64)
     (k, km), (v, vm) = values(cache, 0), values(cache, 1)
+    half = 8 * np.repeat(np.abs(cache[3][..., 0].cpu().numpy().astype(np.float64)), h // cache[3].shape[3], axis=-1)
     qf = q.cpu().numpy().astype(np.float64)
     for i in range(b):
         lim = limits_of(s if lengths is None else lengths[i], s, t)
         with np.errstate(invalid="ignore"):
             want, w, off, w_off = attention(qf[i], k[i], v[i], km[i], vm[i], lim, scale or 1 / math.sqrt(h), cap,
-                                            None if mask is None else mask[i, 0].astype(np.float64))
+                                            None if mask is None else mask[i, 0].astype(np.float64), half[i] if q.dtype == torch.float16 else None)
         bound = off + (EPS16 * np.abs(want) + 2.0 ** -25 if q.dtype == torch.float16 else EPS32 * np.abs(want))
         assert np.isfinite(got[i]).all(), i
         assert (np.abs(got[i] - want) <= bound).all(), (i, lim, np.max(np.abs(got[i] - want) - bound), np.max(np.abs(got[i] - want)))
@@ -409,7 +413,9 @@ def test_offsets_beyond_32_bits(ops, ws):
     ops.kv_append_int4(dev(rows), dev(rows[:, ::-1]), torch.zeros(b, dtype=torch.int32, device="cuda"), *short)
     few = torch.zeros((b, nkv, 40), device="cuda")
     want = ops.sdpa_decode_int4(q, *short, scores=few, ws=ws).float()
-    assert torch.allclose(got, want, rtol=2 * EPS16, atol=2.0 ** -12)  # two roundings to fp16, sums in another order
+    # Two roundings of an output to fp16, and two of the weights: 40 of them, each at most half a step off, times |u - 8| <= 8
+    # times a value scale, which is below (4.5 + 4.5) / 15 for normal numbers. (Sums in another order: below that.)
+    assert torch.allclose(got, want, rtol=2 * EPS16, atol=2 * EPS16 * 8 * 0.6)
     assert torch.allclose(scores[2, :, s - 40:], few[2], rtol=1e-5, atol=1e-9) and not scores[2, :, :s - 40].any()
     kept, new, left = ops.kv_evict_int4(*cache, scores, torch.full((b,), s, dtype=torch.int32, device="cuda"), 16, recent=16)
     assert torch.equal(kept[2, 5].cpu(), torch.arange(s - 16, s, dtype=torch.int32)) and left.tolist() == [16] * 3
@@ -507,11 +513,11 @@ def test_a_reply_with_evictions(ops, ws, n, nkv, h, block, f32):
     def stored(x):
         u, scale, least = quantize(x, block)
         wide = lambda y: np.repeat(y.astype(np.float64), block, -1)  # noqa: E731
-        return u * wide(scale) + wide(least), u * np.abs(wide(scale)) + np.abs(wide(least))
+        return u * wide(scale) + wide(least), u * np.abs(wide(scale)) + np.abs(wide(least)), 8 * np.abs(wide(scale))
 
     k, v = token(40), token(40)
     ops.kv_append_int4(dev(k), dev(v), torch.zeros(b, dtype=torch.int32, device="cuda"), *cache, counts=dev(counts))
-    # per sequence and KV head: (key, its magnitudes, value, its magnitudes) of the tokens still cached
+    # per sequence and KV head: (key, its magnitudes, eight of its scales, value, ...) of the tokens still cached
     held = [[[tuple(z[i, x, j] for y in (k, v) for z in stored(y)) for x in range(counts[i])] for j in range(nkv)] for i in range(b)]
     lengths = dev(counts)
     evictions = 0
@@ -532,14 +538,15 @@ def test_a_reply_with_evictions(ops, ws, n, nkv, h, block, f32):
         lengths = lengths + t
         before = scores.cpu().numpy().copy()
         got = ops.sdpa_decode_int4(dev(q), *cache, lengths=lengths, scores=scores, ws=ws).cpu().numpy().astype(np.float64)
-        (sk, skm), (sv, svm) = stored(k), stored(v)
+        now = stored(k) + stored(v)
         for i in range(b):
             for j in range(nkv):
-                held[i][j] += [(sk[i, x, j], skm[i, x, j], sv[i, x, j], svm[i, x, j]) for x in range(t)]
-            rows = [np.stack([[y[c] for y in held[i][j]] for j in range(nkv)], 1) for c in range(4)]
+                held[i][j] += [tuple(y[i, x, j] for y in now) for x in range(t)]
+            rows = [np.stack([[y[c] for y in held[i][j]] for j in range(nkv)], 1) for c in range(6)]
             lim = limits_of(len(held[i][0]), s, t)
             assert lim[-1] == int(lengths[i])
-            want, w, off, w_off = attention(q[i].astype(np.float64), rows[0], rows[2], rows[1], rows[3], lim, 1 / math.sqrt(h), 0.0, None)
+            want, w, off, w_off = attention(q[i].astype(np.float64), rows[0], rows[3], rows[1], rows[4], lim, 1 / math.sqrt(h), 0.0, None,
+                                             None if f32 else rows[5])
             bound = off + (EPS32 if f32 else EPS16) * np.abs(want) + 2.0 ** -25
             assert (np.abs(got[i] - want) <= bound).all(), (step, i)
             after = scores[i].cpu().numpy()
