@@ -409,8 +409,8 @@ B200_API int b200_kv4_read(const void* d_k_cache, const void* d_v_cache, const v
  * none) as in b200_sdpa_decode, never negative.
  * d_scores [b, nkv, s_max] f32 (optional): += the softmax weights that each slot got from its KV
  * head's n / nkv * t queries (what b200_kv4_evict ranks by); slots beyond the length are left
- * alone. Any number of query heads per KV head. Workspace: on a 16-byte boundary, no initial
- * contents. */
+ * alone. Any number of query heads per KV head. Queries and workspace lie on 16-byte boundaries;
+ * the workspace needs no initial contents. */
 B200_API size_t b200_kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int block, int s_max, int with_scores);
 B200_API int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache, const void* d_k_scale,
                            const void* d_v_scale, const int32_t* d_lengths, const float* d_mask, float* d_scores, void* d_out,

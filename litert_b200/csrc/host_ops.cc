@@ -341,7 +341,8 @@ PyObject* sdpa_decode_int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     In q(a[0], type), lengths(a[5], at::kInt, true), mask(a[6], at::kFloat, true), scores(a[9], at::kFloat, true), ws(ws_o.o, at::kByte);
     float scale, cap;
     if (!c.here(q) || !c.per_sequence(lengths) || !c.here(mask) || !c.here(scores) || !c.here(ws) || !as_float(a[7], &scale) || !as_float(a[8], &cap) ||
-        q.t->dim() != 4 || q.t->size(0) != c.b || q.t->size(3) != c.h || q.t->numel() == 0 || q.t->size(1) > 65535 || q.t->size(2) > 1 << 20)
+        q.t->dim() != 4 || q.t->size(0) != c.b || q.t->size(3) != c.h || q.t->numel() == 0 || q.t->size(1) > 65535 || q.t->size(2) > 1 << 20 ||
+        (reinterpret_cast<uintptr_t>(q.ptr<void>()) & 15) != 0)
       Py_RETURN_NONE;
     const int t = (int)q.t->size(1), n = (int)q.t->size(2);
     if (n % c.nkv != 0 || (mask.t && mask.t->sizes() != at::IntArrayRef{c.b, 1, t, c.s}) ||

@@ -153,6 +153,8 @@ int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache,
   if (!(logit_cap >= 0.0f) || !(scale >= 0.0f)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: scale and logit cap are positive, or 0", name);
   if (b == 0) return B200_OK;
   if (!d_q || !d_out) return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  if (!aligned(d_q, 16) || !aligned(d_out, q_dtype == B200_DTYPE_F32 ? 4 : 2))
+    return fail(B200_ERR_INVALID_ARGUMENT, "%s: queries lie on a 16-byte boundary, outputs on boundaries of their elements", name);
   const size_t need = b200::kv4_sdpa_workspace_bytes(b, t, n, nkv, h, s_max, d_scores != nullptr);
   if (!d_workspace || workspace_bytes < need || !aligned(d_workspace, 16))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes on a 16-byte boundary needed (b200_kv4_sdpa_workspace_bytes), got %zu", name,

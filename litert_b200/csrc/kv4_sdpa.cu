@@ -1166,17 +1166,16 @@ cudaError_t launch_tensor_block(const Kv4Sdpa& p, cudaStream_t s) {
 
 size_t kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int s, int scores) {
   const size_t rows = (size_t)b * t * n;
-  const size_t any = 2 * rows + rows * s;  // (also what queries off a 16-byte boundary need)
-  if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return any * sizeof(float);
+  if (!kv4_tensor_shape(b, t, n, nkv, h, s)) return (2 * rows + rows * s) * sizeof(float);
   const long long pairs = (long long)b * nkv * kv4_rows(t, n, nkv).chunks;
   const size_t tensor = kv4_records_floats((long long)kv4_ctas(pairs, s, h) * kv4_warps(h), h) +
                         (scores ? 16 * (size_t)pairs + (size_t)pairs * tiles_of(s) * kSlots * 8 : 0);
-  return (any > tensor ? any : tensor) * sizeof(float);
+  return tensor * sizeof(float);
 }
 
 cudaError_t launch_kv4_sdpa(const Kv4Sdpa& p, cudaStream_t s) {
   const Kv4Cache& c = p.cache;
-  if (!kv4_tensor_shape(c.b, p.t, p.n, c.nkv, c.h, c.s) || (reinterpret_cast<uintptr_t>(p.q) & 15) != 0) return launch_rows(p, s);
+  if (!kv4_tensor_shape(c.b, p.t, p.n, c.nkv, c.h, c.s)) return launch_rows(p, s);
   return c.h == 256 ? launch_tensor_block<256>(p, s) : c.h == 128 ? launch_tensor_block<128>(p, s) : launch_tensor_block<64>(p, s);
 }
 

@@ -48,6 +48,7 @@ class Workspace:
             check(lib.b200_zero_workspace_init(_ptr(self.zero), _stream()))
         self.scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=self.device)
         self.sdpa = None
+        self.outgrown = []  # captured graphs may hold these
 
     def scratch_for(self, m, k):
         need = _lib.load().b200_fc_scratch_bytes(m, k)
@@ -60,6 +61,8 @@ class Workspace:
 
     def sdpa_bytes(self, need):
         if self.sdpa is None or self.sdpa.numel() < need:
+            if self.sdpa is not None:
+                self.outgrown.append(self.sdpa)
             self.sdpa = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self.sdpa
 
@@ -496,6 +499,8 @@ def sdpa_decode_int4(q, k_cache, v_cache, k_scale, v_scale, lengths=None, mask=N
     if q.dim() != 4 or q.shape[0] != b or q.shape[3] != h or q.shape[1] == 0 or q.shape[2] == 0 or q.shape[2] % nkv:
         raise B200Error("q must be [b, t, n, h] of the cache, n a multiple of its KV heads")
     q = q.contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
     t, n = q.shape[1], q.shape[2]
     lengths = _per_sequence(lengths, b, k_cache, "lengths")
     mask = _need(mask, torch.float32, "mask")

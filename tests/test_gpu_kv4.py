@@ -598,6 +598,82 @@ def test_a_captured_step_replays(ops):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
+def test_a_captured_call_keeps_its_workspace(ops):
+    """A larger call later takes a larger workspace; the graph's stays its own."""
+    cache, g = random_cache(ops, 3, 2, 9000, 2, 64, 32)  # (records of several CTAs, merged)
+    for i in (2, 3):
+        cache[i].copy_(torch.randn(cache[i].shape, generator=g, device="cuda").half() * 0.2)
+    q = torch.randn((2, 1, 8, 64), generator=g, device="cuda")
+    ws = ops.Workspace("cuda")
+    want = ops.sdpa_decode_int4(q, *cache, ws=ws).clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.sdpa_decode_int4(q, *cache, ws=ws)
+    before, size = ws.sdpa.data_ptr(), ws.sdpa.numel()
+    scores = torch.zeros((2, 2, 9000), device="cuda")
+    ops.sdpa_decode_int4(q.expand(2, 1, 8, 64).repeat(1, 64, 1, 1), *cache, scores=scores, ws=ws)
+    assert ws.sdpa.numel() > size and ws.sdpa.data_ptr() != before
+    others = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]  # (what would get its memory)
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want) and all(bool((x == 255).all()) for x in others)
+
+
+def test_rows_off_a_16_byte_boundary(ops, ws):
+    """Queries, keys and values that begin anywhere, broadcast over the sequences, are those on a boundary."""
+    rng = np.random.default_rng(31)
+    for h, dtype in ((64, np.float16), (256, np.float32), (96, np.float16)):
+        b, s, nkv, n = 2, 50, 2, 4
+        def moved(shape):
+            flat = dev(rng.standard_normal(1 + math.prod(shape)).astype(dtype))
+            return flat[1:].view(shape)
+        k, v, q = moved((1, 40, nkv, h)).expand(b, 40, nkv, h), moved((b, 40, nkv, h)), moved((b, 2, n, h))
+        at, caches, outs = torch.zeros(b, dtype=torch.int32, device="cuda"), [], []
+        for copy in (False, True):
+            cache = ops.int4_kv_cache(b, s, nkv, h, 32)
+            ops.kv_append_int4(k.clone() if copy else k, v.clone() if copy else v, at, *cache)
+            caches.append(cache)
+            outs.append(ops.sdpa_decode_int4(q.clone() if copy else q, *cache, lengths=at + 40, ws=ws))
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(*caches))
+        assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("h,block", [(256, 64), (96, 32)])
+def test_both_host_paths_give_the_same(ops, monkeypatch, f32, h, block):
+    """The calls through the extension, and again without it."""
+    from litert_b200 import _lib
+
+    native = ops._host
+    assert native is not _lib._GeneralPath, "the extension is not built"
+    b, s, nkv, n = 3, 70, 2, 6
+    dtype = torch.float32 if f32 else torch.float16
+    g = torch.Generator("cuda").manual_seed(7)
+    k, v = (torch.randn((b, 20, nkv, h), generator=g, device="cuda").to(dtype) for _ in range(2))
+    q = torch.randn((b, 2, n, h), generator=g, device="cuda").to(dtype)
+    mask = torch.randn((b, 1, 2, s), generator=g, device="cuda")
+    at, counts = dev(np.asarray([0, 30, 45], np.int32)), dev(np.asarray([20, 7, 20], np.int32))
+    results = []
+    for path in (native, _lib._GeneralPath):
+        monkeypatch.setattr(ops, "_host", path)
+        ws = ops.Workspace("cuda")
+        cache, scores = ops.int4_kv_cache(b, s, nkv, h, block), torch.zeros((b, nkv, s), device="cuda")
+        ops.kv_append_int4(k, v, at, *cache, counts=counts)
+        got = list(ops.kv_read_int4(*cache, tokens=25, positions=at, counts=counts, dtype=dtype))
+        got += list(ops.kv_read_int4(*cache))
+        for kw in (dict(), dict(scores=scores, lengths=at + counts, mask=mask, scale=0.1, logit_cap=4.0)):
+            ops.sdpa_decode_int4(q, *cache, ws=ws)  # (the workspace is there)
+            got.append(ops.sdpa_decode_int4(q, *cache, ws=ws, **kw))
+        into = ops.int4_kv_cache(b, 30, nkv, h, block)
+        got += list(ops.kv_evict_int4(*cache, scores, at + counts, 30, sinks=2, recent=5, into=into)) + list(into)
+        got += list(ops.kv_evict_int4(*cache, scores, at + counts, 24)) + list(cache) + [scores]
+        results.append(got)
+    for x, y in zip(*results):
+        assert x.dtype == y.dtype and x.shape == y.shape
+        assert torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+
+
 def test_refusals(ops):
     cache = ops.int4_kv_cache(2, 16, 2, 64)
     x = torch.zeros((2, 1, 2, 64), device="cuda")

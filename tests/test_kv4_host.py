@@ -69,7 +69,8 @@ def test_read_refusals(lib, wrong):
 
 @pytest.mark.parametrize("wrong", [dict(q=None), dict(out=None), dict(t=0), dict(t=1 << 20), dict(n=3), dict(n=0), dict(dtype=1),
                                    dict(scale=-1.0), dict(scale=float("nan")), dict(cap=-1.0), dict(cap=float("nan")),
-                                   dict(ws=None), dict(ws_bytes=0), dict(ws=P + 4), dict(ws_bytes=64)])
+                                   dict(ws=None), dict(ws_bytes=0), dict(ws=P + 4), dict(ws_bytes=64), dict(q=P + 8),
+                                   dict(out=P + 1), dict(dtype=2, out=P + 2)])
 def test_attention_refusals(lib, wrong):
     assert _sdpa(lib, **wrong) in (1, 4)
 
@@ -87,6 +88,11 @@ def test_attention_refusals(lib, wrong):
 ])
 def test_eviction_refusals(lib, wrong):
     assert _evict(lib, **wrong) in (1, 4)
+
+
+def test_the_workspace_does_not_grow_with_the_cache_where_no_logit_is_kept(lib):
+    need = [lib.b200_kv4_sdpa_workspace_bytes(64, 1, 8, 1, 256, 64, s, 0) for s in (4096, 32768, 1 << 20)]
+    assert need[0] == need[1] == need[2] < 32 << 20
 
 
 def test_nothing_to_do_is_no_error(lib):
