@@ -190,7 +190,7 @@ __host__ __device__ inline Kv4Rows kv4_rows(int t, int n, int nkv) {
 }
 
 // Workspace of the tensor-core kernels: a record per piece (of which the first of a pair in each CTA is used), then, where
-// scores are wanted, the rows' {maximum, 1 / sum} [pair][8 rows] and the logits [pair][slot (rounded up to a tile)][8 rows].
+// scores are wanted, the rows' {maximum, 1 / sum} [pair][8 rows] of pairs that have a CTA to themselves, and the logits [pair][slot (rounded up to a tile)][8 rows].
 constexpr int kFewRecords = 16;
 __host__ __device__ inline size_t kv4_records_floats(long long pieces, int h) { return (size_t)pieces * 8 * (h + 4); }
 
@@ -977,11 +977,115 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
   }
 }
 
+constexpr int kMergeThreads = 128;
+constexpr int kScoreSlots = 256, kStatChunks = 16;
+
+// Adds the weights that kScoreSlots slots of a KV head got to the scores. A row's maximum and sum come from its pair's records
+// (or from the CTA that has the pair), again in every CTA: a kernel of its own behind the merge, which left them there, took
+// 21.0 us in all instead of 20.3 at 16 x 8192 (16 heads of 128 over 2), and 21.7 instead of 17.9 for drafts of four tokens at
+// 8 x 4096. (128 slots: 21.3 and 18.3 us; 512: 21.2 and 19.3; 1024: 23.3 and 22.4.)
+template <int H>
+__device__ void kv4_add_scores(const Kv4Sdpa& p, const Kv4Cut& cut, const Kv4Rows& rw, int b, int index, int below, int pieces, const float2* stats_ws,
+                               const float* logits_ws) {
+  constexpr int kRec = H + 4, kPerThread = kScoreSlots / kMergeThreads, kAtOnce = 4;
+  __shared__ float2 s_stat[kStatChunks][8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane & 7;
+  const int parts = (p.cache.s + kScoreSlots - 1) / kScoreSlots, kvh = index / parts, slot0 = (index - kvh * parts) * kScoreSlots + tid;
+  const int length = kv4_length(p, b);
+  if (slot0 - tid >= length) return;
+  const size_t pitch = (size_t)tiles_of(p.cache.s) * kSlots * 8;
+  const size_t pair0 = ((size_t)b * p.cache.nkv + kvh) * rw.chunks;
+  float4 next[kPerThread][2];
+  auto ask = [&](int c) {
+    const float* logits = logits_ws + (pair0 + c) * pitch;
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+      const int slot = slot0 + j * kMergeThreads;
+      const float4* from = reinterpret_cast<const float4*>(logits + (size_t)slot * 8);
+      next[j][0] = next[j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (slot < length) next[j][0] = __ldcg(from), next[j][1] = __ldcg(from + 1);
+    }
+  };
+  ask(0);
+  float sums[kPerThread];
+#pragma unroll
+  for (int j = 0; j < kPerThread; ++j) sums[j] = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < rw.chunks; ++c) {
+    if (c % kStatChunks == 0) {
+      __syncthreads();
+#pragma unroll 1
+      for (int k = warp; k < min(kStatChunks, rw.chunks - c); k += kMergeThreads / 32) {
+        const bool there = row < rw.rows - 8 * (c + k);
+        float2 st = make_float2(0.0f, 0.0f);
+        if (cut.own_cta) {
+          if (there) st = __ldcg(stats_ws + (pair0 + c + k) * 8 + row);
+        } else {
+          const int first = below + (kvh * rw.chunks + c + k) * pieces, cta = cut.owner(first), count = cut.owner(first + pieces - 1) - cta + 1;
+          float top = -CUDART_INF_F, sum = 0.0f;
+#pragma unroll 1
+          for (int j0 = lane >> 3; j0 < count; j0 += 4 * kAtOnce) {
+            float2 ml[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+              const int at = j0 + 4 * j;
+              const float* rec = p.ws + (size_t)(at == 0 ? first : cut.begin(cta + min(at, count - 1))) * (8 * kRec);
+              ml[j] = make_float2(-CUDART_INF_F, 0.0f);
+              if (there && at < count) ml[j] = __ldcg(reinterpret_cast<const float2*>(rec + row * kRec + H));
+            }
+            float now = top;
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) now = fmaxf(now, ml[j].x);
+            const float use = now == -CUDART_INF_F ? 0.0f : now;
+            sum *= power2((top - use) * kLog2e);
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) sum = fmaf(power2((ml[j].x - use) * kLog2e), ml[j].y, sum);
+            top = now;
+          }
+#pragma unroll
+          for (int o = 8; o < 32; o <<= 1) {
+            const float top2 = __shfl_xor_sync(0xffffffffu, top, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
+            const float now = fmaxf(top, top2), use = now == -CUDART_INF_F ? 0.0f : now;
+            // (the same sum in both lanes: a + b = b + a)
+            sum = __fadd_rn(__fmul_rn(power2((top - use) * kLog2e), sum), __fmul_rn(power2((top2 - use) * kLog2e), sum2));
+            top = now;
+          }
+          st = make_float2(top == -CUDART_INF_F ? 0.0f : top, sum != 0.0f ? 1.0f / sum : 0.0f);
+        }
+        if (lane < 8) s_stat[k][row] = st;
+      }
+      __syncthreads();
+    }
+    float4 x[kPerThread][2];
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) x[j][0] = next[j][0], x[j][1] = next[j][1];
+    if (c + 1 < rw.chunks) ask(c + 1);
+    const int rows = rw.rows - 8 * c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 st = s_stat[c % kStatChunks][e];
+#pragma unroll
+      for (int j = 0; j < kPerThread; ++j) {
+        const float4 y = x[j][e / 4];
+        const float v = e % 4 == 0 ? y.x : e % 4 == 1 ? y.y : e % 4 == 2 ? y.z : y.w;
+        if (e < rows) sums[j] = fmaf(power2((v - st.x) * kLog2e), st.y, sums[j]);
+      }
+    }
+  }
+  float* scores = p.scores + ((size_t)b * p.cache.nkv + kvh) * p.cache.s;
+#pragma unroll
+  for (int j = 0; j < kPerThread; ++j) {
+    const int slot = slot0 + j * kMergeThreads;
+    if (slot < length) scores[slot] += sums[j];
+  }
+}
+
 // Merges the records of one query row, H >> part_log2 channels per CTA. What it costs are its start and L2 round trips, so
 // there is one for all records up to 32 (64, 128 where the channels are parted), requested before their weights are known.
-constexpr int kMergeThreads = 128;
+// The CTAs behind the first `merge_ctas` of a sequence add to the scores.
 template <int H, bool QF32>
-__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa p, const int ctas, const int part_log2, float2* stats_ws) {
+__global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa p, const int ctas, const int merge_ctas, const int part_log2,
+                                                                  const float2* stats_ws, const float* logits_ws) {
   constexpr int kRec = H + 4, kBatch = H / 16;
   __shared__ float4 s_part[kMergeThreads];
   __shared__ float s_sum[kMergeThreads];
@@ -1004,6 +1108,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
   const float* base = p.ws + (r & 7) * kRec;
   pdl_launch_dependents();
   pdl_wait();
+  if ((int)blockIdx.x >= merge_ctas) return kv4_add_scores<H>(p, cut, rw, b, blockIdx.x - merge_ctas, below, pieces, stats_ws, logits_ws);
   if (cut.own_cta) return;
   float sum = 0.0f, top = -CUDART_INF_F;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1059,56 +1164,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv4_merge_kernel(const Kv4Sdpa 
     acc.w = fmaf(f, v.w, acc.w);
     sum = fmaf(f, s_sum[at], sum);
   }
-  kv4_output<H, QF32>(p, stats_ws, b, i, head, b * per + in_b, r & 7, d, top, sum, acc);
-}
-
-// Adds the weights that 1024 slots of a KV head got to the scores.
-constexpr int kScoreThreads = 256;
-constexpr int kScoreSlots = 1024;
-__global__ void __launch_bounds__(kScoreThreads) kv4_scores_kernel(const Kv4Sdpa p, const float2* stats_ws, const float* logits_ws) {
-  __shared__ float2 s_stat[8];
-  pdl_launch_dependents();
-  const int b = blockIdx.z, kvh = blockIdx.y, slot0 = blockIdx.x * kScoreSlots;
-  const Kv4Rows rw = kv4_rows(p.t, p.n, p.cache.nkv);
-  const size_t pitch = (size_t)tiles_of(p.cache.s) * kSlots * 8;
-  const int length = kv4_length(p, b);  // (the kernel before has waited for whatever wrote it)
-  float* scores = p.scores + ((size_t)b * p.cache.nkv + kvh) * p.cache.s;
-  pdl_wait();
-  if (slot0 >= length) return;
-  float sums[kScoreSlots / kScoreThreads];
-#pragma unroll
-  for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) sums[j] = 0.0f;
-  for (int c = 0; c < rw.chunks; ++c) {
-    const size_t pair = ((size_t)b * p.cache.nkv + kvh) * rw.chunks + c;
-    const int rows = min(8, rw.rows - 8 * c);
-    __syncthreads();
-    if (threadIdx.x < 8) s_stat[threadIdx.x] = (int)threadIdx.x < rows ? __ldcg(stats_ws + pair * 8 + threadIdx.x) : make_float2(0.0f, 0.0f);
-    const float* logits = logits_ws + pair * pitch;
-    float4 x[kScoreSlots / kScoreThreads][2];
-#pragma unroll
-    for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) {
-      const int slot = slot0 + threadIdx.x + j * kScoreThreads;
-      const float4* from = reinterpret_cast<const float4*>(logits + (size_t)slot * 8);
-      x[j][0] = x[j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (slot < length) x[j][0] = __ldcg(from), x[j][1] = __ldcg(from + 1);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 st = s_stat[e];
-#pragma unroll
-      for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) {
-        const float4 y = x[j][e / 4];
-        const float v = e % 4 == 0 ? y.x : e % 4 == 1 ? y.y : e % 4 == 2 ? y.z : y.w;
-        if (e < rows) sums[j] = fmaf(power2((v - st.x) * kLog2e), st.y, sums[j]);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kScoreSlots / kScoreThreads; ++j) {
-    const int slot = slot0 + threadIdx.x + j * kScoreThreads;
-    if (slot < length) scores[slot] += sums[j];
-  }
+  kv4_output<H, QF32>(p, nullptr, b, i, head, b * per + in_b, r & 7, d, top, sum, acc);
 }
 
 // CTAs of a launch: one per SM, fewer when even full caches leave some without a tile, more where the pairs are so many that
@@ -1143,14 +1199,13 @@ cudaError_t launch_tensor(const Kv4Sdpa& p, cudaStream_t s) {
   }
   cudaError_t e = launch_chained(kv4_sdpa_kernel<H, BLOCK, QF32>, dim3(ctas), dim3(T::kThreads), (size_t)T::kSmem, s, p, stats, logits);
   if (e != cudaSuccess) return e;
-  if (pairs > ctas || tiles_of(p.cache.s) > 4 * T::kWarps) {  // (else every pair is a CTA's: kv4_cut)
-    int part_log2 = 0;  // few rows are cut by channels too: their records are many
-    while (part_log2 < 2 && ((long long)p.cache.b * p.n * p.t << part_log2) < 2 * device_sm_count()) ++part_log2;
-    e = launch_chained(kv4_merge_kernel<H, QF32>, dim3((p.n * p.t) << part_log2, p.cache.b), dim3(kMergeThreads), 0, s, p, ctas, part_log2, stats);
-    if (e != cudaSuccess) return e;
-  }
-  if (!p.scores) return cudaSuccess;
-  return launch_chained(kv4_scores_kernel, dim3((p.cache.s + kScoreSlots - 1) / kScoreSlots, p.cache.nkv, p.cache.b), dim3(kScoreThreads), 0, s, p,
+  const bool merge = pairs > ctas || tiles_of(p.cache.s) > 4 * T::kWarps;  // (else every pair is a CTA's: kv4_cut)
+  int part_log2 = 0;  // few rows are cut by channels too: their records are many
+  while (part_log2 < 2 && ((long long)p.cache.b * p.n * p.t << part_log2) < 2 * device_sm_count()) ++part_log2;
+  const int merge_ctas = merge ? (p.n * p.t) << part_log2 : 0;
+  const int score_ctas = p.scores ? (p.cache.s + kScoreSlots - 1) / kScoreSlots * p.cache.nkv : 0;
+  if (merge_ctas + score_ctas == 0) return cudaSuccess;
+  return launch_chained(kv4_merge_kernel<H, QF32>, dim3(merge_ctas + score_ctas, p.cache.b), dim3(kMergeThreads), 0, s, p, ctas, merge_ctas, part_log2,
                         (const float2*)stats, (const float*)logits);
 }
 template <int H, int BLOCK>
