@@ -34,9 +34,10 @@ __device__ __forceinline__ uint32_t operator/(uint32_t n, const Divisor& by) { r
 // is off by 2^-22 of itself at most, so 15 y by 3.6e-6; only what comes within 1e-5 of a border is looked at again, in 64
 // bits where difference and border are exact.
 //
-// Memory-bound by its bytes, and nearly by instruction issue: 67 M elements at 36 T lane operations per second leave 12
-// operations for each in the time that HBM takes. So 16 channels per thread (block / 16 neighbouring lanes have one block),
-// the minimum and the negated maximum of fp16 rows as one pair of halves, nibbles put together by fused products.
+// Memory-bound by its bytes, but really by instruction issue: 67 M elements at 36 T lane operations per second leave 12
+// operations for each in the time that HBM takes, and it has 19. So 16 channels per thread (block / 16 neighbouring lanes have
+// one block), the minimum and the negated maximum of fp16 rows as one pair of halves, nibbles put together by fused products.
+// 16 x 8192 rows of 256 in fp16: 53 us of the 26 that their bytes take (issue slots 75 % busy); 16 x 4096 in float32 32 of 23.
 __device__ __forceinline__ float nearest_float(float n, float x, float least, float scale) {
   const double d = (double)x - (double)least;
   const float below = n * scale > (float)d ? n - 1.0f : n;  // the border lies above it
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append
 
 // ---- reading back ----------------------------------------------------------------------------------------
 // A thread takes two words of nibbles, 256 apart, so that a warp's stores are whole lines. fp16 values are fused products
-// of halves: one rounding.
+// of halves: one rounding. Bound by HBM: 16 x 8192 rows of 256 as fp16 29.3 us (26 for the bytes), 16 x 4096 as float32 35 (23).
 template <bool F32>
 __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Read p, const uint32_t items, const Divisor per_token, const int words_log2) {
   pdl_enter();
@@ -279,7 +280,9 @@ struct EvictShared {
 // In place, rows move down (slot kept[j] >= j), so a pass of the cluster reads the rows of as many destinations as fit
 // into its CTAs' shared memory, waits for the cluster, and writes them: what it overwrites has been read in this pass or
 // an earlier one.
-// Bound by round trips: (MEASURED)
+// Bound by round trips and barriers, not by its bytes: 16 pairs of 4352 slots cut to 4096 in place 20.5 us (the kept rows,
+// read and written, are 5.8 us of HBM time; clusters of 6, 96 SMs), of which the three counts take 6 us, the list 3 us and the
+// rows, one pass of up to 700 per CTA, 7 us; 32 pairs of 32768 to 2048 into another cache 20.8 us on clusters of 4.
 __global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Evict p, const int in_place, const int row_log2, const int smem_bytes) {
   extern __shared__ __align__(16) uint8_t rows_smem[];
   __shared__ EvictShared sh;

@@ -356,9 +356,12 @@ __device__ __forceinline__ uint32_t piece_at(int row, int c) {
   return (uint32_t)(line * 128 + ((pos ^ x) << 4));
 }
 
-// Key nibbles become fp16 operands by a mask alone: in the low bits of a half, nibble u is the subnormal number u 2^-24,
+// For fp16 queries key nibbles become operands by a mask alone: in the low bits of a half, nibble u is the subnormal number u 2^-24,
 // one place up u 2^-20. So a word of eight nibbles is four pairs after one shift and four masks, exactly; the factor 16
-// between the two kinds goes into the queries of those channels, 2^-24 into the logits' factor.
+// between the two kinds goes into the queries of those channels, 2^-24 into the logits' factor. For float32 queries they are
+// centred like the values' (8 x scale joins the least value's factor), and the queries' low halves come first, while the sums
+// are small: the products truncate (weights' error against 64 bits, 2000 tokens of 128: 1.05e-6 -> 3.7e-7, where torch's float32
+// has 1.2e-6; + 0.3 us at 4 x 2000).
 // Value nibbles are centred, u - 8, by way of the exponents that make a nibble's place the unit (1024) or an eighth of it
 // (64): sums of weights times values that are all positive lose to the tensor core's truncation (float32 outputs were
 // 3e-5 off; 8 x scale joins the least value instead). For fp16 queries that costs nothing but a mask: a nibble as the
@@ -561,7 +564,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 
     // Queries: thread (g, t) makes row g's elements at its words of a key, as the B operand: channels 0, 4 | 2, 6 of a word
     // meet low nibbles, 1, 5 | 3, 7 high ones. They are scaled by a power of two that brings the row's largest to 2^5 ..
-    // 2^6: dividing by 16 then loses nothing above 2^-26 of it, and a float32 query is two fp16 numbers to 22 bits.
+    // 2^6: dividing by 16 (fp16 queries) then loses nothing above 2^-26 of it, and a float32 query is two fp16 numbers to 22 bits.
     // They are kept in shared memory, [piece][lane][4 words] (and again for the low halves).
     const uint32_t query_at = part_at + lane * 16;
     float q_sum[G][2], factor[2];  // of the rows 2 t and 2 t + 1 (the products' columns)
@@ -598,11 +601,10 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
           uint32_t high[4], low[4];
           if constexpr (QF32) {
             const uint4 lo = q_bits[2 * sl], hi = q_bits[2 * sl + 1];
-            const float even = scale_up, odd = scale_up * 0.0625f;
-            split_halves(__uint_as_float(lo.x) * even, __uint_as_float(hi.x) * even, high[0], low[0]);
-            split_halves(__uint_as_float(lo.z) * even, __uint_as_float(hi.z) * even, high[1], low[1]);
-            split_halves(__uint_as_float(lo.y) * odd, __uint_as_float(hi.y) * odd, high[2], low[2]);
-            split_halves(__uint_as_float(lo.w) * odd, __uint_as_float(hi.w) * odd, high[3], low[3]);
+            split_halves(__uint_as_float(lo.x) * scale_up, __uint_as_float(hi.x) * scale_up, high[0], low[0]);
+            split_halves(__uint_as_float(lo.z) * scale_up, __uint_as_float(hi.z) * scale_up, high[1], low[1]);
+            split_halves(__uint_as_float(lo.y) * scale_up, __uint_as_float(hi.y) * scale_up, high[2], low[2]);
+            split_halves(__uint_as_float(lo.w) * scale_up, __uint_as_float(hi.w) * scale_up, high[3], low[3]);
             sts128(query_at + (P + sl) * 512, low);
           } else {
             uint32_t v[4] = {q_bits[sl].x, q_bits[sl].y, q_bits[sl].z, q_bits[sl].w};
@@ -623,18 +625,18 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
           // the blocks' sums: products with ones (and sixteens)
 #pragma unroll
           for (int odd = 0; odd < 2; ++odd) {
-            const uint32_t ones = odd ? 0x4c004c00u : 0x3c003c00u;
+            const uint32_t ones = odd && !QF32 ? 0x4c004c00u : 0x3c003c00u;
             product(sum, ones, ones, ones, ones, high[2 * odd], high[2 * odd + 1]);
             if constexpr (QF32) product(sum, ones, ones, ones, ones, low[2 * odd], low[2 * odd + 1]);
           }
         }
-        q_sum[gr][0] = sum[0] * 0x1p-24f;
-        q_sum[gr][1] = sum[1] * 0x1p-24f;
+        q_sum[gr][0] = QF32 ? sum[0] : sum[0] * 0x1p-24f;
+        q_sum[gr][1] = QF32 ? sum[1] : sum[1] * 0x1p-24f;
       }
       const float f = scale_down * p.scale;
       // (in two steps: 2^24 times a small scale stays within fp32 either way)
-      factor[0] = __shfl_sync(0xffffffffu, f, 8 * t) * 0x1p24f;
-      factor[1] = __shfl_sync(0xffffffffu, f, 8 * t + 4) * 0x1p24f;
+      factor[0] = __shfl_sync(0xffffffffu, f, 8 * t) * (QF32 ? 1.0f : 0x1p24f);
+      factor[1] = __shfl_sync(0xffffffffu, f, 8 * t + 4) * (QF32 ? 1.0f : 0x1p24f);
     }
     int limit[2];
     const float* mask[2];
@@ -684,31 +686,37 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 #pragma unroll
         for (int i = 0; i < kAtOnce; i += 2) load_matrices(at + (matrix_at ^ (uint32_t)((i0 + i) * 16)), words[i / 2]);
         float acc[kChains][kApart][4];  // (few chains: low and high nibbles apart)
+// (the low halves of float32 queries first, while the sums are small: the tensor core truncates)
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          uint32_t qs[kChains][4], qls[QF32 ? kChains : 1][4];
+        for (int half = QF32 ? 1 : 0; half >= 0; --half) {
 #pragma unroll
-          for (int c = 0; c < kChains; ++c) {
-            lds128(query_at + (i0 + c * kPer + j) * 512, qs[c]);
-            if constexpr (QF32) lds128(query_at + (P + i0 + c * kPer + j) * 512, qls[c]);
-          }
+          for (int j = 0; j < kPer; ++j) {
+            uint32_t qs[kChains][4];
 #pragma unroll
-          for (int odd = 0; odd < 2; ++odd) {
+            for (int c = 0; c < kChains; ++c) lds128(query_at + (half * P + i0 + c * kPer + j) * 512, qs[c]);
 #pragma unroll
-            for (int c = 0; c < kChains; ++c) {
-              const int i = c * kPer + j;
-              const uint32_t (&q)[4] = qs[c];
-              const uint32_t (&ql)[4] = qls[QF32 ? c : 0];
-              const uint32_t wa = words[i / 2][2 * (i & 1)], wb = words[i / 2][2 * (i & 1) + 1];
-              const uint32_t keep = odd ? kHighNibbles : kLowNibbles;
-              const uint32_t a0 = wa & keep, a1 = wb & keep, a2 = (wa >> 8) & keep, a3 = (wb >> 8) & keep;
-              float (&to_acc)[4] = acc[c][odd % kApart];
-              if (j == 0 && odd < kApart) {
-                first_product(to_acc, a0, a1, a2, a3, q[2 * odd], q[2 * odd + 1]);
-              } else {
-                product(to_acc, a0, a1, a2, a3, q[2 * odd], q[2 * odd + 1]);
+            for (int odd = 0; odd < 2; ++odd) {
+#pragma unroll
+              for (int c = 0; c < kChains; ++c) {
+                const int i = c * kPer + j;
+                const uint32_t (&q)[4] = qs[c];
+                const uint32_t wa = words[i / 2][2 * (i & 1)], wb = words[i / 2][2 * (i & 1) + 1];
+                uint32_t k[4] = {wa, wb, wa >> 8, wb >> 8};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if constexpr (QF32) {
+                    k[e] = odd ? centred.high(k[e]) : centred.low(k[e]);
+                  } else {
+                    k[e] &= odd ? kHighNibbles : kLowNibbles;
+                  }
+                }
+                float (&to_acc)[4] = acc[c][odd % kApart];
+                if (j == 0 && odd < kApart && half == (QF32 ? 1 : 0)) {
+                  first_product(to_acc, k[0], k[1], k[2], k[3], q[2 * odd], q[2 * odd + 1]);
+                } else {
+                  product(to_acc, k[0], k[1], k[2], k[3], q[2 * odd], q[2 * odd + 1]);
+                }
               }
-              if constexpr (QF32) product(to_acc, a0, a1, a2, a3, ql[2 * odd], ql[2 * odd + 1]);
             }
           }
         }
@@ -720,7 +728,8 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = e < 2 ? fa : fb;
-            x[e] = fmaf(f.x, kApart == 2 ? acc[c][0][e] + acc[c][kApart - 1][e] : acc[c][0][e], fmaf(f.y, q_sum[gr][e & 1], x[e]));
+            x[e] = fmaf(f.x, kApart == 2 ? acc[c][0][e] + acc[c][kApart - 1][e] : acc[c][0][e],
+                        fmaf(QF32 ? fmaf(8.0f, f.x, f.y) : f.y, q_sum[gr][e & 1], x[e]));
           }
         }
       }
