@@ -280,9 +280,9 @@ struct EvictShared {
 // In place, rows move down (slot kept[j] >= j), so a pass of the cluster reads the rows of as many destinations as fit
 // into its CTAs' shared memory, waits for the cluster, and writes them: what it overwrites has been read in this pass or
 // an earlier one.
-// Bound by round trips and barriers, not by its bytes: 16 pairs of 4352 slots cut to 4096 in place 20.5 us (the kept rows,
-// read and written, are 5.8 us of HBM time; clusters of 6, 96 SMs), of which the three counts take 6 us, the list 3 us and the
-// rows, one pass of up to 700 per CTA, 7 us; 32 pairs of 32768 to 2048 into another cache 20.8 us on clusters of 4.
+// Bound by round trips and barriers, not by its bytes. 16 pairs of 4352 slots cut to 4096 in place: 19.0 us on clusters of 6 (the
+// kept rows, read and written, are 5.8 us of HBM time); the counts end at 5.7 us, the list at 8, the rows' reading at 13.5.
+// 32 pairs of 32768 to 2048 into another cache: 23.5 us on clusters of 4, counts to 11 us, list to 14.5.
 __global__ void __launch_bounds__(kEvictThreads, 2) kv4_evict_kernel(const Kv4Evict p, const int in_place, const int row_log2, const int smem_bytes) {
   extern __shared__ __align__(16) uint8_t rows_smem[];
   __shared__ EvictShared sh;
