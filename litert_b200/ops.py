@@ -63,6 +63,7 @@ class Workspace:
         if self.sdpa is None or self.sdpa.numel() < need:
             if self.sdpa is not None:
                 self.outgrown.append(self.sdpa)
+                need = max(need, 2 * self.sdpa.numel())  # (all that is kept stays below the one in use)
             self.sdpa = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self.sdpa
 
