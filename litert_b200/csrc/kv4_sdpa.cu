@@ -364,12 +364,10 @@ __device__ __forceinline__ uint32_t piece_at(int row, int c) {
 // has 1.2e-6; + 0.3 us at 4 x 2000).
 // Value nibbles are centred, u - 8, by way of the exponents that make a nibble's place the unit (1024) or an eighth of it
 // (64): sums of weights times values that are all positive lose to the tensor core's truncation (float32 outputs were
-// 3e-5 off; 8 x scale joins the least value instead). For fp16 queries that costs nothing but a mask: a nibble as the
-// subnormal number again for half of the slots, u w, and its complement with the other sign for the other half,
-// -(15 - u) w, are a sum about zero too; - 8 w and + 7 w, which are missing, are one more product per block of channels.
-// A weight times a value scale is one fp16 number for fp16 queries, and two, 22 bits, for float32 ones: one rounding is off
-// by 2^-12 on average, times |u - 8| x scale (16 sequences of up to 8192, error against 64 bits: 2.8e-4 instead of 2.1e-4,
-// which is the output's own rounding; 64 x 32768: 90.0 -> 83.7 us, and 78.1 with the complements).
+// 3e-5 off; 8 x scale joins the least value instead).
+// A weight times a value scale is two fp16 numbers, 22 bits, for either type of query. As one number it is off by 2^-12 on
+// average, times |u - 8| x scale: outputs 2.8e-4 off 64 bits where an fp16 output's own rounding is 2.1e-4. The second number's
+// products cost 64 x 32768 of 8 heads x 256 84 .. 89 -> 88 .. 93 us, 16 x 8192 15.8 .. 16.5 -> 16.3 .. 16.5.
 constexpr uint32_t kLowNibbles = 0x000f000fu, kHighNibbles = 0x00f000f0u;
 __device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -415,10 +413,6 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
   constexpr int P = H / 32;         // 16-byte pieces of a row
   constexpr int kPer = BLOCK / 32;  // of them in a block
   constexpr int kWarps = T::kWarps;
-  // Half of a tile's slots with the nibbles' complements (see Centred): of 8 warps with 250 registers each (32 sequences of
-  // up to 16384, 8 heads x 256, blocks of 64: 31.4 -> 29.9 us; blocks of 32: 35.7 -> 35.0). The 16 warps of the smaller heads have no
-  // registers for its sums (4 KV heads x 64, blocks of 32: 40.0 -> 41.8; 2 x 128: 37.3 -> 39.2).
-  constexpr bool kComplement = !QF32 && H == 256;
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
   __shared__ int s_pair[kWarps];                       // whose the warps' states are
@@ -661,11 +655,9 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     float* logits = logits_ws ? logits_ws + (size_t)pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
 
     // outputs: of piece i and its channels 4 g + {0, 1} and 4 g + {2, 3}, rows 2 t and 2 t + 1
-    float o[P][2][4], least_sum[G], centre[kComplement ? G : 1][4];
+    float o[P][2][4], least_sum[G];
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) least_sum[gr] = 0.0f;
-#pragma unroll
-    for (int gr = 0; gr < (kComplement ? G : 1); ++gr) centre[gr][0] = centre[gr][1] = centre[gr][2] = centre[gr][3] = 0.0f;
 #pragma unroll
     for (int i = 0; i < P; ++i)
 #pragma unroll
@@ -817,13 +809,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
         l_run[0] *= alpha[0];
         l_run[1] *= alpha[1];
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          least_sum[gr] *= mine_alpha;
-          if constexpr (kComplement) {
-            centre[gr][0] *= alpha[0];
-            centre[gr][1] *= alpha[1];
-          }
-        }
+        for (int gr = 0; gr < G; ++gr) least_sum[gr] *= mine_alpha;
 #pragma unroll
         for (int i = 0; i < 2 * P; ++i)
 #pragma unroll
@@ -859,39 +845,27 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
           for (int j = 0; j < 4; ++j) {
             const uint32_t bits = lds32(pairs_at + T::kPairBytes + (uint32_t)(((2 * t + (j & 1) + 8 * (j >> 1)) * G + gr) * 4));
             const float2 f = pair_floats(bits);
-            ps[j] = kComplement && j >= 2 ? -pw[j] * f.x : pw[j] * f.x;
+            ps[j] = pw[j] * f.x;
             if (careful && pw[j] == 0.0f) {
               ps[j] = 0.0f;
             } else {
               least_sum[gr] = fmaf(pw[j], fmaf(8.0f, f.x, f.y), least_sum[gr]);
             }
           }
-          if constexpr (QF32) {
-            split_halves(ps[0], ps[1], high[0], low[0]);
-            split_halves(ps[2], ps[3], high[1], low[1]);
-          } else {
-            high[0] = halves(ps[0], ps[1]);
-            high[1] = halves(ps[2], ps[3]);
-            if constexpr (kComplement) product(centre[gr], 0xc800c800u, 0xc800c800u, 0xc700c700u, 0xc700c700u, high[0], high[1]);  // -8, -7
-          }
+          split_halves(ps[0], ps[1], high[0], low[0]);
+          split_halves(ps[2], ps[3], high[1], low[1]);
         }
         if (i % 2 == 0) load_matrices_transposed(at + T::kNibbleBytes + (matrix_at ^ (uint32_t)(i * 16)), words);
         uint32_t e[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t a = j ? words[2 * (i & 1)] >> 8 : words[2 * (i & 1)], c = j ? words[2 * (i & 1) + 1] >> 8 : words[2 * (i & 1) + 1];
-          if constexpr (kComplement) {
-            e[j][0] = a & kLowNibbles, e[j][1] = a & kHighNibbles, e[j][2] = ~c & kLowNibbles, e[j][3] = ~c & kHighNibbles;
-          } else {
-            e[j][0] = centred.low(a), e[j][1] = centred.high(a), e[j][2] = centred.low(c), e[j][3] = centred.high(c);
-          }
+          e[j][0] = centred.low(a), e[j][1] = centred.high(a), e[j][2] = centred.low(c), e[j][3] = centred.high(c);
         }
         product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], high[0], high[1]);
         product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], high[0], high[1]);
-        if constexpr (QF32) {
-          product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], low[0], low[1]);
-          product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], low[0], low[1]);
-        }
+        product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], low[0], low[1]);
+        product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], low[0], low[1]);
       }
       at = next_at;
 #pragma unroll
@@ -901,7 +875,6 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     cp_async_wait<0>();
 
     // -- the warp's state, as a record: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
-    constexpr float kLowUnits = kComplement ? 0x1p24f : 1.0f, kHighUnits = kComplement ? 0x1p20f : 1.0f;
     const float from_units = __int_as_float((int)(104 + exponent) << 23);  // 2^(exponent - 23)
     float* state = reinterpret_cast<float*>(smem + w * T::kWarpBytes);
 #pragma unroll
@@ -914,18 +887,14 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
       float sum = least_sum[gr];
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      float least[2] = {__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4)};
-      if constexpr (kComplement) {
-        least[0] += centre[gr][0];
-        least[1] += centre[gr][1];
-      }
+      const float least[2] = {__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4)};
 #pragma unroll
       for (int i = gr * kPer; i < (gr + 1) * kPer; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<float4*>(state + (2 * t + e) * T::kRec + i * 32 + g * 4) =
-              make_float4(fmaf(o[i][0][e], kLowUnits, least[e]) * from_units, fmaf(o[i][0][2 + e], kHighUnits, least[e]) * from_units,
-                          fmaf(o[i][1][e], kLowUnits, least[e]) * from_units, fmaf(o[i][1][2 + e], kHighUnits, least[e]) * from_units);
+              make_float4((o[i][0][e] + least[e]) * from_units, (o[i][0][2 + e] + least[e]) * from_units,
+                          (o[i][1][e] + least[e]) * from_units, (o[i][1][2 + e] + least[e]) * from_units);
     }
     if (g < 2) {
       s_m[w][2 * t + g] = g ? m_run[1] : m_run[0];
