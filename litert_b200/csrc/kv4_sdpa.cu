@@ -8,6 +8,8 @@
 // Products of a nibble and an fp16 number are exact and are added in fp32.
 #include <math_constants.h>
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.h"
@@ -367,7 +369,15 @@ __device__ __forceinline__ uint32_t piece_at(int row, int c) {
 // 3e-5 off; 8 x scale joins the least value instead).
 // A weight times a value scale is two fp16 numbers, 22 bits, for either type of query. As one number it is off by 2^-12 on
 // average, times |u - 8| x scale: outputs 2.8e-4 off 64 bits where an fp16 output's own rounding is 2.1e-4. The second number's
-// products cost 64 x 32768 of 8 heads x 256 84 .. 89 -> 88 .. 93 us, 16 x 8192 15.8 .. 16.5 -> 16.3 .. 16.5.
+// products cost 64 x 32768 of 8 heads x 256 71.7 -> 82.1 us replayed, 16 x 8192 15.5 -> 16.2.
+// What a second number leaves is 2^-25 at least, fp16's last place, however small the product. So a row's weights are counted in
+// units of 2^-units such that the largest product of a weight and a scale so far lies in 2^9 .. 2^10, up to 60000 before that is
+// put right: rescaling the outputs at every new maximum would happen in most tiles while a warp has seen few. The unit goes by
+// what slots contribute, not by their scales alone, so hidden slots, and slots or tiles that end up without weight, do not coarsen
+// the others. A scale of zero counts as kLeastScale, which keeps the weights themselves within fp32.
+// Beside a unit of the largest scale: 64 x 32768 82.1 -> 83.5 us replayed, 16 x 8192 16.2 -> 16.5.
+constexpr float kMostOperand = 60000.0f, kLeastScale = 0x1p-40f, kMostUnits = 49.0f;
+constexpr int kUnitBits = 9;
 constexpr uint32_t kLowNibbles = 0x000f000fu, kHighNibbles = 0x00f000f0u;
 __device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -662,8 +672,9 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     for (int i = 0; i < P; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][0][e] = o[i][1][e] = 0.0f;
-    float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, m_use[2] = {0.0f, 0.0f}, l_run[2] = {0.0f, 0.0f};
-    uint32_t exponent = 1;  // fp16 exponent field of the largest value scale so far: weights are in units of 2^(exponent - 23)
+    // the rows' weights are e^(x - m_run) in units of 2^-units (integers; see kMostUnits). The first x that is a number makes a
+    // weight of infinity, or, at the type's lowest value, of one: m_run need not be the largest x.
+    float m_run[2] = {-FLT_MAX, -FLT_MAX}, l_run[2] = {0.0f, 0.0f}, units[2] = {kMostUnits, kMostUnits};
 
     const Centred centred;
     // The logits of a tile's slots g and g + 8, rows 2 t and 2 t + 1, without factor, cap and mask.
@@ -755,6 +766,26 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
       }
 
     };
+    // A tile's largest value scales of this thread's slots g and g + 8, compared as halves by the threads that share them, and
+    // whether any is infinite or NaN (or a least value is). Found a tile ahead of their use.
+    float largest[2];
+    bool infinite;
+    auto find_largest = [&](uint32_t at) {
+      uint32_t scales = 0, either = 0;
+#pragma unroll
+      for (int j = 0; j < (G + 3) / 4; ++j) {
+        const uint32_t from = at + 2 * T::kNibbleBytes + T::kPairBytes + (uint32_t)((g * G + (t + 4 * j) % G) * 4);
+        const uint32_t a = lds32(from) & 0x7fff7fffu, c = lds32(from + 8 * G * 4) & 0x7fff7fffu;
+        scales = __vmaxu2(scales, __byte_perm(a, c, 0x5410));
+        either = __vmaxu2(either, __vmaxu2(a, c));
+      }
+#pragma unroll
+      for (int d = 1; d < (G < 4 ? G : 4); d <<= 1) scales = __vmaxu2(scales, __shfl_xor_sync(0xffffffffu, scales, d));
+      const float2 f = pair_floats(scales);
+      largest[0] = fmaxf(f.x, kLeastScale);
+      largest[1] = fmaxf(f.y, kLeastScale);
+      infinite = guard && __any_sync(0xffffffffu, __vcmpgeu2(either, 0x7c007c00u) != 0u);
+    };
     // A tile's weights and outputs stand in one block of code with the next tile's products with the queries, so that the
     // chains of the one fill the waits of the other.
     uint32_t at = ring;
@@ -763,6 +794,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     float x[4];
     cp_async_wait<T::kStages - 2>();
     __syncwarp();
+    find_largest(at);
     dot(at, x);
     finish(first, x);
 #pragma unroll 1
@@ -772,40 +804,38 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
       request();
       const uint32_t pairs_at = at + 2 * T::kNibbleBytes, next_at = at + T::kBytes == ring + T::kStages * T::kBytes ? ring : at + T::kBytes;
       // -- running maximum and unit; both rarely change --
-      // A weight may exceed 1 by e^kSlack: rescaling the outputs at every new maximum would happen in most tiles while a
-      // warp has seen few. The largest value scale of the tile: pairs compared as halves.
-      constexpr float kSlack = 4.0f;
-      uint32_t largest = 0;
+      float pr[4];
+      auto weigh = [&]() {
 #pragma unroll
-      for (int j = 0; j < kPairCopies; ++j) {
-        const int e = (lane + 32 * j) % (kSlots * G);  // (H = 64: every pair twice)
-        largest = __vmaxu2(largest, lds32(pairs_at + T::kPairBytes + (uint32_t)e * 4) & 0x7fff7fffu);
-      }
-      const uint32_t now = max(exponent, min(__reduce_max_sync(0xffffffffu, largest & 0xffffu) >> 10, 30u));
-      // slots that some row does not see may hold anything: their weights are zero, and so must be their share
-      const bool careful = guard && __any_sync(0xffffffffu, __vcmpgeu2(largest, 0x7c007c00u) != 0u);
-      const float tops[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-      const bool grows = tops[0] > m_run[0] + kSlack || tops[1] > m_run[1] + kSlack;
-      if (__any_sync(0xffffffffu, grows) || now != exponent) {
+        for (int e = 0; e < 4; ++e) pr[e] = power2(fmaf(x[e] - m_run[e & 1], kLog2e, units[e & 1]));
+      };
+      weigh();
+      // (no maximum is NaN)
+      const float operand = fmaxf(fmaxf(pr[0], pr[1]) * largest[0], fmaxf(pr[2], pr[3]) * largest[1]);
+      if (__any_sync(0xffffffffu, operand > kMostOperand)) {
         float alpha[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = tops[e];
+          float top = fmaxf(x[e], x[2 + e]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           top = fmaxf(m_run[e], top);
-          const float use = top == -CUDART_INF_F ? 0.0f : top;
-          alpha[e] = m_run[e] == -CUDART_INF_F ? 0.0f : power2((m_run[e] - use) * kLog2e);
+          alpha[e] = power2((m_run[e] - top) * kLog2e);
           m_run[e] = top;
-          m_use[e] = use;
+          // the largest product so far: of this tile, and by its unit of those before
+          float most = fmaxf(fmaxf(power2((x[e] - top) * kLog2e) * largest[0], power2((x[2 + e] - top) * kLog2e) * largest[1]),
+                             alpha[e] * __int_as_float((127 + kUnitBits - (int)units[e]) << 23));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+          // (a weight is 1 at most here and a finite scale below 2^16, so -6 at least; with an infinite one nothing stays finite)
+          const float now = fmaxf(fminf((float)(127 + kUnitBits - (__float_as_int(most) >> 23)), kMostUnits), -6.0f);
+          alpha[e] *= __int_as_float((127 + (int)(now - units[e])) << 23);
+          units[e] = now;
         }
-        const float shrink = __int_as_float((int)(127 + exponent - now) << 23);
-        exponent = now;
+        weigh();
         // (a least-value sum belongs to row g: its factor is with the threads of column g)
         const float even = __shfl_sync(0xffffffffu, alpha[0], g >> 1), odd = __shfl_sync(0xffffffffu, alpha[1], g >> 1);
-        const float mine_alpha = ((g & 1) ? odd : even) * shrink;
-        alpha[0] *= shrink;
-        alpha[1] *= shrink;
+        const float mine_alpha = (g & 1) ? odd : even;
         l_run[0] *= alpha[0];
         l_run[1] *= alpha[1];
 #pragma unroll
@@ -815,13 +845,9 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i >> 1][i & 1][e] *= alpha[e & 1];
       }
-      // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9, in units of the value scales
+      // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9
       float pw[4];
       {
-        const float to_units = 23.0f - (float)exponent;
-        float pr[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pr[e] = power2(fmaf(x[e] - m_use[e & 1], kLog2e, to_units));
         l_run[0] += pr[0] + pr[2];
         l_run[1] += pr[1] + pr[3];
 #pragma unroll
@@ -833,7 +859,10 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
         }
       }
       float y[4];
-      dot(next_at, y);  // (behind the last tile: of whatever lies there, and not used)
+      // slots that some row does not see may hold anything: their weights are zero, and so must be their share
+      const bool careful = infinite;
+      find_largest(next_at);  // (behind the last tile: of whatever lies there, and not used; so are the logits)
+      dot(next_at, y);
       // -- outputs: channels by slots times slots by rows; a weight is two fp16 numbers --
       uint32_t high[2], low[2], words[4];
 #pragma unroll
@@ -875,7 +904,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     cp_async_wait<0>();
 
     // -- the warp's state, as a record: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
-    const float from_units = __int_as_float((int)(104 + exponent) << 23);  // 2^(exponent - 23)
+    const float from_units[2] = {__int_as_float((127 - (int)units[0]) << 23), __int_as_float((127 - (int)units[1]) << 23)};
     float* state = reinterpret_cast<float*>(smem + w * T::kWarpBytes);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -893,12 +922,12 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<float4*>(state + (2 * t + e) * T::kRec + i * 32 + g * 4) =
-              make_float4((o[i][0][e] + least[e]) * from_units, (o[i][0][2 + e] + least[e]) * from_units,
-                          (o[i][1][e] + least[e]) * from_units, (o[i][1][2 + e] + least[e]) * from_units);
+              make_float4((o[i][0][e] + least[e]) * from_units[e], (o[i][0][2 + e] + least[e]) * from_units[e],
+                          (o[i][1][e] + least[e]) * from_units[e], (o[i][1][2 + e] + least[e]) * from_units[e]);
     }
     if (g < 2) {
       s_m[w][2 * t + g] = g ? m_run[1] : m_run[0];
-      s_l[w][2 * t + g] = (g ? l_run[1] : l_run[0]) * from_units;
+      s_l[w][2 * t + g] = g ? l_run[1] * from_units[1] : l_run[0] * from_units[0];
     }
   } else if (lane < 8) {  // (no slot)
     s_m[w][lane] = -CUDART_INF_F;

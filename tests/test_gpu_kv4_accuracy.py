@@ -170,3 +170,107 @@ def test_the_measure_sees_one_rounding(ops):
         assert near(want.to(dtype), want) is None
         for wrong in (once, coarse, mixed, torch.zeros_like(want)):
             assert near(wrong.to(dtype), want) is not None
+
+
+HEADS = [(8, 1, 256, 64), (8, 1, 256, 32), (8, 2, 128, 32), (4, 4, 64, 64), (6, 2, 64, 32), (6, 2, 96, 32)]
+
+
+def dominated(q, cache, slot, above):
+    """A slot's keys are those that every query of the first token has a logit of about `above` with."""
+    b, t, n, h = q.shape
+    nkv = cache[0].shape[2]
+    mean = q[:, 0].float().reshape(b, nkv, n // nkv, h).mean(2)
+    mean = mean * (above * math.sqrt(h) / mean.square().sum(-1, keepdim=True))
+    cache[0][:, slot], cache[2][:, slot] = quantized(mean, h // cache[2].shape[3])
+
+
+@pytest.mark.parametrize("layout", HEADS)
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("hidden", ["nan", "inf", "large"])
+def test_hidden_slots_do_not_coarsen_the_others(ops, ws, layout, f32, hidden):
+    """Slots behind -inf masks (a prefix; single ones; NaN, infinities, or the largest scales in them) beside small values and one
+    slot of most of the weight: as exact as over a cache that has zeros there. So are slots that a mask of -1e30, the type's lowest
+    value, or their own logits leave without weight, where what they hold is finite."""
+    n, nkv, h, block = layout
+    b, s, t = 4, 3000, 2
+    cache, g = filled(ops, h, b, s, nkv, h, block)
+    q = torch.randn((b, t, n, h), generator=g, device="cuda")
+    q = q if f32 else q.half()
+    cache[3].mul_(0.01)
+    dominated(q, cache, 1500, 8.0)
+    off = torch.zeros((b, s), dtype=torch.bool, device="cuda")
+    off[0, :700] = True
+    off[1, 5::16] = True
+    off[2, 701:1400] = True
+    off[3, :1400] = True
+    off[3, 1700:] = True
+    for i in (2, 3):
+        clean = cache[i].clone()
+        if hidden == "large":
+            cache[i][off] = 65504.0
+        else:
+            cache[i][off] = float(hidden)
+        cache[i][~off] = clean[~off]
+    low = torch.finfo(torch.float32).min
+    for value in (-math.inf,) if hidden != "large" else (-math.inf, -1e30, low):
+        mask = torch.where(off, value, torch.zeros((b, s), device="cuda"))[:, None, None].expand(b, 1, t, s).contiguous()
+        plain = [x.clone() for x in cache]
+        for x in plain:
+            x[off] = 0
+        scores = torch.zeros((b, nkv, s), device="cuda")
+        got = ops.sdpa_decode_int4(q, *cache, mask=mask, scores=scores, ws=ws)
+        want, weights = attention64(q, plain, mask=torch.where(off, -math.inf, 0.0)[:, None, None].expand(b, 1, t, s))
+        wrong = near(got, want, 2 * LIMIT)  # (logits up to twice as large as those that LIMIT is for)
+        assert wrong is None, (value, wrong)
+        off_by = ((scores.double() - weights) / weights.clamp(min=1e-30))[weights > 1e-20]
+        assert float(off_by.square().mean().sqrt()) <= 2 * LIMIT
+
+
+@pytest.mark.parametrize("layout", HEADS)
+@pytest.mark.parametrize("f32", [False, True])
+def test_slots_of_no_weight_and_later_drafts_do_not_coarsen_the_others(ops, ws, layout, f32):
+    """Visible slots with the largest scales and a logit 60 below the others; a last draft's own slot with such scales, which
+    earlier queries do not see; a first slot of zeros (scale 0) that has most of the weight."""
+    n, nkv, h, block = layout
+    b, s, t = 3, 1200, 3
+    cache, g = filled(ops, h + 1, b, s, nkv, h, block)
+    q = 0.5 * torch.randn((b, 1, n, h), generator=g, device="cuda").expand(b, t, n, h).contiguous()
+    q[..., 0] = 6.0
+    q = q if f32 else q.half()
+    cache[3].mul_(0.01)
+    far = torch.zeros((nkv, h), device="cuda")
+    far[:, 0] = -10.0 * math.sqrt(h)  # its logit: -60
+    for slot in (3, 17, 600, 900):
+        cache[0][0, slot], cache[2][0, slot] = quantized(far, block)
+        cache[3][0, slot, ..., 0] = 60000.0
+    cache[3][1, s - 1, ..., 0] = 60000.0
+    near_key = torch.zeros((nkv, h), device="cuda")
+    near_key[:, 0] = 2.0 * math.sqrt(h)  # its logit: 12
+    cache[0][2, 0], cache[2][2, 0] = quantized(near_key, block)
+    cache[1][2, 0], cache[3][2, 0] = 0, 0
+    want, _ = attention64(q, cache)
+    got = ops.sdpa_decode_int4(q, *cache, ws=ws)
+    # the logits' terms are up to 12 here, and what LIMIT counts steps of is 4
+    for i, upto in ((0, t), (1, t - 1), (2, t)):
+        wrong = near(got[i, :upto], want[i, :upto], 3 * LIMIT)
+        assert wrong is None, (i, wrong)
+
+
+@pytest.mark.parametrize("h,block", [(256, 64), (128, 32), (64, 32), (96, 32)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_attention_is_exact_over_values_of_any_size(ops, ws, h, block, f32):
+    """Value scales growing, shrinking and mixed by 2^18 along the cache, and by 2^9 between blocks: each block of a row by its own
+    size."""
+    rng = np.random.default_rng(h)
+    b, s = 4, 700
+    cache, g = filled(ops, h + 2, b, s, 1, h, block)
+    size = 2.0 ** np.linspace(-9, 9, s)
+    for i, z in enumerate((size, size[::-1], rng.permutation(size))):
+        cache[3][i] = (cache[3][i].float() * torch.from_numpy(z.copy()).float().cuda()[:, None, None, None]).half()
+    cache[3][3, :, :, 0] *= 2.0 ** -9
+    q = torch.randn((b, 1, 8, h), generator=g, device="cuda")
+    q = q if f32 else q.half()
+    want, _ = attention64(q, cache)
+    got = ops.sdpa_decode_int4(q, *cache, ws=ws)
+    wrong = near(got.unflatten(-1, (-1, block)), want.unflatten(-1, (-1, block)))
+    assert wrong is None, wrong
