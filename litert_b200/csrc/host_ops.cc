@@ -252,6 +252,7 @@ struct Int4Cache {
     const auto n = k.t->sizes(), m = ks.t->sizes();
     if (n[0] != m[0] || n[1] != m[1] || n[2] != m[2] || m[4] != 2 || m[3] == 0 || 2 * n[3] % m[3] != 0) return;
     if (n[0] > INT32_MAX || n[1] > INT32_MAX || n[2] > INT32_MAX || n[3] > 1 << 20) return;
+    if (n[1] == 0 || n[2] == 0 || n[3] == 0) return;  // (refused; heads are divided by KV heads below)
     const at::Device d = k.t->device();
     if (d.index() != c10::cuda::current_device() || v.t->device() != d || ks.t->device() != d || vs.t->device() != d) return;
     b = (int)n[0], s = (int)n[1], nkv = (int)n[2], h = 2 * (int)n[3], block = h / (int)m[3];

@@ -405,6 +405,8 @@ def int4_kv_cache(b, s_max, nkv, h, block=64, device="cuda"):
     [b, s_max, nkv, h / block, 2], block 32 or 64 channels."""
     if block not in (32, 64) or h % block or not 0 < h <= 512:
         raise B200Error("blocks of 32 or 64 channels that divide a head size up to 512")
+    if b < 0 or s_max < 1 or nkv < 1:
+        raise B200Error("a cache has slots and KV heads")
     nibbles = [torch.zeros((b, s_max, nkv, h // 2), dtype=torch.uint8, device=device) for _ in range(2)]
     pairs = [torch.zeros((b, s_max, nkv, h // block, 2), dtype=torch.float16, device=device) for _ in range(2)]
     return (*nibbles, *pairs)
@@ -424,6 +426,8 @@ def _int4_cache(k_cache, v_cache, k_scale, v_scale):
     if v_cache.shape != k_cache.shape or v_scale.shape != k_scale.shape or k_scale.shape[:3] != k_cache.shape[:3] \
             or k_scale.shape[4] != 2 or groups == 0 or 2 * half % groups:
         raise B200Error("the cache's tensors do not belong together")
+    if 0 in (s_max, nkv, half):
+        raise B200Error("a cache has slots, KV heads and channels")
     return b, s_max, nkv, 2 * half, 2 * half // groups
 
 

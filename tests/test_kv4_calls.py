@@ -1,0 +1,46 @@
+"""Calls on the 4-bit cache at the edges of what is accepted: through the extension and through the general path."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from litert_b200 import ops as o
+
+    return o
+
+
+@pytest.fixture(params=["native", "general"])
+def path(request, ops, monkeypatch):
+    from litert_b200 import _lib
+
+    if request.param == "general":
+        monkeypatch.setattr(ops, "_host", _lib._GeneralPath)
+    else:
+        assert ops._host is not _lib._GeneralPath, "the extension is not built"
+    return request.param
+
+
+def test_a_cache_without_slots_heads_or_channels_is_not_made(ops):
+    for shape in ((2, 0, 1, 64), (2, 8, 0, 64), (2, 8, 1, 0), (-1, 8, 1, 64)):
+        with pytest.raises(ops.B200Error):
+            ops.int4_kv_cache(*shape, device="cpu")
+    assert ops.int4_kv_cache(0, 8, 1, 64, device="cpu")[0].shape == (0, 8, 1, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s,nkv,half", [(16, 0, 32), (0, 2, 32), (16, 2, 0)])
+def test_a_cache_without_slots_heads_or_channels_is_refused(ops, path, s, nkv, half):
+    cache = [torch.zeros((2, s, nkv, half), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    cache += [torch.zeros((2, s, nkv, 1, 2), dtype=torch.float16, device="cuda") for _ in range(2)]
+    ws = ops.Workspace("cuda")
+    ws.sdpa_bytes(1 << 20)
+    q, x = (torch.zeros((2, 1, m, 2 * half), device="cuda") for m in (4, nkv))
+    at = torch.zeros(2, dtype=torch.int32, device="cuda")
+    scores = torch.zeros((2, nkv, s), device="cuda")
+    for call in (lambda: ops.sdpa_decode_int4(q, *cache, ws=ws), lambda: ops.sdpa_decode_int4(q, *cache),
+                 lambda: ops.sdpa_decode_int4(q, *cache, scores=scores, ws=ws), lambda: ops.kv_append_int4(x, x, at, *cache),
+                 lambda: ops.kv_read_int4(*cache), lambda: ops.kv_read_int4(*cache, tokens=1), lambda: ops.kv_evict_int4(*cache, scores, at, 1)):
+        with pytest.raises(ops.B200Error):
+            call()
