@@ -27,7 +27,7 @@ bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(
 
 // The cache's shape and tensors. Row indexes of the kernels' grids are 32 bits, offsets 64.
 int check_cache(const char* name, const void* k, const void* v, const void* kp, const void* vp, int b, int s, int nkv, int h, int block) {
-  if (!k || !v || !kp || !vp) return fail(B200_ERR_INVALID_ARGUMENT, "%s: a cache tensor is null", name);
+  if (b != 0 && (!k || !v || !kp || !vp)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: a cache tensor is null", name);
   if (b < 0 || s <= 0 || nkv <= 0 || h <= 0)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: bad cache shape b=%d s=%d nkv=%d h=%d", name, b, s, nkv, h);
   if ((block != 32 && block != 64) || h % block != 0 || h > 512)

@@ -44,3 +44,33 @@ def test_a_cache_without_slots_heads_or_channels_is_refused(ops, path, s, nkv, h
                  lambda: ops.kv_read_int4(*cache), lambda: ops.kv_read_int4(*cache, tokens=1), lambda: ops.kv_evict_int4(*cache, scores, at, 1)):
         with pytest.raises(ops.B200Error):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f32", [False, True])
+def test_no_sequence_is_no_work(ops, path, f32):
+    dtype = torch.float32 if f32 else torch.float16
+    cache, into = ops.int4_kv_cache(0, 16, 2, 64), ops.int4_kv_cache(0, 8, 2, 64)
+    at, scores = torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros((0, 2, 16), device="cuda")
+    x, q = torch.zeros((0, 3, 2, 64), dtype=dtype, device="cuda"), torch.zeros((0, 1, 4, 64), dtype=dtype, device="cuda")
+    ops.kv_append_int4(x, x, at, *cache, counts=at)
+    assert [tuple(y.shape) for y in ops.kv_read_int4(*cache, tokens=5, dtype=dtype)] == [(0, 5, 2, 64)] * 2
+    for ws in (None, ops.Workspace("cuda")):
+        assert ops.sdpa_decode_int4(q, *cache, lengths=at, scores=scores, ws=ws).shape == q.shape
+    for to, slots in ((None, 16), (into, 8)):
+        kept, new, lengths = ops.kv_evict_int4(*cache, scores, at, 4, into=to)
+        assert (kept.shape, new.shape, lengths.shape) == ((0, 2, 4), (0, 2, slots), (0,))
+
+
+def test_no_sequence_needs_no_memory():
+    """The C ABI, where an empty tensor has no address."""
+    from litert_b200 import _lib, build
+
+    build.build_kernels()
+    lib = _lib.load()
+    none = (None,) * 4
+    assert lib.b200_kv4_append(None, None, 0, 0, 0, 0, 0, None, None, 0, 1, 2, 64, 32, 16, *none, None) == 0
+    assert lib.b200_kv4_read(*none, 0, 16, 2, 64, 32, None, None, 1, 0, None, None, None) == 0
+    assert lib.b200_kv4_sdpa(None, *none, None, None, None, None, 0, 1, 4, 2, 64, 32, 16, 0, 0.0, 0.0, None, 0, None) == 0
+    assert lib.b200_kv4_evict(*none, 0, 16, 2, 64, 32, None, None, 4, 0, 0, *none, 16, None, None, None, None) == 0
+    assert lib.b200_kv4_append(None, None, 0, 0, 0, 0, 0, None, None, 0, 1, 2, 80, 32, 16, *none, None) != 0  # (checked all the same)
