@@ -12,6 +12,7 @@
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -78,6 +79,9 @@ struct In {
     return t ? static_cast<T*>(t->data_ptr()) : nullptr;
   }
 };
+
+// A captured call takes the general path, where the workspace notes that a graph holds its buffer.
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
 
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
@@ -225,7 +229,7 @@ PyObject* sdpa_decode(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (q.t->dim() != 4 || k.t->dim() != 4 || q.t->size(1) != 1 || q.t->numel() == 0) Py_RETURN_NONE;
     const int b = (int)q.t->size(0), n = (int)q.t->size(2), h = (int)q.t->size(3);
     const int s_max = (int)k.t->size(1), nkv = (int)k.t->size(2);
-    if ((size_t)ws.t->numel() < b200_sdpa_workspace_bytes(b, n, nkv, h, s_max)) Py_RETURN_NONE;
+    if ((size_t)ws.t->numel() < b200_sdpa_workspace_bytes(b, n, nkv, h, s_max) || capturing()) Py_RETURN_NONE;
     at::Tensor y = result(Py_None, q.t->sizes(), qt, *q.t);
     auto code = [](at::ScalarType t) { return t == at::kHalf ? B200_DTYPE_F16 : t == at::kChar ? B200_DTYPE_I8 : B200_DTYPE_F32; };
     void* s = stream();
@@ -349,7 +353,7 @@ PyObject* sdpa_decode_int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (n % c.nkv != 0 || (mask.t && mask.t->sizes() != at::IntArrayRef{c.b, 1, t, c.s}) ||
         (scores.t && scores.t->sizes() != at::IntArrayRef{c.b, c.nkv, c.s}))
       Py_RETURN_NONE;
-    if ((size_t)ws.t->numel() < b200_kv4_sdpa_workspace_bytes(c.b, t, n, c.nkv, c.h, c.block, c.s, scores.t ? 1 : 0)) Py_RETURN_NONE;
+    if ((size_t)ws.t->numel() < b200_kv4_sdpa_workspace_bytes(c.b, t, n, c.nkv, c.h, c.block, c.s, scores.t ? 1 : 0) || capturing()) Py_RETURN_NONE;
     at::Tensor y = result(Py_None, q.t->sizes(), type, *q.t);
     void* s = stream();
     int rc;

@@ -47,8 +47,12 @@ class Workspace:
         with torch.cuda.device(self.device):
             check(lib.b200_zero_workspace_init(_ptr(self.zero), _stream()))
         self.scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=self.device)
+        self._no_attention_yet()
+
+    def _no_attention_yet(self):
         self.sdpa = None
-        self.outgrown = []  # captured graphs may hold these
+        self.captured = False  # whether a call that was being captured took self.sdpa
+        self.outgrown = []     # those that graphs hold
 
     def scratch_for(self, m, k):
         need = _lib.load().b200_fc_scratch_bytes(m, k)
@@ -60,11 +64,14 @@ class Workspace:
         return self.sdpa_bytes(_lib.load().b200_sdpa_workspace_bytes(b, n, nkv, h, s_max))
 
     def sdpa_bytes(self, need):
+        """The attention buffer, of `need` bytes at least. One that is too small goes back to the allocator, unless a captured
+        call took it: its graph goes on using it, so it stays for as long as the workspace does."""
         if self.sdpa is None or self.sdpa.numel() < need:
-            if self.sdpa is not None:
+            if self.captured:
                 self.outgrown.append(self.sdpa)
-                need = max(need, 2 * self.sdpa.numel())  # (all that is kept stays below the one in use)
+            self.sdpa, self.captured = None, False  # (its memory may serve the larger one)
             self.sdpa = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self.captured = self.captured or torch.cuda.is_current_stream_capturing()
         return self.sdpa
 
     def check_status(self):
