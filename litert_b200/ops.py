@@ -63,9 +63,12 @@ class Workspace:
     def sdpa_for(self, b, n, nkv, h, s_max):
         return self.sdpa_bytes(_lib.load().b200_sdpa_workspace_bytes(b, n, nkv, h, s_max))
 
-    def sdpa_bytes(self, need):
-        """The attention buffer, of `need` bytes at least. One that is too small goes back to the allocator, unless a captured
+    def sdpa_bytes(self, need, device=None):
+        """The attention buffer, of `need` bytes at least, for a call on `device` where that is given. One that is too small goes back to the allocator, unless a captured
         call took it: its graph goes on using it, so it stays for as long as the workspace does."""
+        at = self.device if self.sdpa is None else self.sdpa.device
+        if device is not None and at != device and (at.type, at.index) != (device.type, None):
+            raise B200Error(f"the workspace is on another device: {at}, the call on {device}")
         if self.sdpa is None or self.sdpa.numel() < need:
             if self.captured:
                 self.outgrown.append(self.sdpa)
@@ -525,7 +528,7 @@ def sdpa_decode_int4(q, k_cache, v_cache, k_scale, v_scale, lengths=None, mask=N
     lib = _lib.load()
     need = lib.b200_kv4_sdpa_workspace_bytes(b, t, n, nkv, h, block, s_max, int(scores is not None))
     with torch.cuda.device(q.device):
-        wsb = torch.empty(need, dtype=torch.uint8, device=q.device) if ws is None else ws.sdpa_bytes(need)
+        wsb = torch.empty(need, dtype=torch.uint8, device=q.device) if ws is None else ws.sdpa_bytes(need, q.device)
         _kcheck(lib.b200_kv4_sdpa(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(lengths), _ptr(mask),
                                   _ptr(scores), _ptr(out), b, t, n, nkv, h, block, s_max, _DT[q.dtype],
                                   float(scale) if scale else 0.0, float(logit_cap), _ptr(wsb), wsb.numel(), _stream()))

@@ -80,3 +80,17 @@ def test_growing_calls_hold_one_workspace(ops):
         attend(ops, [x[:b] for x in cache], ws, t=4, scores=scores)
         need = _lib.load().b200_kv4_sdpa_workspace_bytes(b, 4, 4, 2, 64, 64, 9000, 1)
         assert ws.sdpa.numel() == need and not ws.outgrown
+
+
+def test_a_workspace_of_another_device_is_refused(ops, monkeypatch):
+    """The kernel would read and write the other device's addresses. On the CPU, with stand-ins for devices."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    ws = ops.Workspace.__new__(ops.Workspace)
+    ws.device = torch.device("cpu")
+    ws._no_attention_yet()
+    assert ws.sdpa_bytes(100, torch.device("cpu")).numel() == 100
+    with pytest.raises(ops.B200Error, match="device"):
+        ws.sdpa_bytes(100, torch.device("meta"))
+    with pytest.raises(ops.B200Error, match="device"):
+        ws.sdpa_bytes(200, torch.device("meta"))
+    assert ws.sdpa.numel() == 100
