@@ -31,18 +31,18 @@ __device__ __forceinline__ uint32_t operator/(uint32_t n, const Divisor& by) { r
 // fp32, u = the integer nearest to (x - least) / scale (ties to even), clamped to 0 .. 15. Both roundings to fp16 happen
 // before the nibbles are chosen, so that these are the best ones for the pair that is kept.
 // Which integer is nearest is decided exactly: y = (x - least) / (15 scale), clamped for free by the product's saturation,
-// is off by 2^-22 of itself at most, so 15 y by 3.6e-6; only what comes within 1e-5 of a border is looked at again, in 64
-// bits where difference and border are exact.
+// is off by 3 x 2^-23 of itself at most (the reciprocal 2 of them, difference and product half of one each), so 15 y by 5.4e-6;
+// only what comes within 1e-5 of a border is looked at again, against the border itself: least + (k + 1/2) scale is a multiple
+// of 2^-25 below 2^21, exact in 64 bits. (The difference x - least need not be.)
 //
 // Memory-bound by its bytes, but really by instruction issue: 67 M elements at 36 T lane operations per second leave 12
 // operations for each in the time that HBM takes, and it has 19. So 16 channels per thread (block / 16 neighbouring lanes have
 // one block), the minimum and the negated maximum of fp16 rows as one pair of halves, nibbles put together by fused products.
 // 16 x 8192 rows of 256 in fp16: 53 us of the 26 that their bytes take (issue slots 75 % busy); 16 x 4096 in float32 32 of 23.
 __device__ __forceinline__ float nearest_float(float n, float x, float least, float scale) {
-  const double d = (double)x - (double)least;
-  const float below = n * scale > (float)d ? n - 1.0f : n;  // the border lies above it
-  const double border = ((double)below + 0.5) * (double)scale;
-  const float u = d > border ? below + 1.0f : d < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));  // (ties: the even neighbour)
+  const float below = n * scale > x - least ? n - 1.0f : n;  // the border lies above it
+  const double border = (double)least + ((double)below + 0.5) * (double)scale;
+  const float u = x > border ? below + 1.0f : x < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));  // (ties: the even neighbour)
   return fminf(fmaxf(u, 0.0f), 15.0f);
 }
 __device__ __forceinline__ float min_nan(float a, float b) {  // NaN if either is

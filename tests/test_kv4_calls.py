@@ -74,3 +74,35 @@ def test_no_sequence_needs_no_memory():
     assert lib.b200_kv4_sdpa(None, *none, None, None, None, None, 0, 1, 4, 2, 64, 32, 16, 0, 0.0, 0.0, None, 0, None) == 0
     assert lib.b200_kv4_evict(*none, 0, 16, 2, 64, 32, None, None, 4, 0, 0, *none, 16, None, None, None, None) == 0
     assert lib.b200_kv4_append(None, None, 0, 0, 0, 0, 0, None, None, 0, 1, 2, 80, 32, 16, *none, None) != 0  # (checked all the same)
+
+
+def exact_nibbles(x, scale, least):
+    """The integers nearest to (x - least) / scale in rational arithmetic, ties to even, clamped."""
+    from fractions import Fraction
+
+    s, m = Fraction(float(scale)), Fraction(float(least))
+    return [max(0, min(15, round((Fraction(float(v)) - m) / s))) for v in x]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block", [32, 64])
+def test_the_nearest_nibble_is_exact_for_elements_of_any_size(ops, path, block):
+    """float32 elements next to a border of which the difference to the least value does not fit 64 bits: tiny ones where a
+    border is zero, and neighbours of every border."""
+    import numpy as np
+
+    rng = np.random.default_rng(block)
+    rows = []
+    for least, scale in ((-1.0, 2.0), (-3.0, 2.0), (-0.25, 0.5), (-29.0, 2.0), (-1000.0, 80.0), (-2.0 ** -10, 2.0 ** -9)):
+        tiny = np.float32([0.0, 1e-30, -1e-30, 1e-45, -1e-45, 1e-38, -1e-38, 1e-20, -1e-20, 1e-12, -1e-12, 1e-9, -1e-9])
+        edges = np.float32([least + scale * (k + 0.5) for k in range(15)])
+        near = np.concatenate([edges, np.nextafter(edges, np.float32(np.inf)), np.nextafter(edges, np.float32(-np.inf))])
+        for part in (np.resize(tiny, block - 2), rng.choice(near, block - 2), rng.choice(near, block - 2)):
+            rows.append(np.concatenate([np.float32([least, least + 15 * scale]), part]))
+    x = torch.from_numpy(np.stack(rows).astype(np.float32))[None, :, None].cuda()
+    cache = ops.int4_kv_cache(1, len(rows), 1, block, block)
+    ops.kv_append_int4(x, x, torch.zeros(1, dtype=torch.int32, device="cuda"), *cache)
+    nibbles, pairs = cache[0][0, :, 0].cpu().numpy(), cache[2][0, :, 0, 0].cpu().numpy()
+    got = np.stack((nibbles & 15, nibbles >> 4), -1).reshape(len(rows), block)
+    for i, row in enumerate(rows):
+        assert got[i].tolist() == exact_nibbles(row, pairs[i, 0], pairs[i, 1]), i
