@@ -380,7 +380,8 @@ PyObject* kv_evict_int4(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     In scores(a[4], at::kFloat), lengths(a[5], at::kInt);
     int budget, sinks, recent;
     if (!c.ok || !to.ok || to.b != c.b || to.nkv != c.nkv || to.h != c.h || to.block != c.block || !c.here(scores) || !c.per_sequence(lengths) ||
-        scores.t->sizes() != at::IntArrayRef{c.b, c.nkv, c.s} || !as_int(a[6], &budget) || !as_int(a[7], &sinks) || !as_int(a[8], &recent) || budget <= 0)
+        scores.t->sizes() != at::IntArrayRef{c.b, c.nkv, c.s} || !as_int(a[6], &budget) || !as_int(a[7], &sinks) || !as_int(a[8], &recent) || budget <= 0 ||
+        budget > to.s)
       Py_RETURN_NONE;
     const at::Device d = c.k.t->device();
     at::Tensor kept(at::detail::empty_cuda(std::array<int64_t, 3>{c.b, c.nkv, budget}, at::kInt, d, std::nullopt)),

@@ -106,3 +106,16 @@ def test_the_nearest_nibble_is_exact_for_elements_of_any_size(ops, path, block):
     got = np.stack((nibbles & 15, nibbles >> 4), -1).reshape(len(rows), block)
     for i, row in enumerate(rows):
         assert got[i].tolist() == exact_nibbles(row, pairs[i, 0], pairs[i, 1]), i
+
+
+@pytest.mark.gpu
+def test_a_budget_beyond_the_slots_is_refused_before_memory_is_taken(ops, path):
+    cache = ops.int4_kv_cache(2, 16, 2, 64)
+    scores, at = torch.zeros((2, 2, 16), device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    for budget in (17, 1 << 28):
+        with pytest.raises(ops.B200Error, match="budget"):
+            ops.kv_evict_int4(*cache, scores, at, budget)
+    assert torch.cuda.max_memory_allocated() == before
