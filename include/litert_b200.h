@@ -378,7 +378,7 @@ B200_API int b200_widen_i32_to_i64(const int32_t* d_in, int64_t* d_out, int n, v
  *           of b200_pack_w4's elements), on a 16-byte boundary;
  *   pairs   fp16 [b, s_max, nkv, h / block, 2]: scale and least value of each block of 32
  *           or 64 channels; nibble u stands for scale * u + least. On a 4-byte boundary.
- * h is a multiple of the block, at most 512. All calls: b = 0 or no tokens do nothing. */
+ * h is a multiple of the block, at most 512; s_max at most 2^30. All calls: b = 0 or no tokens do nothing. */
 B200_API const char* b200_kv4_last_error(void);
 
 /* Quantizes t tokens per sequence and stores them: token i of sequence b goes to slot

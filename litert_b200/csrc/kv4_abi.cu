@@ -25,13 +25,15 @@ int done(cudaError_t e, const char* what) {
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-// The cache's shape and tensors. Row indexes of the kernels' grids are 32 bits, offsets 64.
+// The cache's shape and tensors. Row indexes of the kernels' grids are 32 bits, offsets 64; slots are counted in 32 bits, up to
+// a cluster's threads past the last.
 int check_cache(const char* name, const void* k, const void* v, const void* kp, const void* vp, int b, int s, int nkv, int h, int block) {
   if (b != 0 && (!k || !v || !kp || !vp)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: a cache tensor is null", name);
   if (b < 0 || s <= 0 || nkv <= 0 || h <= 0)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: bad cache shape b=%d s=%d nkv=%d h=%d", name, b, s, nkv, h);
   if ((block != 32 && block != 64) || h % block != 0 || h > 512)
     return fail(B200_ERR_UNSUPPORTED, "%s: blocks of 32 or 64 channels that divide a head size up to 512 (block %d, head size %d)", name, block, h);
+  if (s > 1 << 30) return fail(B200_ERR_UNSUPPORTED, "%s: at most 2^30 slots, got %d", name, s);
   if (b > 65535 || nkv > 65535) return fail(B200_ERR_UNSUPPORTED, "%s: at most 65535 sequences and KV heads", name);
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(kp, 4) || !aligned(vp, 4))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: nibbles lie on 16-byte boundaries, pairs on 4-byte boundaries", name);

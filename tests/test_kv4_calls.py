@@ -119,3 +119,24 @@ def test_a_budget_beyond_the_slots_is_refused_before_memory_is_taken(ops, path):
         with pytest.raises(ops.B200Error, match="budget"):
             ops.kv_evict_int4(*cache, scores, at, budget)
     assert torch.cuda.max_memory_allocated() == before
+
+
+def test_caches_beyond_the_kernels_indexes_are_refused():
+    """Slots are walked over in 32-bit integers, some hundreds at a time past the last. Refused on the host, on the CPU."""
+    from litert_b200 import _lib, build
+
+    build.build_kernels()
+    lib = _lib.load()
+    p = 1 << 20
+    cache = (p, 2 * p, 3 * p, 4 * p)
+    for s in (2 ** 31 - 1, 2 ** 30 + 1):
+        calls = [
+            lib.b200_kv4_append(p, p, 0, 0, 0, 0, 0, p, None, 1, 1, 1, 32, 32, s, *cache, None),
+            lib.b200_kv4_read(*cache, 1, s, 1, 32, 32, None, None, 1, 0, p, p, None),
+            lib.b200_kv4_sdpa(p, *cache, None, None, None, p, 1, 1, 1, 1, 32, 32, s, 0, 0.0, 0.0, p, 1 << 62, None),
+            lib.b200_kv4_sdpa(p, *cache, None, None, None, p, 1, 1, 1, 1, 64, 32, s, 0, 0.0, 0.0, p, 1 << 62, None),
+            lib.b200_kv4_evict(*cache, 1, s, 1, 32, 32, p << 10, p << 11, 4, 0, 0, *cache, s, p << 12, p << 13, p << 14, None),
+            lib.b200_kv4_evict(*cache, 1, 64, 1, 32, 32, p << 10, p << 11, 4, 0, 0, p << 20, p << 22, p << 24, p << 26, s, p << 12, p << 30, p << 14, None),
+        ]
+        assert calls == [4] * 6, (s, calls)
+        assert b"slots" in lib.b200_kv4_last_error()
