@@ -366,16 +366,19 @@ __device__ __forceinline__ uint32_t piece_at(int row, int c) {
 // has 1.2e-6; + 0.3 us at 4 x 2000).
 // Value nibbles are centred, u - 8, by way of the exponents that make a nibble's place the unit (1024) or an eighth of it
 // (64): sums of weights times values that are all positive lose to the tensor core's truncation (float32 outputs were
-// 3e-5 off; 8 x scale joins the least value instead).
+// 3e-5 off; 8 x scale joins the least value instead). For fp16 queries and 256 channels that costs nothing but a mask: a nibble
+// as the subnormal number again for half of the slots, u w, and its complement with the other sign for the other half, -(15 - u) w,
+// are a sum about zero too, and 15 x scale joins the least value of the second half only (64 x 32768 of 8 heads x 256, replayed:
+// 83.5 -> 76.8 us; 16 x 8192 16.4 -> 15.9; 16 heads of 128 over 2 with scores 21.1 -> 21.6, in 128 registers, so not those).
 // A weight times a value scale is two fp16 numbers, 22 bits, for either type of query. As one number it is off by 2^-12 on
-// average, times |u - 8| x scale: outputs 2.8e-4 off 64 bits where an fp16 output's own rounding is 2.1e-4. The second number's
-// products cost 64 x 32768 of 8 heads x 256 71.7 -> 82.1 us replayed, 16 x 8192 15.5 -> 16.2.
+// average, times |u - 8| x scale: outputs 2.8e-4 off 64 bits where an fp16 output's own rounding is 2.1e-4. (With the
+// unit below: 64 x 32768 71.5 -> 76.8 us, 16 x 8192 15.4 -> 15.9.)
 // What a second number leaves is 2^-25 at least, fp16's last place, however small the product. So a row's weights are counted in
 // units of 2^-units such that the largest product of a weight and a scale so far lies in 2^9 .. 2^10, up to 60000 before that is
 // put right: rescaling the outputs at every new maximum would happen in most tiles while a warp has seen few. The unit goes by
 // what slots contribute, not by their scales alone, so hidden slots, and slots or tiles that end up without weight, do not coarsen
 // the others. A scale of zero counts as kLeastScale, which keeps the weights themselves within fp32.
-// Beside a unit of the largest scale: 64 x 32768 82.1 -> 83.5 us replayed, 16 x 8192 16.2 -> 16.5.
+// A unit of the largest scale took 1.4 us less at 64 x 32768, 0.2 at 16 x 8192.
 constexpr float kMostOperand = 60000.0f, kLeastScale = 0x1p-40f, kMostUnits = 49.0f;
 constexpr int kUnitBits = 9;
 constexpr uint32_t kLowNibbles = 0x000f000fu, kHighNibbles = 0x00f000f0u;
@@ -423,6 +426,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
   constexpr int P = H / 32;         // 16-byte pieces of a row
   constexpr int kPer = BLOCK / 32;  // of them in a block
   constexpr int kWarps = T::kWarps;
+  constexpr bool kComplement = !QF32 && H == 256;  // (see Centred)
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
   __shared__ int s_pair[kWarps];                       // whose the warps' states are
@@ -874,11 +878,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
           for (int j = 0; j < 4; ++j) {
             const uint32_t bits = lds32(pairs_at + T::kPairBytes + (uint32_t)(((2 * t + (j & 1) + 8 * (j >> 1)) * G + gr) * 4));
             const float2 f = pair_floats(bits);
-            ps[j] = pw[j] * f.x;
+            ps[j] = kComplement && j >= 2 ? -pw[j] * f.x : pw[j] * f.x;
             if (careful && pw[j] == 0.0f) {
               ps[j] = 0.0f;
             } else {
-              least_sum[gr] = fmaf(pw[j], fmaf(8.0f, f.x, f.y), least_sum[gr]);
+              least_sum[gr] = fmaf(pw[j], kComplement && j < 2 ? f.y : fmaf(kComplement ? 15.0f : 8.0f, f.x, f.y), least_sum[gr]);
             }
           }
           split_halves(ps[0], ps[1], high[0], low[0]);
@@ -889,7 +893,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t a = j ? words[2 * (i & 1)] >> 8 : words[2 * (i & 1)], c = j ? words[2 * (i & 1) + 1] >> 8 : words[2 * (i & 1) + 1];
-          e[j][0] = centred.low(a), e[j][1] = centred.high(a), e[j][2] = centred.low(c), e[j][3] = centred.high(c);
+          if constexpr (kComplement) {
+            e[j][0] = a & kLowNibbles, e[j][1] = a & kHighNibbles, e[j][2] = ~c & kLowNibbles, e[j][3] = ~c & kHighNibbles;
+          } else {
+            e[j][0] = centred.low(a), e[j][1] = centred.high(a), e[j][2] = centred.low(c), e[j][3] = centred.high(c);
+          }
         }
         product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], high[0], high[1]);
         product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], high[0], high[1]);
@@ -903,6 +911,7 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     }
     cp_async_wait<0>();
 
+    constexpr float kLowUnits = kComplement ? 0x1p24f : 1.0f, kHighUnits = kComplement ? 0x1p20f : 1.0f;
     // -- the warp's state, as a record: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
     const float from_units[2] = {__int_as_float((127 - (int)units[0]) << 23), __int_as_float((127 - (int)units[1]) << 23)};
     float* state = reinterpret_cast<float*>(smem + w * T::kWarpBytes);
@@ -922,8 +931,8 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<float4*>(state + (2 * t + e) * T::kRec + i * 32 + g * 4) =
-              make_float4((o[i][0][e] + least[e]) * from_units[e], (o[i][0][2 + e] + least[e]) * from_units[e],
-                          (o[i][1][e] + least[e]) * from_units[e], (o[i][1][2 + e] + least[e]) * from_units[e]);
+              make_float4(fmaf(o[i][0][e], kLowUnits, least[e]) * from_units[e], fmaf(o[i][0][2 + e], kHighUnits, least[e]) * from_units[e],
+                          fmaf(o[i][1][e], kLowUnits, least[e]) * from_units[e], fmaf(o[i][1][2 + e], kHighUnits, least[e]) * from_units[e]);
     }
     if (g < 2) {
       s_m[w][2 * t + g] = g ? m_run[1] : m_run[0];
