@@ -1098,13 +1098,14 @@ __device__ void kv4_add_scores(const Kv4Sdpa& p, const Kv4Cut& cut, const Kv4Row
 
 // Merges the records of one query row, H >> part_log2 channels per CTA. What it costs are its start and L2 round trips, so
 // there is one for all records up to 32 (12 for fp16 rows of 256; twice and four times as many where the channels are parted),
-// requested before their weights are known. fp16 rows: 64 registers, so that more CTAs are resident (64 x 32768: 78.2 -> 77.3 us,
-// drafts 8 x 4096 17.9 -> 17.7; float32 rows 4 x 2000 11.3 -> 11.7, so not those. The main kernel at 224 registers, to leave room
-// for these CTAs beside it: 82.6).
+// requested before their weights are known. fp16 rows of up to 128 channels: 64 registers, so that more CTAs, those of the
+// scores too, are resident (16 heads of 128 over 2 with scores, 16 x 8192: 22.6 -> 21.2 us; of 256 channels 15.2 -> 16.0 without scores, and
+// 64 x 32768 75.9 -> 76.7, so not those). (The main kernel at 224 registers, to leave room for these CTAs beside it: 82.6 us where
+// it took 78 at 64 x 32768.)
 // The CTAs behind the first `merge_ctas` of a sequence add to the scores.
 template <int H, bool QF32>
-__global__ void __launch_bounds__(kMergeThreads, QF32 ? 1 : 8) kv4_merge_kernel(const Kv4Sdpa p, const int ctas, const int merge_ctas, const int part_log2,
-                                                                  const float2* stats_ws, const float* logits_ws) {
+__global__ void __launch_bounds__(kMergeThreads, QF32 || H == 256 ? 1 : 8) kv4_merge_kernel(const Kv4Sdpa p, const int ctas, const int merge_ctas, const int part_log2,
+                                                                 const float2* stats_ws, const float* logits_ws) {
   constexpr int kRec = H + 4, kBatch = H == 256 && !QF32 ? 6 : H / 16;
   __shared__ float4 s_part[kMergeThreads];
   __shared__ float s_sum[kMergeThreads];
