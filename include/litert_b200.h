@@ -371,8 +371,8 @@ B200_API int b200_widen_i32_to_i64(const int32_t* d_in, int64_t* d_out, int n, v
 
 /* ---- key/value cache in 4 bits ----------------------------------------------------
  * No counterpart in the reference, whose caches are float32 (odml.update_kv_cache,
- * tflite/experimental/genai/kvcache.cc:230-340): half the bytes of an int8 cache for a
- * decode step that is bound by them. Keys and values each are two tensors, token-major
+ * tflite/experimental/genai/kvcache.cc:230-340): 0.28 to 0.31 of an fp16 cache's bytes, 0.55 to
+ * 0.62 of an int8 one's, for decode steps that are bound by them or by memory. Keys and values each are two tensors, token-major
  * like the other caches here:
  *   nibbles uint8 [b, s_max, nkv, h / 2], channel 2 i in the low half of byte i (the order
  *           of b200_pack_w4's elements), on a 16-byte boundary;
@@ -410,7 +410,8 @@ B200_API int b200_kv4_read(const void* d_k_cache, const void* d_v_cache, const v
  * d_scores [b, nkv, s_max] f32 (optional): += the softmax weights that each slot got from its KV
  * head's n / nkv * t queries (what b200_kv4_evict ranks by); slots beyond the length are left
  * alone. Any number of query heads per KV head. Queries and workspace lie on 16-byte boundaries;
- * the workspace needs no initial contents. */
+ * the workspace needs no initial contents. It has 32 bytes per slot for every eight query rows of
+ * every KV head where d_scores is given. Products and sums keep float32's precision for either type. */
 B200_API size_t b200_kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int block, int s_max, int with_scores);
 B200_API int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache, const void* d_k_scale,
                            const void* d_v_scale, const int32_t* d_lengths, const float* d_mask, float* d_scores, void* d_out,

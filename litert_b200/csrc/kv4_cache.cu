@@ -196,8 +196,9 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const Kv4Append
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------
-// A thread takes two words of nibbles, 256 apart, so that a warp's stores are whole lines. fp16 values are fused products
-// of halves: one rounding. Bound by HBM: 16 x 8192 rows of 256 as fp16 29.3 us (26 for the bytes), 16 x 4096 as float32 35 (23).
+// A thread takes two words of nibbles, 256 apart, so that a warp's stores of fp16 rows are whole lines. fp16 values are fused
+// products of halves: one rounding. fp16 is bound by HBM: 16 x 8192 rows of 256 29.3 us (26 for the bytes). float32 is not: a lane's
+// two stores of 16 bytes lie 32 apart from its neighbour's, so each fills half of every sector; 16 x 4096 rows 35 us (23).
 template <bool F32>
 __global__ void __launch_bounds__(kRowThreads) kv4_read_kernel(const Kv4Read p, const uint32_t items, const Divisor per_token, const int words_log2) {
   pdl_enter();
