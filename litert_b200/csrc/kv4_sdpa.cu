@@ -318,6 +318,27 @@ __device__ __forceinline__ void first_product(float (&d)[4], uint32_t a0, uint32
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
+// Two floats as one operand.
+__device__ __forceinline__ uint64_t packed(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpacked(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // p + j * step in one instruction.
 __device__ __forceinline__ const void* advance(const void* p, int j, uint32_t step) {
   uint64_t r;
@@ -366,13 +387,16 @@ __device__ __forceinline__ uint32_t piece_at(int row, int c) {
 // has 1.2e-6; + 0.3 us at 4 x 2000).
 // Value nibbles are centred, u - 8, by way of the exponents that make a nibble's place the unit (1024) or an eighth of it
 // (64): sums of weights times values that are all positive lose to the tensor core's truncation (float32 outputs were
-// 3e-5 off; 8 x scale joins the least value instead). For fp16 queries and 256 channels that costs nothing but a mask: a nibble
-// as the subnormal number again for half of the slots, u w, and its complement with the other sign for the other half, -(15 - u) w,
-// are a sum about zero too, and 15 x scale joins the least value of the second half only (64 x 32768 of 8 heads x 256, replayed:
-// 83.5 -> 76.8 us; 16 x 8192 16.4 -> 15.9; 16 heads of 128 over 2 with scores 21.1 -> 21.6, in 128 registers, so not those).
+// 3e-5 off; 8 x scale joins the least value instead).
 // A weight times a value scale is two fp16 numbers, 22 bits, for either type of query. As one number it is off by 2^-12 on
-// average, times |u - 8| x scale: outputs 2.8e-4 off 64 bits where an fp16 output's own rounding is 2.1e-4. (With the
-// unit below: 64 x 32768 71.5 -> 76.8 us, 16 x 8192 15.4 -> 15.9.)
+// average, times |u - 8| x scale: outputs 2.8e-4 off 64 bits where an fp16 output's own rounding is 2.1e-4.
+// A tile's sums begin at zero, the second numbers' products first, and are added in fp32 with rounding. In the tensor core's
+// accumulators every product would cut off the sum of all tiles before it: 1.5e-6 off after a tile, 1.4e-5 after 65, 2e-5 after 256
+// (float32 queries, normal values; now 0.6e-6 and 1.2 .. 1.5e-6, plain float32 0.4e-6), ten times that in one direction where
+// nibbles are only positive. (64 x 32768 of 8 heads x 256, replayed: one number each 71.5 us, with a second one and the unit below
+// 83.5, with the sums 86.4; 16 x 8192 15.4, 16.4, 15.8. Half of the slots as complements, 15 - u, to save the centring: 75.9 and
+// 85.5 us, but sums about zero only if both halves have weight: 3e-4 off behind a mask that hides one. Uncentred, with - 8 w as
+// the sums' beginning: 91.6.)
 // What a second number leaves is 2^-25 at least, fp16's last place, however small the product. So a row's weights are counted in
 // units of 2^-units such that the largest product of a weight and a scale so far lies in 2^9 .. 2^10, up to 60000 before that is
 // put right: rescaling the outputs at every new maximum would happen in most tiles while a warp has seen few. The unit goes by
@@ -426,7 +450,6 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
   constexpr int P = H / 32;         // 16-byte pieces of a row
   constexpr int kPer = BLOCK / 32;  // of them in a block
   constexpr int kWarps = T::kWarps;
-  constexpr bool kComplement = !QF32 && H == 256;  // (see Centred)
   extern __shared__ uint8_t kv4_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_smem_raw) + 127) & ~uintptr_t(127));
   __shared__ int s_pair[kWarps];                       // whose the warps' states are
@@ -669,13 +692,14 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     float* logits = logits_ws ? logits_ws + (size_t)pair * ((size_t)tiles_of(s_max) * kSlots * 8) : nullptr;
 
     // outputs: of piece i and its channels 4 g + {0, 1} and 4 g + {2, 3}, rows 2 t and 2 t + 1
-    float o[P][2][4], least_sum[G];
+    uint64_t o[P][2][2];  // pairs of rows
+    float least_sum[G];
 #pragma unroll
     for (int gr = 0; gr < G; ++gr) least_sum[gr] = 0.0f;
 #pragma unroll
     for (int i = 0; i < P; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][0][e] = o[i][1][e] = 0.0f;
+      for (int e = 0; e < 2; ++e) o[i][0][e] = o[i][1][e] = packed(0.0f, 0.0f);
     // the rows' weights are e^(x - m_run) in units of 2^-units (integers; see kMostUnits). The first x that is a number makes a
     // weight of infinity, or, at the type's lowest value, of one: m_run need not be the largest x.
     float m_run[2] = {-FLT_MAX, -FLT_MAX}, l_run[2] = {0.0f, 0.0f}, units[2] = {kMostUnits, kMostUnits};
@@ -844,10 +868,9 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
         l_run[1] *= alpha[1];
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) least_sum[gr] *= mine_alpha;
+        const uint64_t both = packed(alpha[0], alpha[1]);
 #pragma unroll
-        for (int i = 0; i < 2 * P; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[i >> 1][i & 1][e] *= alpha[e & 1];
+        for (int i = 0; i < 4 * P; ++i) o[i >> 2][(i >> 1) & 1][i & 1] = mul2(o[i >> 2][(i >> 1) & 1][i & 1], both);
       }
       // slots by rows -> rows by slots: row g, slots 2 t, 2 t + 1, 2 t + 8, 2 t + 9
       float pw[4];
@@ -878,11 +901,11 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
           for (int j = 0; j < 4; ++j) {
             const uint32_t bits = lds32(pairs_at + T::kPairBytes + (uint32_t)(((2 * t + (j & 1) + 8 * (j >> 1)) * G + gr) * 4));
             const float2 f = pair_floats(bits);
-            ps[j] = kComplement && j >= 2 ? -pw[j] * f.x : pw[j] * f.x;
+            ps[j] = pw[j] * f.x;
             if (careful && pw[j] == 0.0f) {
               ps[j] = 0.0f;
             } else {
-              least_sum[gr] = fmaf(pw[j], kComplement && j < 2 ? f.y : fmaf(kComplement ? 15.0f : 8.0f, f.x, f.y), least_sum[gr]);
+              least_sum[gr] = fmaf(pw[j], fmaf(8.0f, f.x, f.y), least_sum[gr]);
             }
           }
           split_halves(ps[0], ps[1], high[0], low[0]);
@@ -893,16 +916,16 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t a = j ? words[2 * (i & 1)] >> 8 : words[2 * (i & 1)], c = j ? words[2 * (i & 1) + 1] >> 8 : words[2 * (i & 1) + 1];
-          if constexpr (kComplement) {
-            e[j][0] = a & kLowNibbles, e[j][1] = a & kHighNibbles, e[j][2] = ~c & kLowNibbles, e[j][3] = ~c & kHighNibbles;
-          } else {
-            e[j][0] = centred.low(a), e[j][1] = centred.high(a), e[j][2] = centred.low(c), e[j][3] = centred.high(c);
-          }
+          e[j][0] = centred.low(a), e[j][1] = centred.high(a), e[j][2] = centred.low(c), e[j][3] = centred.high(c);
         }
-        product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], high[0], high[1]);
-        product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], high[0], high[1]);
-        product(o[i][0], e[0][0], e[0][1], e[0][2], e[0][3], low[0], low[1]);
-        product(o[i][1], e[1][0], e[1][1], e[1][2], e[1][3], low[0], low[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float sum[4];
+          first_product(sum, e[j][0], e[j][1], e[j][2], e[j][3], low[0], low[1]);
+          product(sum, e[j][0], e[j][1], e[j][2], e[j][3], high[0], high[1]);
+          o[i][j][0] = add2(o[i][j][0], packed(sum[0], sum[1]));
+          o[i][j][1] = add2(o[i][j][1], packed(sum[2], sum[3]));
+        }
       }
       at = next_at;
 #pragma unroll
@@ -911,7 +934,6 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
     }
     cp_async_wait<0>();
 
-    constexpr float kLowUnits = kComplement ? 0x1p24f : 1.0f, kHighUnits = kComplement ? 0x1p20f : 1.0f;
     // -- the warp's state, as a record: thread (g, t) has channels 4 g .. 4 g + 3 of every piece for rows 2 t and 2 t + 1 --
     const float from_units[2] = {__int_as_float((127 - (int)units[0]) << 23), __int_as_float((127 - (int)units[1]) << 23)};
     float* state = reinterpret_cast<float*>(smem + w * T::kWarpBytes);
@@ -927,12 +949,14 @@ __global__ void __launch_bounds__(Kv4Tile<H, BLOCK, QF32>::kThreads, 1) kv4_sdpa
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       const float least[2] = {__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4)};
 #pragma unroll
-      for (int i = gr * kPer; i < (gr + 1) * kPer; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float4*>(state + (2 * t + e) * T::kRec + i * 32 + g * 4) =
-              make_float4(fmaf(o[i][0][e], kLowUnits, least[e]) * from_units[e], fmaf(o[i][0][2 + e], kHighUnits, least[e]) * from_units[e],
-                          fmaf(o[i][1][e], kLowUnits, least[e]) * from_units[e], fmaf(o[i][1][2 + e], kHighUnits, least[e]) * from_units[e]);
+      for (int i = gr * kPer; i < (gr + 1) * kPer; ++i) {
+        const float2 c0 = unpacked(o[i][0][0]), c1 = unpacked(o[i][0][1]), c2 = unpacked(o[i][1][0]), c3 = unpacked(o[i][1][1]);
+        float* to_state = state + 2 * t * T::kRec + i * 32 + g * 4;
+        *reinterpret_cast<float4*>(to_state) = make_float4((c0.x + least[0]) * from_units[0], (c1.x + least[0]) * from_units[0],
+                                                           (c2.x + least[0]) * from_units[0], (c3.x + least[0]) * from_units[0]);
+        *reinterpret_cast<float4*>(to_state + T::kRec) = make_float4((c0.y + least[1]) * from_units[1], (c1.y + least[1]) * from_units[1],
+                                                                     (c2.y + least[1]) * from_units[1], (c3.y + least[1]) * from_units[1]);
+      }
     }
     if (g < 2) {
       s_m[w][2 * t + g] = g ? m_run[1] : m_run[0];

@@ -274,3 +274,28 @@ def test_attention_is_exact_over_values_of_any_size(ops, ws, h, block, f32):
     got = ops.sdpa_decode_int4(q, *cache, ws=ws)
     wrong = near(got.unflatten(-1, (-1, block)), want.unflatten(-1, (-1, block)))
     assert wrong is None, wrong
+
+
+@pytest.mark.parametrize("n,nkv,h,block", [(8, 1, 256, 64), (4, 1, 256, 32), (8, 2, 128, 32), (8, 4, 64, 64)])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("kind", ["normal", "outlier", "halves"])
+def test_sums_over_many_tiles_stay_exact(ops, ws, n, nkv, h, block, f32, kind):
+    """A large batch, of which one warp walks through a hundred tiles of 16 slots and more: normal values; one large channel per
+    block, beside which all others have small nibbles; a mask that hides the second half of every tile."""
+    b, s = 300, 4096
+    cache, g = filled(ops, 3, 2, s, nkv, h, block)
+    if kind == "outlier":
+        v = torch.randn((2, s, nkv, h), generator=g, device="cuda")
+        v.unflatten(-1, (-1, block))[..., 3] = 20.0
+        cache[1][:], cache[3][:] = quantized(v, block)
+    mask = None
+    if kind == "halves":
+        mask = torch.zeros((2, 1, 1, s), device="cuda")
+        mask[..., torch.arange(s, device="cuda") % 16 >= 8] = -math.inf
+    q = 0.5 * torch.randn((2, 1, n, h), generator=g, device="cuda")
+    q = q if f32 else q.half()
+    want, _ = attention64(q, cache, mask=mask)
+    many = lambda x: None if x is None else x.repeat(b // 2, *[1] * (x.dim() - 1))  # noqa: E731
+    got = ops.sdpa_decode_int4(many(q), *[many(x) for x in cache], mask=many(mask), ws=ws)
+    wrong = near(got, many(want))
+    assert wrong is None, wrong
