@@ -411,7 +411,8 @@ B200_API int b200_kv4_read(const void* d_k_cache, const void* d_v_cache, const v
  * head's n / nkv * t queries (what b200_kv4_evict ranks by); slots beyond the length are left
  * alone. Any number of query heads per KV head. Queries and workspace lie on 16-byte boundaries;
  * the workspace needs no initial contents. It has 32 bytes per slot for every eight query rows of
- * every KV head where d_scores is given. Products and sums keep float32's precision for either type. */
+ * every KV head where d_scores is given. For either type products and sums keep float32's precision
+ * beside a row's largest values (those of a block 2^16 times smaller lose bits). */
 B200_API size_t b200_kv4_sdpa_workspace_bytes(int b, int t, int n, int nkv, int h, int block, int s_max, int with_scores);
 B200_API int b200_kv4_sdpa(const void* d_q, const void* d_k_cache, const void* d_v_cache, const void* d_k_scale,
                            const void* d_v_scale, const int32_t* d_lengths, const float* d_mask, float* d_scores, void* d_out,

@@ -1123,8 +1123,8 @@ __device__ void kv4_add_scores(const Kv4Sdpa& p, const Kv4Cut& cut, const Kv4Row
 // Merges the records of one query row, H >> part_log2 channels per CTA. What it costs are its start and L2 round trips, so
 // there is one for all records up to 32 (12 for fp16 rows of 256; twice and four times as many where the channels are parted),
 // requested before their weights are known. fp16 rows of up to 128 channels: 64 registers, so that more CTAs, those of the
-// scores too, are resident (16 heads of 128 over 2 with scores, 16 x 8192: 22.6 -> 21.2 us; of 256 channels 15.2 -> 16.0 without scores, and
-// 64 x 32768 75.9 -> 76.7, so not those). (The main kernel at 224 registers, to leave room for these CTAs beside it: 82.6 us where
+// scores too, are resident (16 heads of 128 over 2 with scores, 16 x 8192: 1.4 us less of 22.6; of 256 channels 0.8 more of 15.2 without
+// scores, and 0.8 more at 64 x 32768, so not those). (The main kernel at 224 registers, to leave room for these CTAs beside it: 82.6 us where
 // it took 78 at 64 x 32768.)
 // The CTAs behind the first `merge_ctas` of a sequence add to the scores.
 template <int H, bool QF32>
